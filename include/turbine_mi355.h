@@ -161,6 +161,32 @@ int mi355_flash_attn_fwd_strided_bf16(const void* q, const void* k, const void* 
                                       float scale, int is_causal, int variant, void* stream);
 
 /*
+ * Flash-attention forward over packed sequences of different lengths: sequence s owns the rows
+ * [cu_seqlens_q[s], cu_seqlens_q[s+1]) of q and o and the rows [cu_seqlens_k[s], cu_seqlens_k[s+1]) of k and v, and
+ * attends to nothing else.  O = softmax(scale . Q K^T [+ causal mask]) V per sequence; is_causal: query i of a sequence
+ * sees its keys j <= i + (len_k - len_q) (lower-right aligned, as in mi355_flash_attn_fwd).  A query with no visible key
+ * gives zeros.
+ * q, o: [total_q, H, 128]; k, v: [total_k, Hkv, 128], H % Hkv == 0 (query head h reads K/V head h / (H / Hkv)), all
+ * dtype (MI355_F16 | MI355_BF16); *_strides: {token, head} in elements, multiples of 8, token strides in [128, 2^24)
+ * (slices of a packed QKV projection are read in place); q, k, v may broadcast a head with stride 0.
+ * cu_seqlens_q, cu_seqlens_k: int32 [num_seqs + 1] in device memory, non-decreasing; offsets outside [0, total] are cut to it,
+ * and a sequence that ends before it begins is empty, so no contents make the kernel leave its operands.  Lengths are
+ * read on the device only: nothing has to be known on the host, and a captured launch serves any lengths.
+ * Rows of o outside every sequence are left as they are; with zero_rest != 0 those in front of the first and behind
+ * the last sequence are set to zero.  total_q, total_k <= 2^24, num_seqs <= 65535.
+ * A weight of zero times a non-finite V row of the same sequence is NaN, as in the formula.
+ * Replaces: the SDPA root of mi355_flash_attn_fwd for a ragged batch, which the reference can only pad
+ * (tests/dynamo/llama_test.py:285-290 builds one rectangular mask).
+ */
+int mi355_flash_attn_varlen_fwd(const void* q, const void* k, const void* v, void* o,
+                                const int32_t* cu_seqlens_q, const int32_t* cu_seqlens_k,
+                                int64_t num_seqs, int64_t total_q, int64_t total_k,
+                                int64_t H, int64_t Hkv, int64_t D,
+                                const int64_t* q_strides, const int64_t* k_strides,
+                                const int64_t* v_strides, const int64_t* o_strides,
+                                float scale, int is_causal, int zero_rest, int dtype, void* stream);
+
+/*
  * Paged GQA decode attention, one query token per sequence.
  * q:           [num_seqs, num_q_heads, D]                 fp16
  * k_cache,
@@ -328,6 +354,103 @@ int mi355_paged_prefill_attn_bf16(const void* q, const void* k_cache, const void
                                   int64_t num_seqs, int64_t num_new, int64_t num_q_heads,
                                   int64_t num_kv_heads, int64_t D, int64_t page_size,
                                   int64_t max_pages_per_seq, int64_t num_pages, float scale, void* stream);
+
+/*
+ * Attention of drafted token trees over a paged KV cache (the target model's step of speculative decoding): the last
+ * num_nodes tokens of every sequence are its drafts, node n at position seq_lens[s] - num_nodes + n, their K/V in the cache
+ * already.  Node n's query sees every token in front of the drafts, itself and its ancestors.
+ * q, out:      [num_seqs, num_nodes, num_q_heads, D]      dtype (MI355_F16 | MI355_BF16)
+ * k_cache,
+ * v_cache:     [num_pages, page_size, num_kv_heads, D]    dtype
+ * block_table: [num_seqs, max_pages_per_seq] int32; ids outside [0, num_pages): those tokens are dropped
+ * seq_lens:    [num_seqs] int32, cut to [0, max_pages_per_seq * page_size]; shorter than num_nodes: the first nodes are not
+ *              in the cache and nobody sees them
+ * parents:     [num_seqs, num_nodes] int32; a value outside [0, n) for node n: it has no ancestors (a root)
+ * A query that sees nothing gives zeros.  1 <= num_nodes <= 64, num_q_heads / num_kv_heads <= 128, D == 128, page_size 16, 32, 64,
+ * 128 or 256, 1 <= num_splits <= 1024.  A chain (parents[n] = n - 1) is the causal mask among the drafts.
+ * num_splits cuts the table's reach into that many chunks, each by its own workgroups; num_splits > 1 needs
+ * part_acc [num_seqs, num_nodes, num_q_heads, num_splits, D] and part_ml [.., num_splits, 2], fp32, written before they are
+ * read in the same call.  No counterpart in the reference; the mask generalises tests/dynamo/llama_test.py:285-290.
+ */
+int mi355_paged_tree_attn(const void* q, const void* k_cache, const void* v_cache,
+                          const int32_t* block_table, const int32_t* seq_lens, const int32_t* parents, void* out,
+                          float* part_acc, float* part_ml,
+                          int64_t num_seqs, int64_t num_nodes, int64_t num_q_heads, int64_t num_kv_heads,
+                          int64_t D, int64_t page_size, int64_t max_pages_per_seq, int64_t num_pages,
+                          int64_t num_splits, float scale, int dtype, void* stream);
+
+/*
+ * Verification of drafted tokens against the target model's probabilities, from given random numbers.  Node 0 of a
+ * sequence is its last certain token; node n > 0 is a draft for the token behind node parents[n] (a chain has
+ * parents[n] = n - 1; a parent outside [0, n) or a token outside [0, vocab): the node takes no part).
+ * target_probs: fp32 [num_seqs, num_nodes, vocab], the target's distribution behind each node
+ * draft_probs:  fp32, the same shape: row i is what node i's children were drawn from; NULL: every draft was certain
+ * tokens, parents: int32 [num_seqs, num_nodes]; uniforms: fp32 [num_seqs, num_nodes], in [0, 1)
+ * From node 0 on, with r = the target's row and M = 1, the present node's children are tried in index order: child n with
+ * token t and draft probability q(t) is accepted where uniforms[n] * M * q(t) < r(t); it is then the present node.
+ * A rejection leaves r = max(r - M q, 0) and M = its sum (both as they were if that is 0).  The next token is the
+ * first one whose running sum of r exceeds uniforms[0] times the total (the last one with mass if rounding leaves none;
+ * -1 if there is no mass).  Siblings drawn independently from q, or certain ones, leave the target's distribution unchanged.  All in 64 bits.
+ * path: int32 [num_seqs, num_nodes], the accepted nodes in order, then -1; num_accepted, next_token: int32 [num_seqs].
+ * num_nodes <= 64, vocab <= 2^24.  workspace: mi355_verify_draft_workspace_bytes, scratch (written before it is read in
+ * the same call).  No counterpart in the reference.
+ */
+int64_t mi355_verify_draft_workspace_bytes(int64_t num_seqs, int64_t num_nodes, int64_t vocab);
+int mi355_verify_draft(const float* target_probs, const float* draft_probs, const int32_t* tokens, const int32_t* parents,
+                       const float* uniforms, int32_t* path, int32_t* num_accepted, int32_t* next_token,
+                       int64_t num_seqs, int64_t num_nodes, int64_t vocab,
+                       void* workspace, int64_t workspace_bytes, void* stream);
+
+/*
+ * Block tables and slot maps of a batch step from per-sequence lengths, built on the device in one launch.
+ * Sequence s holds context_lens[s] tokens and adds new_lens[s] (negative values count as 0).  Its pages
+ * [ceil(c / p), ceil((c + n) / p)) (within max_pages_per_seq) are taken from the front of free_pages in sequence order and
+ * entered in block_table [num_seqs, max_pages_per_seq] in place; where the list has run out the entry is -1.
+ * Rows 0 .. num_tokens - 1 of the flat outputs are the new tokens of all sequences in order, then padding; tokens that find
+ * no row are not admitted (they get no page and are not counted):
+ *   seq_lens[s] = c + n; cu_new[num_seqs + 1]: first row of every sequence, and the end;
+ *   positions[row], seq_ids[row], slots[row] = page id * page_size + position % page_size (int64; -1: no page, or the
+ *   position lies behind the table); padding rows: 0, -1, -1;
+ *   pages_needed[0]: pages the step needs (more than num_free: the rest is missing).
+ * The pages taken are free_pages[0 .. min(pages_needed, num_free)).  The same call again gives the same results.
+ * page_size 16, 32, 64, 128 or 256; num_seqs <= 65535, num_tokens, num_free <= 2^30.  No counterpart in the reference.
+ */
+int mi355_paged_batch_layout(int32_t* block_table, const int32_t* context_lens, const int32_t* new_lens,
+                             const int32_t* free_pages, int64_t num_free, int64_t num_seqs,
+                             int64_t max_pages_per_seq, int64_t page_size, int64_t num_tokens,
+                             int32_t* seq_lens, int32_t* cu_new, int32_t* positions, int32_t* seq_ids,
+                             int64_t* slots, int32_t* pages_needed, void* stream);
+
+/*
+ * Rotary positions: out = x with the pairs of the first rotary_dim elements of every head turned by
+ * positions[token] * inv_freq[i], i < rotary_dim / 2, both products scaled by `scale`:
+ *   (a, b) -> scale (a cos - b sin, a sin + b cos);  inverse != 0: sin negated, the gradient's rotation.
+ * Pair i is (2i, 2i+1) with interleaved != 0, else (i, i + rotary_dim / 2); the elements behind rotary_dim pass through.
+ * x, out: [tokens, heads, D] of dtype (MI355_F16 | MI355_BF16 | MI355_F32); *_strides {token, head} in elements, the D elements
+ * of a row contiguous; in place (out == x, same strides) is allowed.  positions: int32 [tokens].  inv_freq: fp64
+ * (freq_is_f64 != 0) or fp32 [rotary_dim / 2].  Angles are formed in 64 bits, the products in 32, rounded once.
+ * rotary_dim even, <= D and <= 1024.  Rows on 16-byte borders with rotary_dim / 2 and D - rotary_dim multiples of 16
+ * bytes' elements run with wide loads; others element by element.
+ * No counterpart among the reference's kernels.
+ */
+int mi355_rope(const void* x, void* out, const int32_t* positions, const void* inv_freq, int freq_is_f64,
+               int64_t tokens, int64_t heads, int64_t D, int64_t rotary_dim,
+               const int64_t* x_strides, const int64_t* out_strides,
+               int interleaved, int inverse, float scale, int dtype, void* stream);
+
+/*
+ * The serving form: q rotated into q_out [tokens, num_q_heads, 128] (contiguous), k_new rotated and v_new as it is into the
+ * rows slots[token] of k_cache / v_cache ([num_slots, num_kv_heads, 128]: the caches' pages and places flattened).
+ * A slot outside [0, num_slots): the token's key and value go nowhere.  Slots must differ from each other (of two
+ * tokens with one slot, either may be found there).  q, k_new, v_new: [tokens, heads, 128] with {token, head} strides;
+ * dtype MI355_F16 | MI355_BF16.  Slots as mi355_paged_batch_layout gives them.
+ * Replaces: the cache update of tests/dynamo/llama_test.py:160-167 with the rotation in front of it.
+ */
+int mi355_rope_kv_append(const void* q, const void* k_new, const void* v_new, void* q_out, void* k_cache, void* v_cache,
+                         const int32_t* positions, const void* inv_freq, int freq_is_f64, const int64_t* slots,
+                         int64_t tokens, int64_t num_q_heads, int64_t num_kv_heads, int64_t D, int64_t rotary_dim,
+                         int64_t num_slots, const int64_t* q_strides, const int64_t* k_strides,
+                         const int64_t* v_strides, int interleaved, float scale, int dtype, void* stream);
 
 /*
  * Block-scaled MXFP4 GEMM: C[M,N] = dq(A) . dq(B)^T, fp32 accumulation, bf16 out.

@@ -35,14 +35,57 @@ struct FaLayout {
   int H, group;
 };
 
-template <bool CAUSAL, bool BF>
+// Packed sequences of different lengths (the VARLEN form): the queries of sequence s are the rows [cu_q[s], cu_q[s + 1]) of
+// one token stream, its keys and values the rows [cu_k[s], cu_k[s + 1]) of another.
+struct FaVarlen {
+  const int *cu_q, *cu_k;  // [num_seqs + 1]
+  int num_seqs, total_q, total_k;
+  int zero_rest;           // also write zeros to the query rows in front of the first and behind the last sequence
+};
+
+// Rows [begin, begin + len) of sequence s; offsets outside the stream are cut to it, a negative length counts as 0.
+__device__ __forceinline__ int fa_seq_range(const int* cu, int s, int total, int& begin) {
+  int b = cu[s], e = cu[s + 1];
+  b = b < 0 ? 0 : (b > total ? total : b);
+  e = e < b ? b : (e > total ? total : e);
+  begin = b;
+  return e - b;
+}
+
+// The sequence that holds unit number `unit` when sequence s has ceil(len_s / rows) units, in order, and the unit's
+// number inside it; -1 behind the last one.  Every wave finds it by itself, 64 sequences at a time.
+__device__ __forceinline__ int fa_find_unit(const FaVarlen& vl, int rows, int unit, int& inside) {
+  const int lane = threadIdx.x & 63;
+  int base = 0;
+  for (int s0 = 0; s0 < vl.num_seqs; s0 += 64) {
+    int begin, n = 0;
+    if (s0 + lane < vl.num_seqs) n = (fa_seq_range(vl.cu_q, s0 + lane, vl.total_q, begin) + rows - 1) / rows;
+    int incl = n;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const int up = __shfl_up(incl, d);
+      if (lane >= d) incl += up;
+    }
+    const unsigned long long past = __builtin_amdgcn_ballot_w64(base + incl > unit);
+    if (past) {
+      const int l = __builtin_ctzll(past);
+      inside = __builtin_amdgcn_readfirstlane(unit - base - __shfl(incl - n, l));
+      return s0 + l;
+    }
+    base += __shfl(incl, 63);
+  }
+  return -1;
+}
+
+template <bool CAUSAL, bool BF, bool VARLEN = false>
 __global__ __launch_bounds__(256) void fa_fwd_d128(const half_t* __restrict__ Q, const half_t* __restrict__ K,
-                                                   const half_t* __restrict__ V, half_t* __restrict__ O, int BH, int Sq,
-                                                   int Sk, float scale_log2e, int q_blocks, FaLayout lay) {
+                                                   const half_t* __restrict__ V, half_t* __restrict__ O, int BH, int Sq_arg,
+                                                   int Sk_arg, float scale_log2e, int q_blocks, FaLayout lay, FaVarlen vl) {
   extern __shared__ __attribute__((aligned(1024))) char lds[];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int r32 = lane & 31, h = lane >> 5;
+  int Sq = Sq_arg, Sk = Sk_arg;
 
   // workgroup -> (batch*head, query block).  Consecutive ids land on different XCDs; keep all
   // query blocks of one head on one XCD so its K/V stay in that XCD's L2.
@@ -59,7 +102,31 @@ __global__ __launch_bounds__(256) void fa_fwd_d128(const half_t* __restrict__ Q,
       bh = pid / q_blocks;
       qb = pid % q_blocks;
     }
-    if (CAUSAL) qb = q_blocks - 1 - qb;  // longest rows first
+    if (CAUSAL && !VARLEN) qb = q_blocks - 1 - qb;  // longest rows first
+  }
+  int b_idx = VARLEN ? 0 : bh / lay.H;
+  const int h_idx = bh - b_idx * lay.H, hk_idx = h_idx / lay.group;
+  size_t q_base = 0, k_base_row = 0;
+  if constexpr (VARLEN) {
+    if (vl.zero_rest) {
+      int first, last;
+      fa_seq_range(vl.cu_q, 0, vl.total_q, first);
+      const int len = fa_seq_range(vl.cu_q, vl.num_seqs - 1, vl.total_q, last);
+      last += len;
+      const int outside = first + vl.total_q - last;
+      for (int i = qb; i < outside; i += q_blocks) {
+        half_t* row = O + (size_t)(i < first ? i : last + i - first) * lay.o_r + h_idx * lay.o_h;
+        if (threadIdx.x < 128) row[threadIdx.x] = (half_t)0;
+      }
+    }
+    int inside = 0, q_first, k_first;
+    const int seq = fa_find_unit(vl, FA_BLOCK_M, qb, inside);
+    if (seq < 0) return;
+    Sq = __builtin_amdgcn_readfirstlane(fa_seq_range(vl.cu_q, seq, vl.total_q, q_first));
+    Sk = __builtin_amdgcn_readfirstlane(fa_seq_range(vl.cu_k, seq, vl.total_k, k_first));
+    qb = inside;
+    q_base = (size_t)__builtin_amdgcn_readfirstlane(q_first);
+    k_base_row = (size_t)__builtin_amdgcn_readfirstlane(k_first);
   }
   const int causal_off = Sk - Sq;  // query i sees keys <= i + causal_off
   const int q0 = qb * FA_BLOCK_M;
@@ -67,11 +134,10 @@ __global__ __launch_bounds__(256) void fa_fwd_d128(const half_t* __restrict__ Q,
   const int q_row = wq0 + r32;
   const bool q_ok = q_row < Sq;
 
-  const int b_idx = bh / lay.H, h_idx = bh - b_idx * lay.H, hk_idx = h_idx / lay.group;
-  const half_t* Qb = Q + b_idx * lay.q_b + h_idx * lay.q_h;
-  const half_t* Kb = K + b_idx * lay.k_b + hk_idx * lay.k_h;
-  const half_t* Vb = V + b_idx * lay.v_b + hk_idx * lay.v_h;
-  half_t* Ob = O + b_idx * lay.o_b + h_idx * lay.o_h;
+  const half_t* Qb = Q + b_idx * lay.q_b + h_idx * lay.q_h + q_base * lay.q_r;
+  const half_t* Kb = K + b_idx * lay.k_b + hk_idx * lay.k_h + k_base_row * lay.k_r;
+  const half_t* Vb = V + b_idx * lay.v_b + hk_idx * lay.v_h + k_base_row * lay.v_r;
+  half_t* Ob = O + b_idx * lay.o_b + h_idx * lay.o_h + q_base * lay.o_r;
 
   // number of key tiles this workgroup walks
   int k_end = Sk;
@@ -1524,7 +1590,7 @@ static int fa_launch(const void* q, const void* k, const void* v, void* o, int64
   if (variant == 1) {
     auto kern = is_causal ? fa_fwd_d128<true, BF> : fa_fwd_d128<false, BF>;
     hipLaunchKernelGGL(kern, grid, block, lds_bytes, s, (const half_t*)q, (const half_t*)k, (const half_t*)v, (half_t*)o, BH,
-                       (int)Sq, (int)Sk, scale_log2e, q_blocks, lay);
+                       (int)Sq, (int)Sk, scale_log2e, q_blocks, lay, FaVarlen{});
   } else {
     auto kern = is_causal ? fa_fwd_d128_pipe<true, BF> : fa_fwd_d128_pipe<false, BF>;
     hipLaunchKernelGGL(kern, grid, block, lds_bytes, s, (const half_t*)q, (const half_t*)k, (const half_t*)v, (half_t*)o, BH,
@@ -1650,4 +1716,65 @@ extern "C" int mi355_paged_prefill_attn_bf16(const void* q, const void* k_cache,
                                              int64_t max_pages_per_seq, int64_t num_pages, float scale, void* stream) {
   return fa_paged_prefill<true>(q, k_cache, v_cache, block_table, seq_lens, out, num_seqs, num_new, num_q_heads, num_kv_heads, D,
                                 page_size, max_pages_per_seq, num_pages, scale, stream);
+}
+
+template <bool BF>
+static int fa_varlen(const void* q, const void* k, const void* v, void* o, const int32_t* cu_q, const int32_t* cu_k, int64_t num_seqs,
+                     int64_t total_q, int64_t total_k, int64_t H, int64_t Hkv, int64_t D, const int64_t* q_strides,
+                     const int64_t* k_strides, const int64_t* v_strides, const int64_t* o_strides, float scale, int is_causal,
+                     int zero_rest, void* stream) {
+  const char* who = BF ? "flash_attn_varlen_fwd_bf16" : "flash_attn_varlen_fwd";
+  if (!q || !k || !v || !o || !cu_q || !cu_k || !q_strides || !k_strides || !v_strides || !o_strides)
+    return fail(-MI355_E_NULL, "%s: null pointer", who);
+  if (D != 128) return fail(-MI355_E_SHAPE, "%s: head dim %lld not supported (only 128)", who, (long long)D);
+  if (num_seqs <= 0 || num_seqs > 65535 || total_q <= 0 || total_k <= 0 || total_q > (1 << 24) || total_k > (1 << 24) || H <= 0 ||
+      H > 65535)
+    return fail(-MI355_E_SHAPE, "%s: bad sizes seqs=%lld total_q=%lld total_k=%lld H=%lld", who, (long long)num_seqs,
+                (long long)total_q, (long long)total_k, (long long)H);
+  if (Hkv <= 0 || H % Hkv != 0)
+    return fail(-MI355_E_SHAPE, "%s: %lld query heads over %lld key/value heads", who, (long long)H, (long long)Hkv);
+  if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(o))
+    return fail(-MI355_E_ALIGN, "%s: q, k, v, o must be 16-byte aligned", who);
+  if (!(scale > 0.f) || !isfinite(scale)) return fail(-MI355_E_SHAPE, "%s: scale must be positive and finite", who);
+  const int64_t* all[4] = {q_strides, k_strides, v_strides, o_strides};
+  for (const int64_t* st : all) {  // {token, head}
+    if (st[0] < 0 || st[1] < 0 || ((st[0] | st[1]) & 7))
+      return fail(-MI355_E_ALIGN, "%s: strides must be non-negative multiples of 8 elements", who);
+    if (st[0] < 128 || st[0] >= (1ll << 24) || st[1] >= (1ll << 40))
+      return fail(-MI355_E_SHAPE, "%s: token stride %lld outside [128, 2^24)", who, (long long)st[0]);
+  }
+  if (H > 1 && o_strides[1] == 0) return fail(-MI355_E_SHAPE, "%s: the output's head stride must not be 0", who);
+  FaLayout lay;
+  lay.q_b = lay.k_b = lay.v_b = lay.o_b = 0;
+  lay.q_h = q_strides[1], lay.q_r = (unsigned)q_strides[0];
+  lay.k_h = k_strides[1], lay.k_r = (unsigned)k_strides[0];
+  lay.v_h = v_strides[1], lay.v_r = (unsigned)v_strides[0];
+  lay.o_h = o_strides[1], lay.o_r = (unsigned)o_strides[0];
+  lay.H = (int)H, lay.group = (int)(H / Hkv);
+  const FaVarlen vl{cu_q, cu_k, (int)num_seqs, (int)total_q, (int)total_k, zero_rest};
+  // the lengths are known on the device only: as many blocks as num_seqs sequences of total_q rows can have
+  const int64_t blocks = total_q / FA_BLOCK_M + num_seqs;
+  if (blocks * H >= (1ll << 31)) return fail(-MI355_E_SHAPE, "%s: too many query blocks", who);
+  auto kern = is_causal ? fa_fwd_d128<true, BF, true> : fa_fwd_d128<false, BF, true>;
+  const int lds_bytes = 2 * FA_STAGE;
+  static std::atomic<uint64_t> lds_ok[2] = {};
+  if (int rc = allow_lds(reinterpret_cast<const void*>(kern), lds_bytes, lds_ok[is_causal ? 1 : 0], "fa_fwd_d128<varlen>")) return rc;
+  dim3 grid((unsigned)(blocks * H)), block(256);
+  hipLaunchKernelGGL(kern, grid, block, lds_bytes, reinterpret_cast<hipStream_t>(stream), (const half_t*)q, (const half_t*)k,
+                     (const half_t*)v, (half_t*)o, (int)H, 0, 0, scale * 1.4426950408889634f, (int)blocks, lay, vl);
+  return check_launch("fa_fwd_d128<varlen>", grid, block, lds_bytes);
+}
+
+extern "C" int mi355_flash_attn_varlen_fwd(const void* q, const void* k, const void* v, void* o, const int32_t* cu_seqlens_q,
+                                           const int32_t* cu_seqlens_k, int64_t num_seqs, int64_t total_q, int64_t total_k, int64_t H,
+                                           int64_t Hkv, int64_t D, const int64_t* q_strides, const int64_t* k_strides,
+                                           const int64_t* v_strides, const int64_t* o_strides, float scale, int is_causal,
+                                           int zero_rest, int dtype, void* stream) {
+  if (dtype == MI355_BF16)
+    return fa_varlen<true>(q, k, v, o, cu_seqlens_q, cu_seqlens_k, num_seqs, total_q, total_k, H, Hkv, D, q_strides, k_strides, v_strides,
+                           o_strides, scale, is_causal, zero_rest, stream);
+  if (dtype == MI355_F16)
+    return fa_varlen<false>(q, k, v, o, cu_seqlens_q, cu_seqlens_k, num_seqs, total_q, total_k, H, Hkv, D, q_strides, k_strides, v_strides,
+                            o_strides, scale, is_causal, zero_rest, stream);
+  return fail(-MI355_E_DTYPE, "flash_attn_varlen_fwd: dtype %d (MI355_F16 or MI355_BF16)", dtype);
 }

@@ -1,0 +1,389 @@
+// Attention of drafted token trees over a paged KV cache (the verification step of speculative decoding), head dim 128.
+//
+// Sequence s holds L = seq_lens[s] tokens, the last N of them its drafts, node n at position L - N + n.  A node's query
+// sees every token in front of the drafts, itself and its ancestors.  With G query heads per kv head there are R = N * G
+// query rows (row r: node r / G, head r % G of the group) that read the same keys and values: they share one pass.
+//
+// The op is HBM bound up to about 160 rows (a K and a V row are 512 bytes and 512 flop per query row), so the kernel is
+// the one-token decode kernel's: every wave streams its own steps of 32 tokens -- K straight into MFMA operand
+// registers, V through a private LDS ring by direct-to-LDS loads, both one step ahead -- and no wave waits for another
+// before the end.  What differs: a step's K and V serve C column groups of 16 query rows (C = 1, 2 or 4; more rows than
+// 64 take further workgroups, which find the pages in the caches), and scores of draft positions are masked by the
+// node's set of ancestors, a 64-bit word per node made from the parents once per workgroup by pointer doubling.
+//
+// The table's reach is cut into num_splits chunks of equally many 32-token steps; a sequence that fits one chunk writes
+// its result directly, the others write fp32 partials that a second launch merges.
+#include "common.hpp"
+#include <math.h>
+
+namespace mi355 {
+
+constexpr int PT_WAVES = 4;
+constexpr int PT_WAVE_LDS = 2 * 8192;  // two stages of 32 V rows
+constexpr int PT_MAX_NODES = 64;
+constexpr int PT_MAX_GROUP = 128;  // query heads per kv head
+
+struct PtArgs {
+  const half_t *q, *kc, *vc;
+  const int *table, *seq_lens, *parents;
+  half_t* out;
+  float *part_acc, *part_ml;  // [S, N, Hq, splits, 128] and [.., 2]
+  int num_kv_heads, group, nodes, max_pages, num_pages, page_shift, num_splits, chunk_steps, row_blocks;
+  float scale_log2e;
+};
+
+// ancestors (and self) of node `lane` as a bit set; a parent that does not come before its node is none
+__device__ __forceinline__ unsigned long long pt_ancestors(const int* parents, int nodes) {
+  const int lane = threadIdx.x & 63;
+  int up = lane < nodes ? parents[lane] : -1;
+  up = (up >= 0 && up < lane) ? up : -1;
+  unsigned long long set = 1ull << lane;
+#pragma unroll
+  for (int i = 0; i < 6; i++) {
+    const int from = up < 0 ? lane : up;
+    const unsigned long long s = __shfl(set, from);
+    const int next = __shfl(up, from);
+    if (up >= 0) {
+      set |= s;
+      up = next;
+    }
+  }
+  return set;
+}
+
+// Which of the four positions d, .. , d + 3 (counted from the first draft) a node with ancestor set `seen` sees, as bits 0 .. 3:
+// all in front of the drafts, then the set's; the set has no bits behind the last draft.
+__device__ __forceinline__ unsigned pt_visible4(unsigned long long seen, int d) {
+  const int up = d > 0 ? (d < 63 ? d : 63) : 0, down = d < 0 ? (d > -4 ? -d : 4) : 0;
+  const unsigned w = d > 63 ? 0u : (unsigned)(seen >> up);
+  return (w << down) | ((1u << down) - 1u);
+}
+
+// v where bit r of `visible` is set, else -inf, by bit operations: the selection on a chain of conditions (dropped, behind
+// the end, a draft that is no ancestor) has been compiled to one that keeps the score.
+__device__ __forceinline__ float pt_hide(float v, unsigned visible, int r) {
+  const unsigned keep = (unsigned)((int)(visible << (31 - r)) >> 31);
+  return __builtin_bit_cast(float, (__builtin_bit_cast(unsigned, v) & keep) | (0xFF800000u & ~keep));
+}
+
+template <int C, bool BF>
+__global__ __launch_bounds__(PT_WAVES * 64) __attribute__((amdgpu_waves_per_eu(C == 4 ? 1 : 2, C == 4 ? 1 : 2))) void paged_tree_kernel(PtArgs a) {
+  extern __shared__ __attribute__((aligned(1024))) char lds[];
+  constexpr int ROWS = 16 * C;
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int i16 = lane & 15, g = lane >> 4;
+  const int split = blockIdx.x / a.row_blocks, rb = blockIdx.x - split * a.row_blocks;
+  const int kvh = blockIdx.y, seq = blockIdx.z;
+  const int R = a.nodes * a.group, row0 = rb * ROWS;
+  const int num_q_heads = a.num_kv_heads * a.group;
+
+  const int reach = (a.max_pages << a.page_shift) * 16;
+  const int L_in = a.seq_lens[seq];
+  const int L = L_in < 0 ? 0 : (L_in > reach ? reach : L_in);
+  const int draft0 = L - a.nodes;  // position of node 0 (negative: the first nodes are not in the cache)
+  const int steps = (L + 31) >> 5;
+  const int s_begin = split * a.chunk_steps;
+  const int s_end = s_begin + a.chunk_steps < steps ? s_begin + a.chunk_steps : steps;
+  // a chunk behind the sequence's end has nothing to do; chunk 0 of an empty sequence writes its zeros
+  if (s_begin >= steps && split > 0) return;
+  const bool single = steps <= a.chunk_steps;
+  const int p_end = (L + 15) >> 4;  // 16-token blocks
+  const int n_steps = s_end - s_begin;
+
+  unsigned long long* anc = reinterpret_cast<unsigned long long*>(lds);
+  if (wave == 0) anc[lane] = pt_ancestors(a.parents + (size_t)seq * a.nodes, a.nodes);
+  __syncthreads();
+  unsigned long long seen[C];
+  half8 qf[C][4];
+#pragma unroll
+  for (int c = 0; c < C; c++) {
+    const int r = row0 + c * 16 + i16;
+    const int node = r < R ? r / a.group : 0;
+    const int head = kvh * a.group + (r < R ? r - node * a.group : 0);
+    seen[c] = anc[node];
+#pragma unroll
+    for (int ks = 0; ks < 4; ks++) {
+      if (r < R) {
+        qf[c][ks] = *reinterpret_cast<const half8*>(a.q + (((size_t)seq * a.nodes + node) * num_q_heads + head) * 128 + ks * 32 + g * 8);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; e++) qf[c][ks][e] = (half_t)0;
+      }
+    }
+  }
+  __syncthreads();  // the words are part of the V ring
+
+  const int* bt = a.table + (size_t)seq * a.max_pages;
+  char* my_lds = lds + wave * PT_WAVE_LDS;
+  const size_t tok_stride = (size_t)a.num_kv_heads * 128;
+  const half_t* k_lane = a.kc + (size_t)kvh * 128 + i16 * tok_stride + g * 8;
+  const int vl_row = lane >> 4, vl_slot = lane & 15;
+  const half_t* v_lane = a.vc + (size_t)kvh * 128 + vl_row * tok_stride;
+  const int vr_row = 4 * g + (i16 >> 2);
+  const int vr_base = vr_row * 256 + ((((i16 & 3) >> 1) ^ (2 * (vr_row & 7))) * 16) + (i16 & 1) * 8;  // ^ (dt * 32)
+
+  half8 kf[2][2][4];  // [buffer][16-token block][ks]
+  int bad[2] = {0, 0};  // bit x: block x of the step in this buffer has no page (its tokens are dropped)
+  auto issue = [&](int step, int buf) {
+    const int pa = 2 * (s_begin + wave + PT_WAVES * step);
+    const int sub = (1 << a.page_shift) - 1;
+    int id0 = bt[pa >> a.page_shift];
+    int id1 = (pa + 1 < p_end) ? bt[(pa + 1) >> a.page_shift] : id0;
+    const int drop0 = (unsigned)id0 >= (unsigned)a.num_pages, drop1 = (unsigned)id1 >= (unsigned)a.num_pages;
+    id0 = drop0 ? 0 : id0;
+    id1 = drop1 ? 0 : id1;
+    bad[buf] = drop0 | (drop1 << 1);
+    const size_t blk0 = ((size_t)id0 << a.page_shift) + (pa & sub);
+    const size_t blk1 = (pa + 1 < p_end) ? ((size_t)id1 << a.page_shift) + ((pa + 1) & sub) : blk0;
+    char* dst = my_lds + buf * 8192;
+#pragma unroll
+    for (int x = 0; x < 2; x++) {
+      const size_t off = (x ? blk1 : blk0) * 16 * tok_stride;
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        const int chunk = vl_slot ^ (2 * ((4 * (i & 1) + vl_row) & 7));
+        load_lds_16B(v_lane + off + (size_t)(4 * i) * tok_stride + chunk * 8, dst + x * 4096 + i * 1024);
+      }
+    }
+#pragma unroll
+    for (int x = 0; x < 2; x++) {
+      const size_t off = (x ? blk1 : blk0) * 16 * tok_stride;
+#pragma unroll
+      for (int ks = 0; ks < 4; ks++) kf[buf][x][ks] = *reinterpret_cast<const half8*>(k_lane + off + ks * 32);
+    }
+  };
+
+  floatx4 oacc[C][8];
+  float m_run[C], l_run[C];
+#pragma unroll
+  for (int c = 0; c < C; c++) {
+    m_run[c] = -INFINITY, l_run[c] = 0.f;
+#pragma unroll
+    for (int dt = 0; dt < 8; dt++) oacc[c][dt] = floatx4{0.f, 0.f, 0.f, 0.f};
+  }
+
+  const int my_steps = n_steps > wave ? (n_steps - wave + PT_WAVES - 1) / PT_WAVES : 0;
+  if (my_steps > 0) issue(0, 0);
+#pragma unroll 1
+  for (int u = 0; u < my_steps; u += 2) {
+#pragma unroll
+    for (int b = 0; b < 2; b++) {
+      const int step = u + b;
+      if (step < my_steps) {
+        if (step + 1 < my_steps) {
+          issue(step + 1, b ^ 1);
+          asm volatile("s_waitcnt vmcnt(16)" ::: "memory");
+        } else {
+          asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        }
+        const int pa = 2 * (s_begin + wave + PT_WAVES * step);
+        const int tok0 = pa * 16 + 4 * g;  // lane (row i16, g) holds tokens tok0 + r and tok0 + 16 + r
+        const bool drop0 = bad[b] & 1, drop1 = bad[b] & 2;
+        const bool edge = pa * 16 + 32 > draft0 || bad[b] != 0;  // the step reaches into the drafts, past the end, or drops a block
+        half8 pf[C];
+#pragma unroll
+        for (int c = 0; c < C; c++) {
+          floatx4 s0 = {0.f, 0.f, 0.f, 0.f}, s1 = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int ks = 0; ks < 4; ks++) s0 = mfma16_16x16x32<BF>(kf[b][0][ks], qf[c][ks], s0);
+#pragma unroll
+          for (int ks = 0; ks < 4; ks++) s1 = mfma16_16x16x32<BF>(kf[b][1][ks], qf[c][ks], s1);
+          if (edge) {
+            const unsigned vis0 = drop0 ? 0u : pt_visible4(seen[c], tok0 - draft0);
+            const unsigned vis1 = drop1 ? 0u : pt_visible4(seen[c], tok0 + 16 - draft0);
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+              s0[r] = pt_hide(s0[r], vis0, r);
+              s1[r] = pt_hide(s1[r], vis1, r);
+            }
+          }
+          float mx = fmaxf(fmaxf(fmaxf(s0[0], s0[1]), fmaxf(s0[2], s0[3])), fmaxf(fmaxf(s1[0], s1[1]), fmaxf(s1[2], s1[3])));
+          mx = fmaxf(mx, __shfl_xor(mx, 16));
+          mx = fmaxf(mx, __shfl_xor(mx, 32));
+          const float m_new = fmaxf(m_run[c], mx);
+          const bool none_yet = m_new == -INFINITY;
+          const float alpha = none_yet ? 1.f : __builtin_amdgcn_exp2f((m_run[c] - m_new) * a.scale_log2e);
+          const float mc = none_yet ? 0.f : m_new * a.scale_log2e;
+          m_run[c] = m_new;
+          float psum = 0.f;
+#pragma unroll
+          for (int r = 0; r < 4; r++) {
+            const float p0 = __builtin_amdgcn_exp2f(s0[r] * a.scale_log2e - mc);
+            const float p1 = __builtin_amdgcn_exp2f(s1[r] * a.scale_log2e - mc);
+            psum += p0 + p1;
+            pf[c][r] = cvt16<BF>(p0);
+            pf[c][4 + r] = cvt16<BF>(p1);
+          }
+          l_run[c] = l_run[c] * alpha + psum;
+#pragma unroll
+          for (int dt = 0; dt < 8; dt++) oacc[c][dt] = oacc[c][dt] * alpha;
+        }
+        const char* vst = my_lds + b * 8192;
+#pragma unroll
+        for (int dt = 0; dt < 8; dt++) {
+          half4 lo = lds_read_tr16(vst + (vr_base ^ (dt * 32)));
+          half4 hi = lds_read_tr16(vst + 4096 + (vr_base ^ (dt * 32)));
+          if (edge) {  // tokens at or beyond L may hold anything (NaN included): 0 * garbage must stay 0
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+              if (drop0 || tok0 + e >= L) lo[e] = (half_t)0;
+              if (drop1 || tok0 + 16 + e >= L) hi[e] = (half_t)0;
+            }
+          }
+          const half8 vf = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+#pragma unroll
+          for (int c = 0; c < C; c++) oacc[c][dt] = mfma16_16x16x32<BF>(vf, pf[c], oacc[c][dt]);
+        }
+      }
+    }
+  }
+
+  // ---- merge the four waves through LDS, one column group at a time ----
+  float* sm = reinterpret_cast<float*>(lds);  // [wave][16]
+  float* sl = sm + PT_WAVES * 16;
+  float* sacc = sl + PT_WAVES * 16;           // [wave][16][128]
+#pragma unroll
+  for (int c = 0; c < C; c++) {
+    float l = l_run[c] + __shfl_xor(l_run[c], 16);
+    l += __shfl_xor(l, 32);
+    __syncthreads();  // the V rings (or the group before) are done with
+    if (g == 0) {
+      sm[wave * 16 + i16] = m_run[c];
+      sl[wave * 16 + i16] = l;
+    }
+#pragma unroll
+    for (int dt = 0; dt < 8; dt++) *reinterpret_cast<floatx4*>(sacc + ((wave * 16 + i16) * 128 + dt * 16 + 4 * g)) = oacc[c][dt];
+    __syncthreads();
+    for (int idx = threadIdx.x; idx < 16 * 128; idx += PT_WAVES * 64) {
+      const int col = idx >> 7, d = idx & 127, r = row0 + c * 16 + col;
+      if (r >= R) continue;
+      float m_tot = -INFINITY;
+#pragma unroll
+      for (int w = 0; w < PT_WAVES; w++) m_tot = fmaxf(m_tot, sm[w * 16 + col]);
+      float acc = 0.f, lt = 0.f;
+      if (m_tot > -INFINITY) {
+#pragma unroll
+        for (int w = 0; w < PT_WAVES; w++) {
+          const float mw = sm[w * 16 + col];
+          const float wgt = mw > -INFINITY ? __builtin_amdgcn_exp2f((mw - m_tot) * a.scale_log2e) : 0.f;
+          acc += wgt * sacc[(w * 16 + col) * 128 + d];
+          lt += wgt * sl[w * 16 + col];
+        }
+      }
+      const int node = r / a.group;
+      const size_t row = ((size_t)seq * a.nodes + node) * num_q_heads + kvh * a.group + (r - node * a.group);
+      if (single) {
+        a.out[row * 128 + d] = cvt16<BF>(lt > 0.f ? acc / lt : 0.f);
+      } else {
+        const size_t at = row * a.num_splits + split;
+        a.part_acc[at * 128 + d] = acc;
+        if (d == 0) {
+          a.part_ml[at * 2] = m_tot * a.scale_log2e;
+          a.part_ml[at * 2 + 1] = lt;
+        }
+      }
+    }
+  }
+}
+
+// Merge of the chunks of every row whose sequence has more than one: one wave per row, two elements per lane.
+template <bool BF>
+__global__ __launch_bounds__(64) void paged_tree_merge_kernel(PtArgs a) {
+  const size_t row = blockIdx.x;
+  const int rows_per_seq = a.nodes * a.num_kv_heads * a.group;
+  const int seq = (int)(row / rows_per_seq);
+  const int reach = (a.max_pages << a.page_shift) * 16;
+  const int L_in = a.seq_lens[seq];
+  const int L = L_in < 0 ? 0 : (L_in > reach ? reach : L_in);
+  const int steps = (L + 31) >> 5;
+  if (steps <= a.chunk_steps) return;
+  const int n = (steps + a.chunk_steps - 1) / a.chunk_steps;
+  const int lane = threadIdx.x;
+  const float* ml = a.part_ml + row * a.num_splits * 2;
+  float m_tot = -INFINITY;
+  for (int s = 0; s < n; s++) m_tot = fmaxf(m_tot, ml[2 * s]);
+  float a0 = 0.f, a1 = 0.f, l = 0.f;
+  if (m_tot > -INFINITY) {
+    for (int s = 0; s < n; s++) {
+      const float w = __builtin_amdgcn_exp2f(ml[2 * s] - m_tot);
+      const floatx2 p = *reinterpret_cast<const floatx2*>(a.part_acc + (row * a.num_splits + s) * 128 + 2 * lane);
+      a0 = __builtin_fmaf(w, p[0], a0);
+      a1 = __builtin_fmaf(w, p[1], a1);
+      l = __builtin_fmaf(w, ml[2 * s + 1], l);
+    }
+  }
+  const float inv = l > 0.f ? 1.f / l : 0.f;
+  *reinterpret_cast<half2v*>(a.out + row * 128 + 2 * lane) = cvt16x2<BF>(a0 * inv, a1 * inv);
+}
+
+template <int C, bool BF>
+static int launch_tree(const PtArgs& a, int num_seqs, hipStream_t stream) {
+  auto kern = paged_tree_kernel<C, BF>;
+  constexpr int lds_bytes = PT_WAVES * PT_WAVE_LDS;
+  static_assert(lds_bytes >= (int)((2 * PT_WAVES * 16 + PT_WAVES * 16 * 128) * sizeof(float)), "merge area must fit");
+  static std::atomic<uint64_t> lds_ok{0};
+  if (int rc = allow_lds(reinterpret_cast<const void*>(kern), lds_bytes, lds_ok, "paged_tree_kernel")) return rc;
+  dim3 grid(a.num_splits * a.row_blocks, a.num_kv_heads, num_seqs), block(PT_WAVES * 64);
+  hipLaunchKernelGGL(kern, grid, block, lds_bytes, stream, a);
+  return check_launch("paged_tree_kernel", grid, block, lds_bytes);
+}
+
+template <bool BF>
+static int run_tree(PtArgs a, int num_seqs, hipStream_t stream) {
+  const int R = a.nodes * a.group;
+  const int C = R <= 16 ? 1 : R <= 32 ? 2 : 4;
+  a.row_blocks = (R + 16 * C - 1) / (16 * C);
+  int rc;
+  if (C == 1) rc = launch_tree<1, BF>(a, num_seqs, stream);
+  else if (C == 2) rc = launch_tree<2, BF>(a, num_seqs, stream);
+  else rc = launch_tree<4, BF>(a, num_seqs, stream);
+  if (rc || a.num_splits == 1) return rc;
+  dim3 grid((unsigned)((int64_t)num_seqs * R * a.num_kv_heads)), block(64);
+  hipLaunchKernelGGL(paged_tree_merge_kernel<BF>, grid, block, 0, stream, a);
+  return check_launch("paged_tree_merge_kernel", grid, block, 0);
+}
+
+}  // namespace mi355
+
+using namespace mi355;
+
+extern "C" int mi355_paged_tree_attn(const void* q, const void* k_cache, const void* v_cache, const int32_t* block_table,
+                                     const int32_t* seq_lens, const int32_t* parents, void* out, float* part_acc, float* part_ml,
+                                     int64_t num_seqs, int64_t num_nodes, int64_t num_q_heads, int64_t num_kv_heads, int64_t D,
+                                     int64_t page_size, int64_t max_pages_per_seq, int64_t num_pages, int64_t num_splits, float scale,
+                                     int dtype, void* stream) {
+  const char* fn = "paged_tree_attn";
+  if (!q || !k_cache || !v_cache || !block_table || !seq_lens || !parents || !out) return fail(-MI355_E_NULL, "%s: null pointer", fn);
+  if (dtype != MI355_F16 && dtype != MI355_BF16) return fail(-MI355_E_DTYPE, "%s: dtype %d (MI355_F16 or MI355_BF16)", fn, dtype);
+  if (D != 128) return fail(-MI355_E_SHAPE, "%s: head dim %lld not supported (only 128)", fn, (long long)D);
+  int page_shift = -1;
+  for (int sh = 0; sh <= 4; sh++)
+    if (page_size == (16ll << sh)) page_shift = sh;
+  if (page_shift < 0) return fail(-MI355_E_SHAPE, "%s: page size %lld not supported (16, 32, 64, 128 or 256)", fn, (long long)page_size);
+  if (num_nodes <= 0 || num_nodes > PT_MAX_NODES)
+    return fail(-MI355_E_SHAPE, "%s: %lld nodes per sequence, supported: 1 to %d", fn, (long long)num_nodes, PT_MAX_NODES);
+  if (num_seqs <= 0 || num_seqs > 65535 || num_q_heads <= 0 || num_kv_heads <= 0 || num_kv_heads > 65535 || num_q_heads > 65535 ||
+      max_pages_per_seq <= 0 || max_pages_per_seq > (1 << 22) || num_pages <= 0 || num_pages > (1 << 26) ||
+      num_seqs * num_nodes * num_q_heads > (1ll << 30) || max_pages_per_seq * page_size > (1ll << 30))
+    return fail(-MI355_E_SHAPE, "%s: bad sizes seqs=%lld nodes=%lld hq=%lld hkv=%lld max_pages=%lld num_pages=%lld", fn,
+                (long long)num_seqs, (long long)num_nodes, (long long)num_q_heads, (long long)num_kv_heads,
+                (long long)max_pages_per_seq, (long long)num_pages);
+  if (num_q_heads % num_kv_heads != 0)
+    return fail(-MI355_E_SHAPE, "%s: q heads %lld not a multiple of kv heads %lld", fn, (long long)num_q_heads, (long long)num_kv_heads);
+  if (num_q_heads / num_kv_heads > PT_MAX_GROUP)
+    return fail(-MI355_E_SHAPE, "%s: q heads per kv head = %lld, supported: up to %d", fn, (long long)(num_q_heads / num_kv_heads), PT_MAX_GROUP);
+  if (num_splits < 1 || num_splits > 1024) return fail(-MI355_E_SHAPE, "%s: num_splits %lld out of range [1, 1024]", fn, (long long)num_splits);
+  if (!(scale > 0.f) || !isfinite(scale)) return fail(-MI355_E_SHAPE, "%s: scale must be positive and finite", fn);
+  if (!aligned16(q) || !aligned16(k_cache) || !aligned16(v_cache) || !aligned16(out))
+    return fail(-MI355_E_ALIGN, "%s: q, k_cache, v_cache, out must be 16-byte aligned", fn);
+  if (num_splits > 1 && (!part_acc || !part_ml)) return fail(-MI355_E_SCRATCH, "%s: num_splits > 1 needs part_acc / part_ml scratch", fn);
+  if (num_splits > 1 && !aligned16(part_acc)) return fail(-MI355_E_ALIGN, "%s: part_acc must be 16-byte aligned", fn);
+  const int64_t reach_steps = (max_pages_per_seq * page_size + 31) / 32;
+  PtArgs a{(const half_t*)q, (const half_t*)k_cache, (const half_t*)v_cache, block_table, seq_lens, parents, (half_t*)out,
+           part_acc, part_ml, (int)num_kv_heads, (int)(num_q_heads / num_kv_heads), (int)num_nodes, (int)max_pages_per_seq,
+           (int)num_pages, page_shift, (int)num_splits, (int)((reach_steps + num_splits - 1) / num_splits), 1,
+           scale * 1.4426950408889634f};
+  hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  return dtype == MI355_BF16 ? run_tree<true>(a, (int)num_seqs, s) : run_tree<false>(a, (int)num_seqs, s);
+}

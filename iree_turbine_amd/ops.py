@@ -17,7 +17,7 @@ from . import launch
 from .contract import PAGE_SIZES, check_mx_operand as _check_mx_operand, check_paged_args as _check_paged_args  # noqa: F401
 from . import contract
 from .contract import require as _require
-from .op_reg import CustomOp, KernelSelection
+from .op_reg import CustomOp, KernelSelection, TensorArg
 
 __all__ = [
     "gemm_nt",
@@ -27,6 +27,13 @@ __all__ = [
     "kv_cache_append",
     "paged_decode_phase0",
     "paged_decode_phase1",
+    "paged_batch_layout",
+    "rope",
+    "rope_inv_freq",
+    "rope_kv_append",
+    "flash_attn_varlen_fwd",
+    "paged_tree_attn",
+    "verify_draft",
     "mxfp4_gemm",
     "mxfp4_dequant",
     "mxfp4_quantize",
@@ -442,3 +449,199 @@ class mxfp8_quantize(CustomOp):
         codes = torch.empty((x.shape[0], x.shape[1]), dtype=torch.uint8, device=x.device)
         scales = torch.empty((x.shape[0], x.shape[1] // 32), dtype=torch.uint8, device=x.device)
         return launch.mxfp8_quantize_out(x, codes, scales)
+
+
+# ---- a packed serving step around the paged cache --------------------------------------------------------------------
+
+
+@CustomOp.register
+class paged_batch_layout(CustomOp):
+    """Block tables and slot maps of a step from request lengths, on the device: sequence s holds context_lens[s] tokens and
+    adds new_lens[s]; the pages that the new tokens need come from the front of `free_pages` in sequence order and are
+    entered in `block_table` int32 [S, max_pages] in place (-1 where the list has run out).
+
+    Returns (seq_lens [S], cu_new [S + 1], positions [T], seq_ids [T], slots int64 [T], pages_needed [1]), int32 but for
+    the slots, T = num_tokens rows for the new tokens of all sequences in order; rows behind them are padding (0, -1, -1).
+    `slots` is what rope_kv_append takes, `cu_new` what flash_attn_varlen_fwd takes, `seq_lens` what the paged attention
+    ops take.  Tokens that find no row are not admitted.  The same call again gives the same results."""
+
+    signature = "paged_batch_layout(Tensor(a!) block_table, Tensor context_lens, Tensor new_lens, Tensor free_pages, int page_size, int num_tokens) -> (Tensor, Tensor, Tensor, Tensor, Tensor, Tensor)"
+
+    def select(self, sel: KernelSelection):
+        bt, cl, nl, fp = (sel.arg_tensor(i) for i in range(4))
+        page, T = sel.attr_int(4).v, sel.arg_int(5).v
+        contract.check_batch_layout("paged_batch_layout", bt.t, cl.t, nl.t, fp.t, page, T)
+        S = cl.t.size(0)
+        for n in (S, S + 1, T, T):
+            sel.return_new_tensor([n], torch.int32)
+        sel.return_new_tensor([T], torch.int64)
+        sel.return_new_tensor([1], torch.int32)
+
+    def eager_execute(self, block_table, context_lens, new_lens, free_pages, page_size, num_tokens):
+        S = context_lens.shape[0]
+        new = lambda n, dt=torch.int32: torch.empty(n, dtype=dt, device=block_table.device)
+        outs = (new(S), new(S + 1), new(num_tokens), new(num_tokens), new(num_tokens, torch.int64), new(1))
+        launch.paged_batch_layout_out(block_table, context_lens, new_lens, free_pages, page_size, *outs)
+        return outs
+
+
+def rope_inv_freq(rotary_dim: int, theta: float = 10000.0, scaling: str = "none", factor: float = 1.0, trained_len: int = 4096,
+                  device=None) -> tuple[Tensor, float]:
+    """(inv_freq float64 [rotary_dim / 2], scale) for `rope` and `rope_kv_append`: f_i = theta^(-2i / rotary_dim), stretched
+    for contexts `factor` times as long as the trained length.
+
+    scaling "none": as they are; "linear": f_i / factor (position interpolation); "ntk": theta times
+    factor^(rotary_dim / (rotary_dim - 2)), which leaves the fastest frequency and divides the slowest by `factor`;
+    "yarn": f_i for those that turn more than 32 times within trained_len, f_i / factor for those that turn less than
+    once, blended linearly in the number of turns between, and scale = 0.1 ln(factor) + 1 (Peng et al., 2023)."""
+    _require(rotary_dim > 0 and rotary_dim % 2 == 0 and rotary_dim <= contract.MAX_ROTARY_DIM, f"rope_inv_freq: rotary_dim {rotary_dim} must be even, in [2, {contract.MAX_ROTARY_DIM}]")
+    _require(theta > 0 and factor >= 1 and trained_len > 0, "rope_inv_freq: theta > 0, factor >= 1 and trained_len > 0 are required")
+    _require(scaling in ("none", "linear", "ntk", "yarn"), f"rope_inv_freq: scaling must be 'none', 'linear', 'ntk' or 'yarn', got {scaling!r}")
+    if scaling == "ntk" and rotary_dim > 2:
+        theta = theta * factor ** (rotary_dim / (rotary_dim - 2))
+    f = theta ** (-torch.arange(0, rotary_dim, 2, dtype=torch.float64) / rotary_dim)
+    scale = 1.0
+    if scaling == "linear":
+        f = f / factor
+    elif scaling == "yarn":
+        keep = ((f * trained_len / (2 * math.pi) - 1) / 31).clamp(0, 1)
+        f = f * keep + f / factor * (1 - keep)
+        scale = 0.1 * math.log(factor) + 1
+    return f.to(device) if device is not None else f, scale
+
+
+@CustomOp.register
+class rope(CustomOp):
+    """Rotary positions: the pairs of the first R = 2 len(inv_freq) elements of x [tokens, heads, D] (fp16, bf16 or fp32; any token
+    and head strides) turned by positions[token] * inv_freq[i], times `scale`; elements from R on pass through.  Pair i is
+    (2i, 2i + 1) when `interleaved`, else (i, i + R/2).  positions int32 [tokens]; inv_freq float64 or float32 (see
+    `rope_inv_freq`): angles are formed in 64 bits either way.  `inverse` turns back (times `scale`, not divided by it): the
+    gradient, which autograd takes for x; positions and inv_freq get none."""
+
+    signature = "rope(Tensor x, Tensor positions, Tensor inv_freq, bool interleaved, bool inverse, float scale) -> Tensor"
+
+    def select(self, sel: KernelSelection):
+        x, pos, freq = (sel.arg_tensor(i) for i in range(3))
+        sel.attr_bool(3)
+        sel.attr_bool(4)
+        sel.attr_float(5)
+        contract.check_rope("rope", x.t, pos.t, freq.t)
+        x.specialize_dims(1, 2)
+        sel.return_new_tensor(list(x.t.shape), x.t.dtype)
+
+    def eager_execute(self, x, positions, inv_freq, interleaved, inverse, scale):
+        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        return launch.rope_out(x, positions, inv_freq, out, interleaved, inverse, scale)
+
+
+def _rope_setup_context(ctx, inputs, output):
+    _, positions, inv_freq, ctx.interleaved, ctx.inverse, ctx.scale = inputs
+    ctx.save_for_backward(positions, inv_freq)
+
+
+def _rope_backward(ctx, grad):
+    """The rotation is linear in x: its transpose is the rotation by the negated angles."""
+    positions, inv_freq = ctx.saved_tensors
+    return torch.ops.mi355.rope(grad, positions, inv_freq, ctx.interleaved, not ctx.inverse, ctx.scale), None, None, None, None, None
+
+
+torch.library.register_autograd("mi355::rope", _rope_backward, setup_context=_rope_setup_context)
+
+
+@CustomOp.register
+class rope_kv_append(CustomOp):
+    """One pass over a step's projections: q [T, Hq, 128] rotated (the result), k_new [T, Hkv, 128] rotated and v_new as it is into
+    the rows `slots` int64 [T] of k_cache, v_cache [P, page, Hkv, 128] (page * page_size + place, as paged_batch_layout gives
+    them; -1 or anything outside the cache: that token is not stored).  q, k_new, v_new may be slices of a packed
+    projection.  Slots must differ.  Angles, layouts and `scale` as in `rope`."""
+
+    signature = "rope_kv_append(Tensor q, Tensor k_new, Tensor v_new, Tensor positions, Tensor inv_freq, Tensor(a!) k_cache, Tensor(b!) v_cache, Tensor slots, bool interleaved, float scale) -> Tensor"
+
+    def select(self, sel: KernelSelection):
+        q, kn, vn, pos, freq, kc, vc, sl = (sel.arg_tensor(i) for i in range(8))
+        sel.attr_bool(8)
+        sel.attr_float(9)
+        contract.check_rope_append("rope_kv_append", q.t, kn.t, vn.t, pos.t, freq.t, kc.t, vc.t, sl.t)
+        q.specialize_dims(1, 2)
+        sel.return_new_tensor(list(q.t.shape), q.t.dtype)
+
+    def eager_execute(self, q, k_new, v_new, positions, inv_freq, k_cache, v_cache, slots, interleaved, scale):
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        return launch.rope_kv_append_out(q, k_new, v_new, positions, inv_freq, k_cache, v_cache, slots, out, interleaved, scale)
+
+
+@CustomOp.register
+class flash_attn_varlen_fwd(CustomOp):
+    """flash_attn_fwd over packed sequences of different lengths: q [Tq, H, 128], k, v [Tk, Hkv, 128] (fp16 or bf16, H % Hkv == 0; slices
+    of a packed projection are read in place); sequence s is the rows cu_seqlens_q[s] .. cu_seqlens_q[s + 1] - 1 of q and
+    likewise of k and v (int32 [S + 1], non-decreasing).  is_causal aligns each sequence's mask to its last key, as
+    flash_attn_fwd does, so the earlier part of a prompt may stand in front of its keys.  scale <= 0 selects 1/sqrt(D).
+    Lengths stay on the device.  Queries without a visible key and rows outside every sequence give zeros."""
+
+    signature = "flash_attn_varlen_fwd(Tensor q, Tensor k, Tensor v, Tensor cu_seqlens_q, Tensor cu_seqlens_k, bool is_causal, float scale) -> Tensor"
+
+    def select(self, sel: KernelSelection):
+        q, k, v, cq, ck = (sel.arg_tensor(i) for i in range(5))
+        sel.attr_bool(5)
+        sel.attr_float(6)
+        contract.check_varlen_attention("flash_attn_varlen_fwd", q.t, k.t, v.t, cq.t, ck.t)
+        for d in (q, k, v):
+            d.specialize_dims(1, 2)
+        sel.return_new_tensor(list(q.t.shape), q.t.dtype)
+
+    def eager_execute(self, q, k, v, cu_seqlens_q, cu_seqlens_k, is_causal, scale):
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        return launch.flash_attn_varlen_fwd_out(q, k, v, cu_seqlens_q, cu_seqlens_k, out, is_causal, scale, zero_rest=True)
+
+
+@CustomOp.register
+class paged_tree_attn(CustomOp):
+    """Attention of drafted token trees over the paged cache: q [S, N, Hq, 128], N <= 64 nodes per sequence, whose K/V are the last N
+    tokens of the cache (seq_lens int32 [S] counts them); parents int32 [S, N] (a value outside [0, n) for node n: a root).
+    Node n sees every token in front of the drafts, its ancestors and itself; with parents[n] = n - 1 this is
+    paged_prefill_attn of N new tokens.  num_kv_splits <= 0 picks a default from the table width; scale <= 0 selects
+    1/sqrt(D).  Returns [S, N, Hq, 128]."""
+
+    signature = "paged_tree_attn(Tensor q, Tensor k_cache, Tensor v_cache, Tensor block_table, Tensor seq_lens, Tensor parents, float scale, int num_kv_splits) -> Tensor"
+
+    def select(self, sel: KernelSelection):
+        q, kc, vc, bt, sl, par = (sel.arg_tensor(i) for i in range(6))
+        sel.attr_float(6)
+        sel.attr_int(7)
+        contract.check_tree_attention("paged_tree_attn", q.t, kc.t, vc.t, bt.t, sl.t, par.t)
+        q.specialize_dims(1, 2, 3)
+        sel.return_new_tensor(list(q.t.shape), q.t.dtype)
+
+    def eager_execute(self, q, k_cache, v_cache, block_table, seq_lens, parents, scale, num_kv_splits):
+        if num_kv_splits <= 0:
+            num_kv_splits = default_num_kv_splits(block_table.shape[1] * k_cache.shape[1], q.shape[0], k_cache.shape[2])
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        return launch.paged_tree_attn_out(q, k_cache, v_cache, block_table, seq_lens, parents, out, scale, num_kv_splits)
+
+
+@CustomOp.register
+class verify_draft(CustomOp):
+    """Which drafted tokens the target model accepts, and the token behind them, from given random numbers: speculative sampling
+    over a tree (a chain has parents[n] = n - 1).  target_probs float32 [S, N, V], row n the target's distribution behind node
+    n, node 0 the last certain token; draft_probs the same shape, row n what node n's children were drawn from, or None for
+    drafts that were certain; tokens, parents int32 [S, N]; uniforms float32 [S, N] in [0, 1): entry n > 0 decides node n,
+    entry 0 draws the next token.
+
+    Returns (path [S, N], num_accepted [S], next_token [S]) int32: the accepted nodes in order, then -1.  The rule stands at
+    mi355_verify_draft; sums and comparisons are in 64 bits.  With parents as given to paged_tree_attn."""
+
+    signature = "verify_draft(Tensor target_probs, Tensor? draft_probs, Tensor tokens, Tensor parents, Tensor uniforms) -> (Tensor, Tensor, Tensor)"
+
+    def select(self, sel: KernelSelection):
+        tp, tok, par, u = (sel.arg_tensor(i) for i in (0, 2, 3, 4))
+        dp = sel.arg_optional_tensor(1)
+        contract.check_verify_draft("verify_draft", tp.t, dp.t if isinstance(dp, TensorArg) else None, tok.t, par.t, u.t)
+        S, N, _ = tp.t.shape
+        sel.return_new_tensor([S, N], torch.int32)
+        sel.return_new_tensor([S], torch.int32)
+        sel.return_new_tensor([S], torch.int32)
+
+    def eager_execute(self, target_probs, draft_probs, tokens, parents, uniforms):
+        S, N, _ = target_probs.shape
+        new = lambda *n: torch.empty(n, dtype=torch.int32, device=target_probs.device)
+        return launch.verify_draft_out(target_probs, draft_probs, tokens, parents, uniforms, new(S, N), new(S), new(S))
