@@ -35,57 +35,14 @@ struct FaLayout {
   int H, group;
 };
 
-// Packed sequences of different lengths (the VARLEN form): the queries of sequence s are the rows [cu_q[s], cu_q[s + 1]) of
-// one token stream, its keys and values the rows [cu_k[s], cu_k[s + 1]) of another.
-struct FaVarlen {
-  const int *cu_q, *cu_k;  // [num_seqs + 1]
-  int num_seqs, total_q, total_k;
-  int zero_rest;           // also write zeros to the query rows in front of the first and behind the last sequence
-};
-
-// Rows [begin, begin + len) of sequence s; offsets outside the stream are cut to it, a negative length counts as 0.
-__device__ __forceinline__ int fa_seq_range(const int* cu, int s, int total, int& begin) {
-  int b = cu[s], e = cu[s + 1];
-  b = b < 0 ? 0 : (b > total ? total : b);
-  e = e < b ? b : (e > total ? total : e);
-  begin = b;
-  return e - b;
-}
-
-// The sequence that holds unit number `unit` when sequence s has ceil(len_s / rows) units, in order, and the unit's
-// number inside it; -1 behind the last one.  Every wave finds it by itself, 64 sequences at a time.
-__device__ __forceinline__ int fa_find_unit(const FaVarlen& vl, int rows, int unit, int& inside) {
-  const int lane = threadIdx.x & 63;
-  int base = 0;
-  for (int s0 = 0; s0 < vl.num_seqs; s0 += 64) {
-    int begin, n = 0;
-    if (s0 + lane < vl.num_seqs) n = (fa_seq_range(vl.cu_q, s0 + lane, vl.total_q, begin) + rows - 1) / rows;
-    int incl = n;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-      const int up = __shfl_up(incl, d);
-      if (lane >= d) incl += up;
-    }
-    const unsigned long long past = __builtin_amdgcn_ballot_w64(base + incl > unit);
-    if (past) {
-      const int l = __builtin_ctzll(past);
-      inside = __builtin_amdgcn_readfirstlane(unit - base - __shfl(incl - n, l));
-      return s0 + l;
-    }
-    base += __shfl(incl, 63);
-  }
-  return -1;
-}
-
-template <bool CAUSAL, bool BF, bool VARLEN = false>
+template <bool CAUSAL, bool BF>
 __global__ __launch_bounds__(256) void fa_fwd_d128(const half_t* __restrict__ Q, const half_t* __restrict__ K,
-                                                   const half_t* __restrict__ V, half_t* __restrict__ O, int BH, int Sq_arg,
-                                                   int Sk_arg, float scale_log2e, int q_blocks, FaLayout lay, FaVarlen vl) {
+                                                   const half_t* __restrict__ V, half_t* __restrict__ O, int BH, int Sq,
+                                                   int Sk, float scale_log2e, int q_blocks, FaLayout lay) {
   extern __shared__ __attribute__((aligned(1024))) char lds[];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int r32 = lane & 31, h = lane >> 5;
-  int Sq = Sq_arg, Sk = Sk_arg;
 
   // workgroup -> (batch*head, query block).  Consecutive ids land on different XCDs; keep all
   // query blocks of one head on one XCD so its K/V stay in that XCD's L2.
@@ -102,31 +59,7 @@ __global__ __launch_bounds__(256) void fa_fwd_d128(const half_t* __restrict__ Q,
       bh = pid / q_blocks;
       qb = pid % q_blocks;
     }
-    if (CAUSAL && !VARLEN) qb = q_blocks - 1 - qb;  // longest rows first
-  }
-  int b_idx = VARLEN ? 0 : bh / lay.H;
-  const int h_idx = bh - b_idx * lay.H, hk_idx = h_idx / lay.group;
-  size_t q_base = 0, k_base_row = 0;
-  if constexpr (VARLEN) {
-    if (vl.zero_rest) {
-      int first, last;
-      fa_seq_range(vl.cu_q, 0, vl.total_q, first);
-      const int len = fa_seq_range(vl.cu_q, vl.num_seqs - 1, vl.total_q, last);
-      last += len;
-      const int outside = first + vl.total_q - last;
-      for (int i = qb; i < outside; i += q_blocks) {
-        half_t* row = O + (size_t)(i < first ? i : last + i - first) * lay.o_r + h_idx * lay.o_h;
-        if (threadIdx.x < 128) row[threadIdx.x] = (half_t)0;
-      }
-    }
-    int inside = 0, q_first, k_first;
-    const int seq = fa_find_unit(vl, FA_BLOCK_M, qb, inside);
-    if (seq < 0) return;
-    Sq = __builtin_amdgcn_readfirstlane(fa_seq_range(vl.cu_q, seq, vl.total_q, q_first));
-    Sk = __builtin_amdgcn_readfirstlane(fa_seq_range(vl.cu_k, seq, vl.total_k, k_first));
-    qb = inside;
-    q_base = (size_t)__builtin_amdgcn_readfirstlane(q_first);
-    k_base_row = (size_t)__builtin_amdgcn_readfirstlane(k_first);
+    if (CAUSAL) qb = q_blocks - 1 - qb;  // longest rows first
   }
   const int causal_off = Sk - Sq;  // query i sees keys <= i + causal_off
   const int q0 = qb * FA_BLOCK_M;
@@ -134,10 +67,11 @@ __global__ __launch_bounds__(256) void fa_fwd_d128(const half_t* __restrict__ Q,
   const int q_row = wq0 + r32;
   const bool q_ok = q_row < Sq;
 
-  const half_t* Qb = Q + b_idx * lay.q_b + h_idx * lay.q_h + q_base * lay.q_r;
-  const half_t* Kb = K + b_idx * lay.k_b + hk_idx * lay.k_h + k_base_row * lay.k_r;
-  const half_t* Vb = V + b_idx * lay.v_b + hk_idx * lay.v_h + k_base_row * lay.v_r;
-  half_t* Ob = O + b_idx * lay.o_b + h_idx * lay.o_h + q_base * lay.o_r;
+  const int b_idx = bh / lay.H, h_idx = bh - b_idx * lay.H, hk_idx = h_idx / lay.group;
+  const half_t* Qb = Q + b_idx * lay.q_b + h_idx * lay.q_h;
+  const half_t* Kb = K + b_idx * lay.k_b + hk_idx * lay.k_h;
+  const half_t* Vb = V + b_idx * lay.v_b + hk_idx * lay.v_h;
+  half_t* Ob = O + b_idx * lay.o_b + h_idx * lay.o_h;
 
   // number of key tiles this workgroup walks
   int k_end = Sk;
@@ -646,6 +580,74 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
 }
 
 
+// Packed sequences of different lengths (the VARLEN form of fa_fwd_d128_m16): the queries of sequence s are the rows
+// [cu_q[s], cu_q[s + 1]) of one token stream, its keys and values the rows [cu_k[s], cu_k[s + 1]) of another.
+struct FaVarlen {
+  const int *cu_q, *cu_k;  // [num_seqs + 1]
+  int num_seqs, total_q, total_k;
+  int zero_rest;           // also write zeros to the query rows in front of the first and behind the last sequence
+  int pairs;               // (causal) a unit is a pair of query blocks, else one block
+};
+
+// Rows [begin, begin + len) of sequence s; offsets outside the stream are cut to it, a negative length counts as 0.
+__device__ __forceinline__ int fa_seq_range(const int* cu, int s, int total, int& begin) {
+  int b = cu[s], e = cu[s + 1];
+  b = b < 0 ? 0 : (b > total ? total : b);
+  e = e < b ? b : (e > total ? total : e);
+  begin = b;
+  return e - b;
+}
+
+// The sequence whose units hold place `loc` when every unit takes `per_unit` places (its heads), and the place inside the
+// sequence's; -1 behind the last.  Sequences come in order of falling key length as far as one wave can rank them
+// (64), so that short ones make up the tail of the grid; more than 64 come as they are.  `block_rows` query rows make a block,
+// one or two blocks a unit.  Every wave finds the place by itself, one sequence per lane.
+__device__ __forceinline__ int fa_find_unit(const FaVarlen& vl, int block_rows, int per_unit, int loc, int& inside, int& units) {
+  const int lane = threadIdx.x & 63;
+  auto units_of = [&](int s, int& key) {
+    int begin;
+    const int blocks = (fa_seq_range(vl.cu_q, s, vl.total_q, begin) + block_rows - 1) / block_rows;
+    key = fa_seq_range(vl.cu_k, s, vl.total_k, begin);
+    return vl.pairs ? (blocks + 1) >> 1 : blocks;
+  };
+  int base = 0;
+  if (vl.num_seqs <= 64) {
+    int key = -1, n = 0, before = 0;
+    if (lane < vl.num_seqs) n = units_of(lane, key);
+    for (int j = 0; j < vl.num_seqs; j++) {
+      const int kj = __builtin_amdgcn_readlane(key, j), nj = __builtin_amdgcn_readlane(n, j);
+      before += (kj > key || (kj == key && j < lane)) ? nj : 0;
+    }
+    const int at = loc / per_unit;
+    const unsigned long long hit = __builtin_amdgcn_ballot_w64(before <= at && at < before + n);
+    if (!hit) return -1;
+    const int l = __builtin_ctzll(hit);
+    inside = loc - __builtin_amdgcn_readlane(before, l) * per_unit;
+    units = __builtin_amdgcn_readlane(n, l);
+    return l;
+  }
+  const int at = loc / per_unit;
+  for (int s0 = 0; s0 < vl.num_seqs; s0 += 64) {
+    int key, n = 0;
+    if (s0 + lane < vl.num_seqs) n = units_of(s0 + lane, key);
+    int incl = n;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const int up = __shfl_up(incl, d);
+      if (lane >= d) incl += up;
+    }
+    const unsigned long long past = __builtin_amdgcn_ballot_w64(base + incl > at);
+    if (past) {
+      const int l = __builtin_ctzll(past);
+      units = __builtin_amdgcn_readlane(n, l);
+      inside = loc - (base + __builtin_amdgcn_readlane(incl, l) - units) * per_unit;
+      return s0 + l;
+    }
+    base += __builtin_amdgcn_readlane(incl, 63);
+  }
+  return -1;
+}
+
 // The pipelined form on v_mfma_f32_16x16x32 (variant "..._m16").  Same tiles, rings, loads, passes and barriers as
 // fa_fwd_d128_pipe; what changes is the MFMA shape and with it every fragment layout.  On benchmark-like data a
 // 16x16x32 MFMA costs the board less energy per flop than a 32x32x16 (register-only loops with this tile's structure:
@@ -665,10 +667,10 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
 // the score MFMAs (vector work behind 48 of the trip's 64 MFMAs instead of 32).  Measured on 2 x 32 x 4096: ahead with
 // eight waves (unmasked 475 against 484 us), behind with four (causal 268 against 263); each form is built the way it
 // runs faster.
-template <bool CAUSAL, bool BF, int NW, bool SPREAD, bool PAGED = false>
+template <bool CAUSAL, bool BF, int NW, bool SPREAD, bool PAGED = false, bool VARLEN = false>
 __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2))) void fa_fwd_d128_m16(
     const half_t* __restrict__ Q, const half_t* __restrict__ K, const half_t* __restrict__ V, half_t* __restrict__ O, int BH,
-    int Sq, int Sk_arg, float scale_log2e, int q_blocks, FaLayout lay, FaPaged pg) {
+    int Sq_arg, int Sk_arg, float scale_log2e, int q_blocks_arg, FaLayout lay, std::conditional_t<VARLEN, FaVarlen, FaPaged> pg) {
   extern __shared__ __attribute__((aligned(1024))) char lds[];
   static_assert(NW == 4 || !PAGED, "the paged form maps one page to one wave-load of a 4-wave workgroup");
   constexpr int BLOCK_M = NW * 32, NI = 16 / NW;
@@ -677,9 +679,45 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int q16 = lane & 15, g = lane >> 4;
 
-  const int units = CAUSAL ? (q_blocks + 1) / 2 : q_blocks;
-  int bh, unit;
-  {
+  int Sq = Sq_arg, Sk = Sk_arg, q_blocks = q_blocks_arg;
+  int units = CAUSAL ? (q_blocks + 1) / 2 : q_blocks;
+  int bh, unit, b_idx, h_idx;
+  size_t q_first = 0, k_first = 0;  // (VARLEN) the sequence's first rows
+  if constexpr (VARLEN) {
+    const int pid = blockIdx.x;
+    if (pg.zero_rest) {
+      int first, last;
+      fa_seq_range(pg.cu_q, 0, pg.total_q, first);
+      const int len = fa_seq_range(pg.cu_q, pg.num_seqs - 1, pg.total_q, last);
+      last += len;
+      const long long outside = (long long)(first + pg.total_q - last) * lay.H;  // head rows, sixteen lanes each
+      for (long long i = (long long)pid * (NW * 4) + (threadIdx.x >> 4); i < outside; i += (long long)gridDim.x * (NW * 4)) {
+        const int r = (int)(i / lay.H), hd = (int)(i - (long long)r * lay.H);
+        half_t* row = O + (size_t)(r < first ? r : last + r - first) * lay.o_r + hd * lay.o_h;
+        *reinterpret_cast<half8*>(row + q16 * 8) = half8{};
+      }
+    }
+    // The heads that share a K/V head sit on one XCD when the K/V heads divide over the eight; a sequence's heads follow
+    // each other, a head's units too.
+    const bool spread = (lay.H / lay.group) % 8 == 0;
+    const int xcd = pid & 7, per_unit = spread ? lay.H / 8 : lay.H;
+    int inside;
+    const int seq = fa_find_unit(pg, BLOCK_M, per_unit, spread ? pid >> 3 : pid, inside, units);
+    if (seq < 0) return;
+    h_idx = inside / units;
+    unit = inside - h_idx * units;
+    if (spread) {
+      const int kv = h_idx / lay.group;
+      h_idx = (kv * 8 + xcd) * lay.group + (h_idx - kv * lay.group);
+    }
+    int row;
+    Sq = fa_seq_range(pg.cu_q, seq, pg.total_q, row);
+    q_first = row;
+    Sk = fa_seq_range(pg.cu_k, seq, pg.total_k, row);
+    k_first = row;
+    q_blocks = (Sq + BLOCK_M - 1) / BLOCK_M;
+    bh = b_idx = 0;
+  } else {
     const int pid = blockIdx.x;
     if (((BH / lay.group) & 7) == 0) {
       const int xcd = pid & 7, loc = pid >> 3, per_kv = units * lay.group;
@@ -690,10 +728,10 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
       bh = pid / units;
       unit = pid % units;
     }
+    b_idx = bh / lay.H;
+    h_idx = bh - b_idx * lay.H;
   }
-  int b_idx = bh / lay.H;
-  const int h_idx = bh - b_idx * lay.H, hk_idx = h_idx / lay.group;
-  int Sk = Sk_arg;
+  const int hk_idx = h_idx / lay.group;
   if constexpr (PAGED) {
     // Sequences differ in length and workgroups are dispatched in grid order: take the sequences longest first,
     // so that the short ones make up the tail.  Thread t counts the sequences that come before sequence t.
@@ -719,10 +757,10 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
     Sk = Sk < 0 ? 0 : (Sk > cap ? cap : Sk);
   }
   const int causal_off = Sk - Sq;
-  const half_t* Qb = Q + b_idx * lay.q_b + h_idx * lay.q_h;
-  const half_t* Kb = K + (PAGED ? 0 : b_idx * lay.k_b) + hk_idx * lay.k_h;
-  const half_t* Vb = V + (PAGED ? 0 : b_idx * lay.v_b) + hk_idx * lay.v_h;
-  half_t* Ob = O + b_idx * lay.o_b + h_idx * lay.o_h;
+  const half_t* Qb = Q + (VARLEN ? q_first * lay.q_r : b_idx * lay.q_b) + h_idx * lay.q_h;
+  const half_t* Kb = K + (PAGED ? 0 : VARLEN ? k_first * lay.k_r : b_idx * lay.k_b) + hk_idx * lay.k_h;
+  const half_t* Vb = V + (PAGED ? 0 : VARLEN ? k_first * lay.v_r : b_idx * lay.v_b) + hk_idx * lay.v_h;
+  half_t* Ob = O + (VARLEN ? q_first * lay.o_r : b_idx * lay.o_b) + h_idx * lay.o_h;
 
   // fragment read addresses, opaque (see fa_fwd_d128_pipe): K by step over d, V by d group
   typedef const __attribute__((address_space(3))) half8* lds_half8_t;
@@ -743,7 +781,9 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
     }
   }
 
-  for (int pass = 0; pass < (CAUSAL ? 2 : 1); pass++) {
+  int passes = CAUSAL ? 2 : 1;
+  if constexpr (VARLEN) passes = pg.pairs ? 2 : 1;
+  for (int pass = 0; pass < passes; pass++) {
   const int qb = CAUSAL ? (pass == 0 ? q_blocks - 1 - unit : unit) : unit;
   if (CAUSAL && pass == 1 && 2 * unit == q_blocks - 1) break;
   const int q0 = qb * BLOCK_M;
@@ -785,8 +825,8 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
   // paged form: page ids come through the scalar cache (constant address space: the table is not written while the
   // kernel runs), one tile ahead of their use, so that no K/V load waits for a table read
   typedef const int __attribute__((address_space(4)))* table_ptr_t;
-  const table_ptr_t table_row =
-      PAGED ? (table_ptr_t)(unsigned long long)(pg.block_table + (size_t)b_idx * pg.max_pages) : (table_ptr_t)0;
+  table_ptr_t table_row = (table_ptr_t)0;
+  if constexpr (PAGED) table_row = (table_ptr_t)(unsigned long long)(pg.block_table + (size_t)b_idx * pg.max_pages);
   auto load_ids = [&](int tile, int* ids) {
     if constexpr (PAGED) {
 #pragma unroll
@@ -1057,7 +1097,7 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
     // bytes in a private region (chunk c of row r in slot c ^ (r & 15)) from 8-byte pieces -- the lane holds d = 16 dg +
     // 4 g .. + 3 of its query in either group -- and stores whole rows, 16 bytes per lane.
     char* ep = lds + wave * 8192;
-    const int el = CAUSAL ? opaque_lane_id() : lane;  // (see fa_fwd_d128_pipe)
+    const int el = (CAUSAL || VARLEN) ? opaque_lane_id() : lane;  // (see fa_fwd_d128_pipe)
     const int e16 = el & 15, eg = el >> 4;
 #pragma unroll
     for (int qg = 0; qg < 2; qg++) {
@@ -1590,7 +1630,7 @@ static int fa_launch(const void* q, const void* k, const void* v, void* o, int64
   if (variant == 1) {
     auto kern = is_causal ? fa_fwd_d128<true, BF> : fa_fwd_d128<false, BF>;
     hipLaunchKernelGGL(kern, grid, block, lds_bytes, s, (const half_t*)q, (const half_t*)k, (const half_t*)v, (half_t*)o, BH,
-                       (int)Sq, (int)Sk, scale_log2e, q_blocks, lay, FaVarlen{});
+                       (int)Sq, (int)Sk, scale_log2e, q_blocks, lay);
   } else {
     auto kern = is_causal ? fa_fwd_d128_pipe<true, BF> : fa_fwd_d128_pipe<false, BF>;
     hipLaunchKernelGGL(kern, grid, block, lds_bytes, s, (const half_t*)q, (const half_t*)k, (const half_t*)v, (half_t*)o, BH,
@@ -1751,18 +1791,22 @@ static int fa_varlen(const void* q, const void* k, const void* v, void* o, const
   lay.v_h = v_strides[1], lay.v_r = (unsigned)v_strides[0];
   lay.o_h = o_strides[1], lay.o_r = (unsigned)o_strides[0];
   lay.H = (int)H, lay.group = (int)(H / Hkv);
-  const FaVarlen vl{cu_q, cu_k, (int)num_seqs, (int)total_q, (int)total_k, zero_rest};
-  // the lengths are known on the device only: as many blocks as num_seqs sequences of total_q rows can have
-  const int64_t blocks = total_q / FA_BLOCK_M + num_seqs;
-  if (blocks * H >= (1ll << 31)) return fail(-MI355_E_SHAPE, "%s: too many query blocks", who);
-  auto kern = is_causal ? fa_fwd_d128<true, BF, true> : fa_fwd_d128<false, BF, true>;
+  // With the mask, a pair of blocks (the i-th from the end and the i-th from the start) is the same work everywhere in a sequence,
+  // and half as many workgroups; where even single blocks would not fill the chip twice (512 workgroups are resident), they
+  // are handed out singly.
+  const int pairs = is_causal && total_q / FA_BLOCK_M * H >= 2048;
+  const FaVarlen vl{cu_q, cu_k, (int)num_seqs, (int)total_q, (int)total_k, zero_rest, pairs};
+  // the lengths are known on the device only: as many units as num_seqs sequences of total_q rows can have
+  const int64_t units = total_q / (FA_BLOCK_M << pairs) + num_seqs;
+  if (units * H >= (1ll << 31)) return fail(-MI355_E_SHAPE, "%s: too many query blocks", who);
+  auto kern = is_causal ? fa_fwd_d128_m16<true, BF, 4, false, false, true> : fa_fwd_d128_m16<false, BF, 4, false, false, true>;
   const int lds_bytes = 2 * FA_STAGE;
   static std::atomic<uint64_t> lds_ok[2] = {};
-  if (int rc = allow_lds(reinterpret_cast<const void*>(kern), lds_bytes, lds_ok[is_causal ? 1 : 0], "fa_fwd_d128<varlen>")) return rc;
-  dim3 grid((unsigned)(blocks * H)), block(256);
+  if (int rc = allow_lds(reinterpret_cast<const void*>(kern), lds_bytes, lds_ok[is_causal ? 1 : 0], "fa_fwd_d128_m16<varlen>")) return rc;
+  dim3 grid((unsigned)(units * H)), block(256);
   hipLaunchKernelGGL(kern, grid, block, lds_bytes, reinterpret_cast<hipStream_t>(stream), (const half_t*)q, (const half_t*)k,
-                     (const half_t*)v, (half_t*)o, (int)H, 0, 0, scale * 1.4426950408889634f, (int)blocks, lay, vl);
-  return check_launch("fa_fwd_d128<varlen>", grid, block, lds_bytes);
+                     (const half_t*)v, (half_t*)o, (int)H, 0, 0, scale * 1.4426950408889634f, 0, lay, vl);
+  return check_launch("fa_fwd_d128_m16<varlen>", grid, block, lds_bytes);
 }
 
 extern "C" int mi355_flash_attn_varlen_fwd(const void* q, const void* k, const void* v, void* o, const int32_t* cu_seqlens_q,
