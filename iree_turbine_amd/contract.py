@@ -150,85 +150,141 @@ def check_quantize_input(op: str, x: Tensor) -> None:
 MAX_TREE_NODES = 64  # drafted nodes per sequence: a node's set of ancestors is one 64-bit word
 MAX_ROTARY_DIM = 1024
 
+# The checks below stand in front of calls that take a few microseconds: a message is formatted only when it is raised.
 
-def _check_int32(op: str, name: str, t: Tensor, shape: tuple) -> None:
-    require(t.dtype == torch.int32 and tuple(t.shape) == shape, f"{op}: {name} must be int32 {list(shape)}, got {t.dtype} {tuple(t.shape)}")
+
+def refuse(op: str, msg: str) -> None:
+    raise ValueError(f"{op}: {msg}")
+
+
+def _check_int32(op: str, name: str, t: Tensor, *shape: int) -> None:
+    if t.dtype != torch.int32 or t.shape != shape:
+        refuse(op, f"{name} must be int32 {list(shape)}, got {t.dtype} {tuple(t.shape)}")
+
+
+def _check_caches(op: str, k_cache: Tensor, v_cache: Tensor) -> None:
+    if k_cache.dim() != 4 or v_cache.shape != k_cache.shape:
+        refuse(op, "k_cache / v_cache must both be [num_pages, page_size, num_kv_heads, D]")
+    _, page, hkv, D = k_cache.shape
+    if D != 128:
+        refuse(op, f"head dim must be 128, got {D}")
+    if page not in PAGE_SIZES:
+        refuse(op, f"page size {page} not supported {PAGE_SIZES}")
+    if k_cache.size(0) == 0 or hkv == 0:
+        refuse(op, "empty cache")
 
 
 def check_varlen_attention(op: str, q: Tensor, k: Tensor, v: Tensor, cu_q: Tensor, cu_k: Tensor) -> None:
-    require(q.dim() == 3 and k.dim() == 3 and v.dim() == 3, f"{op}: q must be [total_q, H, D], k and v [total_k, Hkv, D]")
-    require(same_half_dtype((q, k, v)), f"{op}: q, k, v must all be float16 or all bfloat16")
-    require(q.size(2) == 128 and k.size(2) == 128, f"{op}: head dim must be 128")
-    require(k.shape == v.shape, f"{op}: k and v shapes differ")
-    require(k.size(1) > 0 and q.size(1) > 0 and q.size(1) % k.size(1) == 0, f"{op}: {q.size(1)} query heads over {k.size(1)} key/value heads")
-    require(0 < q.size(0) <= 1 << 24 and 0 < k.size(0) <= 1 << 24, f"{op}: q and k need 1 to 2^24 rows, got {q.size(0)} and {k.size(0)}")
-    require(cu_q.dim() == 1 and 2 <= cu_q.size(0) <= 65536, f"{op}: cu_seqlens_q must be int32 [num_seqs + 1] with 1 to 65535 sequences")
-    _check_int32(op, "cu_seqlens_q", cu_q, (cu_q.size(0),))
-    _check_int32(op, "cu_seqlens_k", cu_k, (cu_q.size(0),))
+    if q.dim() != 3 or k.dim() != 3 or v.dim() != 3:
+        refuse(op, "q must be [total_q, H, D], k and v [total_k, Hkv, D]")
+    if not same_half_dtype((q, k, v)):
+        refuse(op, "q, k, v must all be float16 or all be bfloat16")
+    (tq, h, d), (tk, hkv, dk) = q.shape, k.shape
+    if d != 128 or dk != 128:
+        refuse(op, f"head dim must be 128, got {d} and {dk}")
+    if v.shape != k.shape:
+        refuse(op, "k and v shapes differ")
+    if hkv == 0 or h == 0 or h % hkv or h > 65535:
+        refuse(op, f"{h} query heads over {hkv} key/value heads")
+    if not (0 < tq <= 1 << 24 and 0 < tk <= 1 << 24):
+        refuse(op, f"q and k need 1 to 2^24 rows, got {tq} and {tk}")
+    if cu_q.dim() != 1 or not 2 <= cu_q.size(0) <= 65536:
+        refuse(op, "cu_seqlens_q must be int32 [num_seqs + 1] with 1 to 65535 sequences")
+    _check_int32(op, "cu_seqlens_q", cu_q, cu_q.size(0))
+    _check_int32(op, "cu_seqlens_k", cu_k, cu_q.size(0))
 
 
 def check_tree_attention(op: str, q: Tensor, k_cache: Tensor, v_cache: Tensor, block_table: Tensor, seq_lens: Tensor, parents: Tensor) -> None:
-    require(q.dim() == 4, f"{op}: q must be [num_seqs, num_nodes, num_q_heads, D]")
-    require(k_cache.dim() == 4 and v_cache.shape == k_cache.shape, f"{op}: k_cache / v_cache must both be [num_pages, page_size, num_kv_heads, D]")
-    require(same_half_dtype((q, k_cache, v_cache)), f"{op}: q, k_cache, v_cache must all be float16 or all bfloat16")
-    require(q.size(3) == 128 and k_cache.size(3) == 128, f"{op}: head dim must be 128")
-    require(k_cache.size(1) in PAGE_SIZES, f"{op}: page size {k_cache.size(1)} not supported {PAGE_SIZES}")
-    hq, hkv = q.size(2), k_cache.size(2)
-    require(hkv > 0 and hq > 0 and hq % hkv == 0 and hq // hkv <= 128, f"{op}: {hq} q heads over {hkv} kv heads is not supported (a multiple, up to 128)")
-    require(1 <= q.size(1) <= MAX_TREE_NODES, f"{op}: {q.size(1)} nodes per sequence, supported: 1 to {MAX_TREE_NODES}")
-    check_block_table(op, block_table, seq_lens, q.size(0))
-    _check_int32(op, "parents", parents, (q.size(0), q.size(1)))
-    require(k_cache.size(0) > 0, f"{op}: empty cache")
+    if q.dim() != 4:
+        refuse(op, "q must be [num_seqs, num_nodes, num_q_heads, D]")
+    if not same_half_dtype((q, k_cache, v_cache)):
+        refuse(op, "q, k_cache, v_cache must all be float16 or all be bfloat16")
+    _check_caches(op, k_cache, v_cache)
+    S, N, hq, D = q.shape
+    hkv = k_cache.size(2)
+    if D != 128:
+        refuse(op, f"head dim must be 128, got {D}")
+    if hq == 0 or hq % hkv or hq // hkv > 128:
+        refuse(op, f"{hq} q heads over {hkv} kv heads is not supported (a multiple, up to 128)")
+    if not 1 <= N <= MAX_TREE_NODES:
+        refuse(op, f"{N} nodes per sequence, supported: 1 to {MAX_TREE_NODES}")
+    if block_table.dim() != 2 or block_table.dtype != torch.int32 or seq_lens.dtype != torch.int32 or block_table.size(0) != S or seq_lens.shape != (S,) \
+            or S == 0 or block_table.size(1) == 0:
+        check_block_table(op, block_table, seq_lens, S)
+    _check_int32(op, "parents", parents, S, N)
 
 
 def check_verify_draft(op: str, target_probs: Tensor, draft_probs: Tensor | None, tokens: Tensor, parents: Tensor, uniforms: Tensor) -> None:
-    require(target_probs.dim() == 3 and target_probs.dtype == torch.float32, f"{op}: target_probs must be float32 [num_seqs, num_nodes, vocab]")
+    if target_probs.dim() != 3 or target_probs.dtype != torch.float32:
+        refuse(op, "target_probs must be float32 [num_seqs, num_nodes, vocab]")
     S, N, V = target_probs.shape
-    require(1 <= S <= 65535 and 1 <= N <= MAX_TREE_NODES and 1 <= V <= 1 << 24,
-            f"{op}: {S} sequences of {N} nodes over {V} tokens, supported: 1 to 65535, 1 to {MAX_TREE_NODES}, 1 to 2^24")
-    if draft_probs is not None:
-        require(draft_probs.dtype == torch.float32 and draft_probs.shape == target_probs.shape, f"{op}: draft_probs must be float32 {[S, N, V]}")
-    _check_int32(op, "tokens", tokens, (S, N))
-    _check_int32(op, "parents", parents, (S, N))
-    require(uniforms.dtype == torch.float32 and tuple(uniforms.shape) == (S, N), f"{op}: uniforms must be float32 {[S, N]}")
+    if not (1 <= S <= 65535 and 1 <= N <= MAX_TREE_NODES and 1 <= V <= 1 << 24):
+        refuse(op, f"{S} sequences of {N} nodes over {V} tokens, supported: 1 to 65535, 1 to {MAX_TREE_NODES}, 1 to 2^24")
+    if draft_probs is not None and (draft_probs.dtype != torch.float32 or draft_probs.shape != target_probs.shape):
+        refuse(op, f"draft_probs must be float32 {[S, N, V]}")
+    _check_int32(op, "tokens", tokens, S, N)
+    _check_int32(op, "parents", parents, S, N)
+    if uniforms.dtype != torch.float32 or uniforms.shape != (S, N):
+        refuse(op, f"uniforms must be float32 {[S, N]}")
 
 
 def check_batch_layout(op: str, block_table: Tensor, context_lens: Tensor, new_lens: Tensor, free_pages: Tensor, page_size: int, num_tokens: int) -> None:
-    check_block_table(op, block_table, context_lens, context_lens.size(0) if context_lens.dim() == 1 else -1, "context_lens")
-    S = context_lens.size(0)
-    require(S <= 65535 and block_table.size(1) <= 1 << 22, f"{op}: at most 65535 sequences of 2^22 pages")
-    require(block_table.is_contiguous(), f"{op}: block_table is written in place and must be contiguous")
-    _check_int32(op, "new_lens", new_lens, (S,))
-    require(free_pages.dim() == 1 and free_pages.dtype == torch.int32 and free_pages.size(0) <= 1 << 30, f"{op}: free_pages must be int32 [num_free]")
-    require(page_size in PAGE_SIZES, f"{op}: page size {page_size} not supported {PAGE_SIZES}")
-    require(1 <= num_tokens <= 1 << 30, f"{op}: num_tokens must be in [1, 2^30], got {num_tokens}")
+    if block_table.dim() != 2 or block_table.dtype != torch.int32 or context_lens.dtype != torch.int32 or context_lens.shape != block_table.shape[:1] \
+            or block_table.numel() == 0:
+        check_block_table(op, block_table, context_lens, block_table.size(0) if block_table.dim() == 2 else -1, "context_lens")
+    S, W = block_table.shape
+    if S > 65535 or W > 1 << 22:
+        refuse(op, f"at most 65535 sequences of 2^22 pages, got {S} of {W}")
+    if not block_table.is_contiguous():
+        refuse(op, "block_table is written in place and must be contiguous")
+    _check_int32(op, "new_lens", new_lens, S)
+    if free_pages.dim() != 1 or free_pages.dtype != torch.int32 or free_pages.size(0) > 1 << 30:
+        refuse(op, "free_pages must be int32 [num_free]")
+    if page_size not in PAGE_SIZES:
+        refuse(op, f"page size {page_size} not supported {PAGE_SIZES}")
+    if not 1 <= num_tokens <= 1 << 30:
+        refuse(op, f"num_tokens must be in [1, 2^30], got {num_tokens}")
 
 
-def check_rope(op: str, x: Tensor, positions: Tensor, inv_freq: Tensor, dtypes=(torch.float16, torch.bfloat16, torch.float32)) -> None:
-    require(x.dim() == 3 and x.dtype in dtypes, f"{op}: x must be [tokens, heads, D] in {', '.join(str(d).removeprefix('torch.') for d in dtypes)}, got {x.dtype} {tuple(x.shape)}")
+ROPE_DTYPES = (torch.float16, torch.bfloat16, torch.float32)
+
+
+def check_rope(op: str, x: Tensor, positions: Tensor, inv_freq: Tensor) -> None:
+    if x.dim() != 3 or x.dtype not in ROPE_DTYPES:
+        refuse(op, f"x must be [tokens, heads, D] in float16, bfloat16 or float32, got {x.dtype} {tuple(x.shape)}")
     T, H, D = x.shape
-    require(T > 0 and 0 < H <= 65535 and 0 < D <= 65536, f"{op}: bad size {tuple(x.shape)}")
+    if not (T > 0 and 0 < H <= 65535 and 0 < D <= 65536 and H * D <= 1 << 30):
+        refuse(op, f"bad size {tuple(x.shape)}")
     check_rope_angles(op, positions, inv_freq, T, D)
 
 
 def check_rope_angles(op: str, positions: Tensor, inv_freq: Tensor, tokens: int, D: int) -> None:
-    _check_int32(op, "positions", positions, (tokens,))
-    require(inv_freq.dim() == 1 and inv_freq.dtype in (torch.float64, torch.float32), f"{op}: inv_freq must be float64 or float32 [rotary_dim / 2]")
+    _check_int32(op, "positions", positions, tokens)
+    if inv_freq.dim() != 1 or inv_freq.dtype not in (torch.float64, torch.float32):
+        refuse(op, "inv_freq must be float64 or float32 [rotary_dim / 2]")
     R = 2 * inv_freq.size(0)
-    require(0 < R <= min(D, MAX_ROTARY_DIM), f"{op}: {R} rotary elements of a head of {D} (at most {MAX_ROTARY_DIM})")
+    if not 0 < R <= min(D, MAX_ROTARY_DIM):
+        refuse(op, f"{R} rotary elements of a head of {D} (at most {MAX_ROTARY_DIM})")
 
 
 def check_rope_append(op: str, q: Tensor, k_new: Tensor, v_new: Tensor, positions: Tensor, inv_freq: Tensor, k_cache: Tensor,
                       v_cache: Tensor, slots: Tensor) -> None:
-    require(q.dim() == 3 and k_new.dim() == 3 and k_new.shape == v_new.shape, f"{op}: q must be [tokens, Hq, D], k_new and v_new both [tokens, Hkv, D]")
-    require(k_cache.dim() == 4 and k_cache.shape == v_cache.shape, f"{op}: k_cache and v_cache must both be [P, page, Hkv, D]")
-    require(same_half_dtype((q, k_new, v_new, k_cache, v_cache)), f"{op}: tensors must all be float16 or all bfloat16")
-    require(q.size(2) == 128 and k_new.size(2) == 128 and k_cache.size(3) == 128, f"{op}: head dim must be 128")
-    require(k_cache.size(1) in PAGE_SIZES, f"{op}: page size {k_cache.size(1)} not supported {PAGE_SIZES}")
-    T = q.size(0)
-    require(0 < q.size(1) <= 65535 and 0 < k_new.size(1) <= 65535, f"{op}: bad head counts {q.size(1)} and {k_new.size(1)}")
-    require(T > 0 and k_new.size(0) == T and k_cache.size(0) > 0, f"{op}: empty or unequal tokens ({T} and {k_new.size(0)}) or empty cache")
-    require(k_new.size(1) == k_cache.size(2), f"{op}: k_new and k_cache disagree on the number of kv heads")
-    require(k_cache.is_contiguous() and v_cache.is_contiguous(), f"{op}: k_cache and v_cache are written in place and must be contiguous")
-    require(slots.dtype == torch.int64 and tuple(slots.shape) == (T,), f"{op}: slots must be int64 [tokens], got {slots.dtype} {tuple(slots.shape)}")
+    if q.dim() != 3 or k_new.dim() != 3 or k_new.shape != v_new.shape:
+        refuse(op, "q must be [tokens, Hq, D], k_new and v_new both [tokens, Hkv, D]")
+    if not same_half_dtype((q, k_new, v_new, k_cache, v_cache)):
+        refuse(op, "tensors must all be float16 or all be bfloat16")
+    _check_caches(op, k_cache, v_cache)
+    (T, hq, D), (Tk, hkv, Dk) = q.shape, k_new.shape
+    if D != 128 or Dk != 128:
+        refuse(op, f"head dim must be 128, got {D} and {Dk}")
+    if not (0 < hq <= 65535 and 0 < hkv <= 65535):
+        refuse(op, f"bad head counts {hq} and {hkv}")
+    if T == 0 or Tk != T:
+        refuse(op, f"empty or unequal tokens ({T} and {Tk})")
+    if hkv != k_cache.size(2):
+        refuse(op, "k_new and k_cache disagree on the number of kv heads")
+    if not (k_cache.is_contiguous() and v_cache.is_contiguous()):
+        refuse(op, "k_cache and v_cache are written in place and must be contiguous")
+    if slots.dtype != torch.int64 or slots.shape != (T,):
+        refuse(op, f"slots must be int64 [tokens], got {slots.dtype} {tuple(slots.shape)}")
     check_rope_angles(op, positions, inv_freq, T, 128)

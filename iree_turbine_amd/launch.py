@@ -5,6 +5,7 @@ contract (contract.py) on its tensors before it takes a single device pointer.""
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import math
 
@@ -305,6 +306,16 @@ def paged_prefill_attn_out(q: Tensor, k_cache: Tensor, v_cache: Tensor, block_ta
     return out
 
 
+# ---- the packed serving step ----------------------------------------------------------------------------------------
+# `*_out` checks its tensors and calls `_*`; the custom ops, whose `select` has run the contract and which make their own
+# outputs, call `_*` directly.
+
+
+def _on(dev: torch.device):
+    """The device guard of a call; none when the device is the current one already (the guard costs a short call 1.4 us)."""
+    return contextlib.nullcontext() if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
+
+
 def _row_strides(t: Tensor) -> tuple[int, int] | None:
     """{token, head} element strides of [tokens, heads, 128] rows that the attention kernels can read in place, else None."""
     st, sh, sd = t.stride()
@@ -319,8 +330,39 @@ def _row_strides(t: Tensor) -> tuple[int, int] | None:
     return (st, sh)
 
 
-def _i64s(*values: int):
-    return (ctypes.c_int64 * len(values))(*values)
+_Strides = ctypes.c_int64 * 2
+
+
+def _default_scale(scale: float | None, D: int) -> float:
+    return 1.0 / math.sqrt(D) if scale is None or scale <= 0 else scale
+
+
+def _readable_rows(op: str, t: Tensor) -> tuple[Tensor, tuple[int, int]]:
+    st = _row_strides(t)
+    if st is None:
+        t = t.clone(memory_format=torch.contiguous_format)
+        st = _row_strides(t)
+        contract.require(st is not None, f"{op}: rows of {tuple(t.shape)} are too far apart")
+    return t, st
+
+
+def _flash_attn_varlen_fwd(dev, q, k, v, cu_q, cu_k, o, is_causal, scale, zero_rest):
+    op = "flash_attn_varlen_fwd"
+    q, qs = _readable_rows(op, q)
+    k, ks = _readable_rows(op, k)
+    v, vs = _readable_rows(op, v)
+    os_ = _row_strides(o)
+    if os_ is None or (o.size(1) > 1 and os_[1] == 0):
+        raise ValueError(f"{op}: output rows must be contiguous, 16-byte aligned and not overlapping")
+    cu_q, cu_k = cu_q.contiguous(), cu_k.contiguous()
+    with _on(dev):
+        rc = _lib.load().mi355_flash_attn_varlen_fwd(
+            q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), cu_q.data_ptr(), cu_k.data_ptr(), cu_q.size(0) - 1, q.size(0),
+            k.size(0), q.size(1), k.size(1), 128, _Strides(*qs), _Strides(*ks), _Strides(*vs), _Strides(*os_),
+            _default_scale(scale, 128), is_causal, zero_rest, _lib.dtype_code(q.dtype), _lib.raw_stream(dev))
+    if rc:
+        _lib.check(rc, f"{op} {q.dtype} q={tuple(q.shape)} k={tuple(k.shape)} seqs={cu_q.shape[0] - 1} causal={is_causal}")
+    return o
 
 
 def flash_attn_varlen_fwd_out(q: Tensor, k: Tensor, v: Tensor, cu_seqlens_q: Tensor, cu_seqlens_k: Tensor, o: Tensor, is_causal: bool,
@@ -329,34 +371,32 @@ def flash_attn_varlen_fwd_out(q: Tensor, k: Tensor, v: Tensor, cu_seqlens_q: Ten
     are left as they are unless `zero_rest`."""
     contract.check_varlen_attention("flash_attn_varlen_fwd", q, k, v, cu_seqlens_q, cu_seqlens_k)
     dev = _dev(q, k, v, cu_seqlens_q, cu_seqlens_k, o)
-    dt = _half_dtype("flash_attn_varlen_fwd", q, k, v, o)
+    _half_dtype("flash_attn_varlen_fwd", q, k, v, o)
     if o.shape != q.shape:
         raise ValueError("flash_attn_varlen_fwd: o must have q's shape")
-    ins = []
-    for t in (q, k, v):
-        st = _row_strides(t)
-        if st is None:
-            t = t.contiguous()
-            st = _row_strides(t)
-            if st is None:  # rows of a contiguous tensor are 2^24 elements apart, or its storage starts off a 16-byte border
-                t = t.clone(memory_format=torch.contiguous_format)
-                st = _row_strides(t)
-                contract.require(st is not None, f"flash_attn_varlen_fwd: rows of {tuple(t.shape)} are too far apart")
-        ins.append((t, st))
-    o_st = _row_strides(o)
-    if o_st is None or (o.size(1) > 1 and o_st[1] == 0):
-        raise ValueError("flash_attn_varlen_fwd: output rows must be contiguous, 16-byte aligned and not overlapping")
-    if scale is None or scale <= 0:
-        scale = 1.0 / math.sqrt(q.shape[2])
-    cu_seqlens_q, cu_seqlens_k = cu_seqlens_q.contiguous(), cu_seqlens_k.contiguous()
-    with torch.cuda.device(dev):
-        rc = _lib.load().mi355_flash_attn_varlen_fwd(
-            ins[0][0].data_ptr(), ins[1][0].data_ptr(), ins[2][0].data_ptr(), o.data_ptr(), cu_seqlens_q.data_ptr(),
-            cu_seqlens_k.data_ptr(), cu_seqlens_q.shape[0] - 1, q.shape[0], k.shape[0], q.shape[1], k.shape[1], 128, _i64s(*ins[0][1]),
-            _i64s(*ins[1][1]), _i64s(*ins[2][1]), _i64s(*o_st), scale, int(bool(is_causal)), int(bool(zero_rest)), _lib.dtype_code(dt),
-            _lib.current_stream_ptr(dev))
-    _lib.check(rc, f"flash_attn_varlen_fwd {dt} q={tuple(q.shape)} k={tuple(k.shape)} seqs={cu_seqlens_q.shape[0] - 1} causal={is_causal}")
-    return o
+    return _flash_attn_varlen_fwd(dev, q, k, v, cu_seqlens_q, cu_seqlens_k, o, bool(is_causal), scale, bool(zero_rest))
+
+
+def _paged_tree_attn(dev, q, k_cache, v_cache, block_table, seq_lens, parents, out, scale, splits, part_acc, part_ml):
+    q, k_cache, v_cache = q.contiguous(), k_cache.contiguous(), v_cache.contiguous()
+    block_table, seq_lens, parents = block_table.contiguous(), seq_lens.contiguous(), parents.contiguous()
+    S, N, Hq, D = q.shape
+    P, page, Hkv, _ = k_cache.shape
+    pa = pm = None
+    if splits > 1:
+        if part_acc is None:
+            part_acc = torch.empty((S, N, Hq, splits, D), dtype=torch.float32, device=dev)
+        if part_ml is None:
+            part_ml = torch.empty((S, N, Hq, splits, 2), dtype=torch.float32, device=dev)
+        pa, pm = part_acc.data_ptr(), part_ml.data_ptr()
+    with _on(dev):
+        rc = _lib.load().mi355_paged_tree_attn(q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), block_table.data_ptr(),
+                                               seq_lens.data_ptr(), parents.data_ptr(), out.data_ptr(), pa, pm, S, N, Hq, Hkv, D, page,
+                                               block_table.size(1), P, splits, _default_scale(scale, D), _lib.dtype_code(q.dtype),
+                                               _lib.raw_stream(dev))
+    if rc:
+        _lib.check(rc, f"paged_tree_attn {q.dtype} seqs={S} nodes={N} hq={Hq} hkv={Hkv} pages={P} splits={splits}")
+    return out
 
 
 def paged_tree_attn_out(q: Tensor, k_cache: Tensor, v_cache: Tensor, block_table: Tensor, seq_lens: Tensor, parents: Tensor, out: Tensor,
@@ -365,60 +405,61 @@ def paged_tree_attn_out(q: Tensor, k_cache: Tensor, v_cache: Tensor, block_table
     part_acc [S, N, Hq, splits, 128] and part_ml [S, N, Hq, splits, 2], allocated here if not given."""
     contract.check_tree_attention("paged_tree_attn", q, k_cache, v_cache, block_table, seq_lens, parents)
     contract.require(1 <= num_kv_splits <= 1024, f"paged_tree_attn: num_kv_splits must be in [1, 1024], got {num_kv_splits}")
-    dev = _dev(q, k_cache, v_cache, block_table, seq_lens, parents, out)
-    dt = _half_dtype("paged_tree_attn", q, k_cache, v_cache, out)
+    dev = _dev(q, k_cache, v_cache, block_table, seq_lens, parents, out, *(t for t in (part_acc, part_ml) if t is not None))
+    _half_dtype("paged_tree_attn", q, k_cache, v_cache, out)
     _contig_out(out, "paged_tree_attn")
     if out.shape != q.shape:
         raise ValueError("paged_tree_attn: out must have q's shape")
-    q, k_cache, v_cache = q.contiguous(), k_cache.contiguous(), v_cache.contiguous()
-    block_table, seq_lens, parents = block_table.contiguous(), seq_lens.contiguous(), parents.contiguous()
-    S, N, Hq, D = q.shape
-    P, page, Hkv, _ = k_cache.shape
-    if scale is None or scale <= 0:
-        scale = 1.0 / math.sqrt(D)
-    pa = pm = None
     if num_kv_splits > 1:
-        if part_acc is None:
-            part_acc = torch.empty((S, N, Hq, num_kv_splits, D), dtype=torch.float32, device=dev)
-        if part_ml is None:
-            part_ml = torch.empty((S, N, Hq, num_kv_splits, 2), dtype=torch.float32, device=dev)
-        _dev(q, part_acc, part_ml)
-        for t, last in ((part_acc, D), (part_ml, 2)):
-            if t.dtype != torch.float32 or tuple(t.shape) != (S, N, Hq, num_kv_splits, last):
-                raise ValueError(f"paged_tree_attn: scratch must be fp32 {(S, N, Hq, num_kv_splits, last)}, got {t.dtype} {tuple(t.shape)}")
-            _contig_out(t, "paged_tree_attn")
-        pa, pm = part_acc.data_ptr(), part_ml.data_ptr()
-    with torch.cuda.device(dev):
-        rc = _lib.load().mi355_paged_tree_attn(q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), block_table.data_ptr(),
-                                               seq_lens.data_ptr(), parents.data_ptr(), out.data_ptr(), pa, pm, S, N, Hq, Hkv, D, page,
-                                               block_table.shape[1], P, num_kv_splits, scale, _lib.dtype_code(dt),
-                                               _lib.current_stream_ptr(dev))
-    _lib.check(rc, f"paged_tree_attn {dt} seqs={S} nodes={N} hq={Hq} hkv={Hkv} pages={P} splits={num_kv_splits}")
-    return out
+        for t, last in ((part_acc, 128), (part_ml, 2)):
+            if t is not None:
+                if t.dtype != torch.float32 or tuple(t.shape) != (*q.shape[:3], num_kv_splits, last):
+                    raise ValueError(f"paged_tree_attn: scratch must be fp32 {(*q.shape[:3], num_kv_splits, last)}, got {t.dtype} {tuple(t.shape)}")
+                _contig_out(t, "paged_tree_attn")
+    return _paged_tree_attn(dev, q, k_cache, v_cache, block_table, seq_lens, parents, out, scale, num_kv_splits, part_acc, part_ml)
+
+
+def _verify_draft(dev, target_probs, draft_probs, tokens, parents, uniforms, path, num_accepted, next_token):
+    S, N, V = target_probs.shape
+    target_probs, tokens, parents, uniforms = target_probs.contiguous(), tokens.contiguous(), parents.contiguous(), uniforms.contiguous()
+    draft = None
+    if draft_probs is not None:
+        draft_probs = draft_probs.contiguous()
+        draft = draft_probs.data_ptr()
+    lib = _lib.load()
+    ws_bytes = lib.mi355_verify_draft_workspace_bytes(S, N, V)
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
+    with _on(dev):
+        rc = lib.mi355_verify_draft(target_probs.data_ptr(), draft, tokens.data_ptr(), parents.data_ptr(), uniforms.data_ptr(),
+                                    path.data_ptr(), num_accepted.data_ptr(), next_token.data_ptr(), S, N, V, ws.data_ptr(), ws_bytes,
+                                    _lib.raw_stream(dev))
+    if rc:
+        _lib.check(rc, f"verify_draft seqs={S} nodes={N} vocab={V}")
+    return path, num_accepted, next_token
 
 
 def verify_draft_out(target_probs: Tensor, draft_probs: Tensor | None, tokens: Tensor, parents: Tensor, uniforms: Tensor, path: Tensor,
                      num_accepted: Tensor, next_token: Tensor) -> tuple[Tensor, Tensor, Tensor]:
     """path int32 [S, N], num_accepted and next_token int32 [S] (see mi355_verify_draft)."""
     contract.check_verify_draft("verify_draft", target_probs, draft_probs, tokens, parents, uniforms)
-    ins = [target_probs, tokens, parents, uniforms] + ([draft_probs] if draft_probs is not None else [])
-    dev = _dev(*ins, path, num_accepted, next_token)
+    dev = _dev(target_probs, tokens, parents, uniforms, path, num_accepted, next_token, *([draft_probs] if draft_probs is not None else []))
     S, N, V = target_probs.shape
     for name, t, shape in (("path", path, (S, N)), ("num_accepted", num_accepted, (S,)), ("next_token", next_token, (S,))):
         if t.dtype != torch.int32 or tuple(t.shape) != shape:
             raise ValueError(f"verify_draft: {name} must be int32 {shape}, got {t.dtype} {tuple(t.shape)}")
         _contig_out(t, "verify_draft")
-    target_probs, tokens, parents, uniforms = (t.contiguous() for t in ins[:4])
-    draft_probs = draft_probs.contiguous() if draft_probs is not None else None
-    lib = _lib.load()
-    ws_bytes = lib.mi355_verify_draft_workspace_bytes(S, N, V)
-    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
-    with torch.cuda.device(dev):
-        rc = lib.mi355_verify_draft(target_probs.data_ptr(), draft_probs.data_ptr() if draft_probs is not None else None, tokens.data_ptr(),
-                                    parents.data_ptr(), uniforms.data_ptr(), path.data_ptr(), num_accepted.data_ptr(),
-                                    next_token.data_ptr(), S, N, V, ws.data_ptr(), ws_bytes, _lib.current_stream_ptr(dev))
-    _lib.check(rc, f"verify_draft seqs={S} nodes={N} vocab={V}")
-    return path, num_accepted, next_token
+    return _verify_draft(dev, target_probs, draft_probs, tokens, parents, uniforms, path, num_accepted, next_token)
+
+
+def _paged_batch_layout(dev, block_table, context_lens, new_lens, free_pages, page_size, num_tokens, outs):
+    S, W = block_table.shape
+    context_lens, new_lens, free_pages = context_lens.contiguous(), new_lens.contiguous(), free_pages.contiguous()
+    with _on(dev):
+        rc = _lib.load().mi355_paged_batch_layout(block_table.data_ptr(), context_lens.data_ptr(), new_lens.data_ptr(),
+                                                  free_pages.data_ptr() or None, free_pages.size(0), S, W, page_size, num_tokens,
+                                                  *[t.data_ptr() for t in outs], _lib.raw_stream(dev))
+    if rc:
+        _lib.check(rc, f"paged_batch_layout seqs={S} pages={W} tokens={num_tokens}")
 
 
 def paged_batch_layout_out(block_table: Tensor, context_lens: Tensor, new_lens: Tensor, free_pages: Tensor, page_size: int, seq_lens: Tensor,
@@ -426,20 +467,30 @@ def paged_batch_layout_out(block_table: Tensor, context_lens: Tensor, new_lens: 
     """Fills the per-sequence and per-token arrays of a step and enters its new pages in block_table (see mi355_paged_batch_layout)."""
     T = positions.shape[0] if positions.dim() == 1 else 0
     contract.check_batch_layout("paged_batch_layout", block_table, context_lens, new_lens, free_pages, page_size, T)
-    dev = _dev(block_table, context_lens, new_lens, free_pages, seq_lens, cu_new, positions, seq_ids, slots, pages_needed)
-    S, W = block_table.shape
-    for name, t, n, dt in (("seq_lens", seq_lens, S, torch.int32), ("cu_new", cu_new, S + 1, torch.int32), ("positions", positions, T, torch.int32),
-                           ("seq_ids", seq_ids, T, torch.int32), ("slots", slots, T, torch.int64), ("pages_needed", pages_needed, 1, torch.int32)):
+    outs = (seq_lens, cu_new, positions, seq_ids, slots, pages_needed)
+    dev = _dev(block_table, context_lens, new_lens, free_pages, *outs)
+    S = block_table.shape[0]
+    for name, t, n, dt in zip(("seq_lens", "cu_new", "positions", "seq_ids", "slots", "pages_needed"), outs, (S, S + 1, T, T, T, 1),
+                              (torch.int32,) * 4 + (torch.int64, torch.int32)):
         if t.dtype != dt or tuple(t.shape) != (n,):
             raise ValueError(f"paged_batch_layout: {name} must be {dt} ({n},), got {t.dtype} {tuple(t.shape)}")
         _contig_out(t, "paged_batch_layout")
-    context_lens, new_lens, free_pages = context_lens.contiguous(), new_lens.contiguous(), free_pages.contiguous()
-    with torch.cuda.device(dev):
-        rc = _lib.load().mi355_paged_batch_layout(block_table.data_ptr(), context_lens.data_ptr(), new_lens.data_ptr(), free_pages.data_ptr() or None,
-                                                  free_pages.shape[0], S, W, page_size, T, seq_lens.data_ptr(), cu_new.data_ptr(),
-                                                  positions.data_ptr(), seq_ids.data_ptr(), slots.data_ptr(), pages_needed.data_ptr(),
-                                                  _lib.current_stream_ptr(dev))
-    _lib.check(rc, f"paged_batch_layout seqs={S} pages={W} tokens={T}")
+    _paged_batch_layout(dev, block_table, context_lens, new_lens, free_pages, page_size, T, outs)
+
+
+def _rope(dev, x, positions, inv_freq, out, interleaved, inverse, scale):
+    if x.stride(2) != 1 and x.size(2) > 1:
+        x = x.contiguous()
+    positions, inv_freq = positions.contiguous(), inv_freq.contiguous()
+    T, H, D = x.shape
+    half = inv_freq.size(0)
+    with _on(dev):
+        rc = _lib.load().mi355_rope(x.data_ptr(), out.data_ptr(), positions.data_ptr(), inv_freq.data_ptr(), inv_freq.dtype == torch.float64,
+                                    T, H, D, 2 * half, _Strides(x.stride(0), x.stride(1)), _Strides(out.stride(0), out.stride(1)),
+                                    interleaved, inverse, scale, _lib.dtype_code(x.dtype), _lib.raw_stream(dev))
+    if rc:
+        _lib.check(rc, f"rope {x.dtype} x={tuple(x.shape)} rotary={2 * half}")
+    return out
 
 
 def rope_out(x: Tensor, positions: Tensor, inv_freq: Tensor, out: Tensor, interleaved: bool, inverse: bool, scale: float) -> Tensor:
@@ -448,18 +499,26 @@ def rope_out(x: Tensor, positions: Tensor, inv_freq: Tensor, out: Tensor, interl
     dev = _dev(x, positions, inv_freq, out)
     if out.shape != x.shape or out.dtype != x.dtype:
         raise ValueError("rope: out must have x's shape and dtype")
-    if x.stride(2) != 1 and x.size(2) > 1:
-        x = x.contiguous()
     if (out.stride(2) != 1 and out.size(2) > 1) or any(out.stride(i) == 0 and out.size(i) > 1 for i in (0, 1)):
         raise ValueError("rope: output rows must be contiguous and not overlapping")
-    positions, inv_freq = positions.contiguous(), inv_freq.contiguous()
-    T, H, D = x.shape
-    with torch.cuda.device(dev):
-        rc = _lib.load().mi355_rope(x.data_ptr(), out.data_ptr(), positions.data_ptr(), inv_freq.data_ptr(), int(inv_freq.dtype == torch.float64),
-                                    T, H, D, 2 * inv_freq.shape[0], _i64s(x.stride(0), x.stride(1)), _i64s(out.stride(0), out.stride(1)),
-                                    int(bool(interleaved)), int(bool(inverse)), scale, _lib.dtype_code(x.dtype), _lib.current_stream_ptr(dev))
-    _lib.check(rc, f"rope {x.dtype} x={tuple(x.shape)} rotary={2 * inv_freq.shape[0]}")
-    return out
+    return _rope(dev, x, positions, inv_freq, out, bool(interleaved), bool(inverse), scale)
+
+
+def _rope_kv_append(dev, q, k_new, v_new, positions, inv_freq, k_cache, v_cache, slots, q_out, interleaved, scale):
+    q, k_new, v_new = (t if t.stride(2) == 1 else t.contiguous() for t in (q, k_new, v_new))
+    positions, inv_freq, slots = positions.contiguous(), inv_freq.contiguous(), slots.contiguous()
+    T, Hq, D = q.shape
+    P, page, Hkv, _ = k_cache.shape
+    half = inv_freq.size(0)
+    with _on(dev):
+        rc = _lib.load().mi355_rope_kv_append(q.data_ptr(), k_new.data_ptr(), v_new.data_ptr(), q_out.data_ptr(), k_cache.data_ptr(),
+                                              v_cache.data_ptr(), positions.data_ptr(), inv_freq.data_ptr(), inv_freq.dtype == torch.float64,
+                                              slots.data_ptr(), T, Hq, Hkv, D, 2 * half, P * page, _Strides(q.stride(0), q.stride(1)),
+                                              _Strides(k_new.stride(0), k_new.stride(1)), _Strides(v_new.stride(0), v_new.stride(1)),
+                                              interleaved, scale, _lib.dtype_code(q.dtype), _lib.raw_stream(dev))
+    if rc:
+        _lib.check(rc, f"rope_kv_append {q.dtype} tokens={T} hq={Hq} hkv={Hkv} pages={P}")
+    return q_out
 
 
 def rope_kv_append_out(q: Tensor, k_new: Tensor, v_new: Tensor, positions: Tensor, inv_freq: Tensor, k_cache: Tensor, v_cache: Tensor,
@@ -467,23 +526,11 @@ def rope_kv_append_out(q: Tensor, k_new: Tensor, v_new: Tensor, positions: Tenso
     """Rotates q into q_out and k_new, with v_new as it is, into the cache rows `slots` names (see mi355_rope_kv_append)."""
     contract.check_rope_append("rope_kv_append", q, k_new, v_new, positions, inv_freq, k_cache, v_cache, slots)
     dev = _dev(q, k_new, v_new, positions, inv_freq, k_cache, v_cache, slots, q_out)
-    dt = _half_dtype("rope_kv_append", q, k_new, v_new, k_cache, v_cache, q_out)
+    _half_dtype("rope_kv_append", q, k_new, v_new, k_cache, v_cache, q_out)
     _contig_out(q_out, "rope_kv_append")
     if q_out.shape != q.shape:
         raise ValueError("rope_kv_append: q_out must have q's shape")
-    q, k_new, v_new = (t if t.stride(2) == 1 else t.contiguous() for t in (q, k_new, v_new))
-    positions, inv_freq, slots = positions.contiguous(), inv_freq.contiguous(), slots.contiguous()
-    T, Hq, D = q.shape
-    P, page, Hkv, _ = k_cache.shape
-    with torch.cuda.device(dev):
-        rc = _lib.load().mi355_rope_kv_append(q.data_ptr(), k_new.data_ptr(), v_new.data_ptr(), q_out.data_ptr(), k_cache.data_ptr(),
-                                              v_cache.data_ptr(), positions.data_ptr(), inv_freq.data_ptr(),
-                                              int(inv_freq.dtype == torch.float64), slots.data_ptr(), T, Hq, Hkv, D, 2 * inv_freq.shape[0],
-                                              P * page, _i64s(q.stride(0), q.stride(1)), _i64s(k_new.stride(0), k_new.stride(1)),
-                                              _i64s(v_new.stride(0), v_new.stride(1)), int(bool(interleaved)), scale, _lib.dtype_code(dt),
-                                              _lib.current_stream_ptr(dev))
-    _lib.check(rc, f"rope_kv_append {dt} tokens={T} hq={Hq} hkv={Hkv} pages={P}")
-    return q_out
+    return _rope_kv_append(dev, q, k_new, v_new, positions, inv_freq, k_cache, v_cache, slots, q_out, bool(interleaved), scale)
 
 
 def _check_mx_out(op: str, c: Tensor) -> None:

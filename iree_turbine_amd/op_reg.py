@@ -76,6 +76,40 @@ class TensorArg(ArgDescriptor):
         return f"tensor[{self.t.dim()}:{self.t.dtype}]<[{dims}]>"
 
 
+class ResultArg(ArgDescriptor):
+    """A result described by size and dtype; its meta tensor is made when somebody asks for it (the Meta kernel does, a
+    launch does not: creating six of them cost it 7 us)."""
+
+    __slots__ = ["size", "dtype", "spec_dims", "_t"]
+
+    def __init__(self, size: Sequence[int], dtype: torch.dtype):
+        super().__init__(None)
+        self.size, self.dtype = list(size), dtype
+        self.spec_dims: list[Optional[int]] = [None] * len(self.size)
+        self._t: Optional[Tensor] = None
+
+    @property
+    def t(self) -> Tensor:
+        if self._t is None:
+            self._t = torch.empty(self.size, dtype=self.dtype, device="meta")
+        return self._t
+
+    def specialize_all_dims(self):
+        self.spec_dims = list(self.size)
+
+    def specialize_dims(self, *indices: int):
+        for i in indices:
+            self.spec_dims[i] = self.size[i]
+
+    def generate_meta(self) -> Tensor:
+        return self.t
+
+    @property
+    def spec_key(self) -> str:
+        dims = ", ".join("?" if d is None else str(d) for d in self.spec_dims)
+        return f"tensor[{len(self.size)}:{self.dtype}]<[{dims}]>"
+
+
 class KernelSelection:
     """What `CustomOp.select` fills in for one call: checked arguments and result descriptors."""
 
@@ -83,7 +117,7 @@ class KernelSelection:
         self.op = op
         self.args = list(args)
         self.arg_descs: list[Optional[ArgDescriptor]] = [None] * len(args)
-        self.result_descs: list[TensorArg] = []
+        self.result_descs: list[Union[TensorArg, ResultArg]] = []
         self.variant = "default"
 
     def arg_tensor(self, arg: int) -> TensorArg:
@@ -128,8 +162,10 @@ class KernelSelection:
         self.result_descs.append(desc)
         return desc
 
-    def return_new_tensor(self, size: Sequence[int], dtype: torch.dtype) -> TensorArg:
-        return self.return_tensor(torch.empty(list(size), dtype=dtype, device="meta"))
+    def return_new_tensor(self, size: Sequence[int], dtype: torch.dtype) -> ResultArg:
+        desc = ResultArg(size, dtype)
+        self.result_descs.append(desc)
+        return desc
 
     def generate_meta_returns(self):
         results = [d.generate_meta() for d in self.result_descs]

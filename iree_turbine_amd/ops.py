@@ -17,7 +17,7 @@ from . import launch
 from .contract import PAGE_SIZES, check_mx_operand as _check_mx_operand, check_paged_args as _check_paged_args  # noqa: F401
 from . import contract
 from .contract import require as _require
-from .op_reg import CustomOp, KernelSelection, TensorArg
+from .op_reg import CustomOp, KernelSelection
 
 __all__ = [
     "gemm_nt",
@@ -478,10 +478,11 @@ class paged_batch_layout(CustomOp):
         sel.return_new_tensor([1], torch.int32)
 
     def eager_execute(self, block_table, context_lens, new_lens, free_pages, page_size, num_tokens):
-        S = context_lens.shape[0]
-        new = lambda n, dt=torch.int32: torch.empty(n, dtype=dt, device=block_table.device)
-        outs = (new(S), new(S + 1), new(num_tokens), new(num_tokens), new(num_tokens, torch.int64), new(1))
-        launch.paged_batch_layout_out(block_table, context_lens, new_lens, free_pages, page_size, *outs)
+        dev = launch._dev(block_table, context_lens, new_lens, free_pages)
+        S, T, i32 = context_lens.size(0), num_tokens, torch.int32
+        outs = (torch.empty(S, dtype=i32, device=dev), torch.empty(S + 1, dtype=i32, device=dev), torch.empty(T, dtype=i32, device=dev),
+                torch.empty(T, dtype=i32, device=dev), torch.empty(T, dtype=torch.int64, device=dev), torch.empty(1, dtype=i32, device=dev))
+        launch._paged_batch_layout(dev, block_table, context_lens, new_lens, free_pages, page_size, T, outs)
         return outs
 
 
@@ -530,8 +531,8 @@ class rope(CustomOp):
         sel.return_new_tensor(list(x.t.shape), x.t.dtype)
 
     def eager_execute(self, x, positions, inv_freq, interleaved, inverse, scale):
-        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        return launch.rope_out(x, positions, inv_freq, out, interleaved, inverse, scale)
+        dev = launch._dev(x, positions, inv_freq)
+        return launch._rope(dev, x, positions, inv_freq, torch.empty(x.shape, dtype=x.dtype, device=dev), interleaved, inverse, scale)
 
 
 def _rope_setup_context(ctx, inputs, output):
@@ -566,8 +567,9 @@ class rope_kv_append(CustomOp):
         sel.return_new_tensor(list(q.t.shape), q.t.dtype)
 
     def eager_execute(self, q, k_new, v_new, positions, inv_freq, k_cache, v_cache, slots, interleaved, scale):
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        return launch.rope_kv_append_out(q, k_new, v_new, positions, inv_freq, k_cache, v_cache, slots, out, interleaved, scale)
+        dev = launch._dev(q, k_new, v_new, positions, inv_freq, k_cache, v_cache, slots)
+        out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+        return launch._rope_kv_append(dev, q, k_new, v_new, positions, inv_freq, k_cache, v_cache, slots, out, interleaved, scale)
 
 
 @CustomOp.register
@@ -590,8 +592,9 @@ class flash_attn_varlen_fwd(CustomOp):
         sel.return_new_tensor(list(q.t.shape), q.t.dtype)
 
     def eager_execute(self, q, k, v, cu_seqlens_q, cu_seqlens_k, is_causal, scale):
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        return launch.flash_attn_varlen_fwd_out(q, k, v, cu_seqlens_q, cu_seqlens_k, out, is_causal, scale, zero_rest=True)
+        dev = launch._dev(q, k, v, cu_seqlens_q, cu_seqlens_k)
+        out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+        return launch._flash_attn_varlen_fwd(dev, q, k, v, cu_seqlens_q, cu_seqlens_k, out, is_causal, scale, True)
 
 
 @CustomOp.register
@@ -614,9 +617,11 @@ class paged_tree_attn(CustomOp):
 
     def eager_execute(self, q, k_cache, v_cache, block_table, seq_lens, parents, scale, num_kv_splits):
         if num_kv_splits <= 0:
-            num_kv_splits = default_num_kv_splits(block_table.shape[1] * k_cache.shape[1], q.shape[0], k_cache.shape[2])
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        return launch.paged_tree_attn_out(q, k_cache, v_cache, block_table, seq_lens, parents, out, scale, num_kv_splits)
+            num_kv_splits = default_num_kv_splits(block_table.size(1) * k_cache.size(1), q.size(0), k_cache.size(2))
+        _require(num_kv_splits <= 1024, "paged_tree_attn: num_kv_splits must be at most 1024")
+        dev = launch._dev(q, k_cache, v_cache, block_table, seq_lens, parents)
+        out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+        return launch._paged_tree_attn(dev, q, k_cache, v_cache, block_table, seq_lens, parents, out, scale, num_kv_splits, None, None)
 
 
 @CustomOp.register
@@ -635,13 +640,14 @@ class verify_draft(CustomOp):
     def select(self, sel: KernelSelection):
         tp, tok, par, u = (sel.arg_tensor(i) for i in (0, 2, 3, 4))
         dp = sel.arg_optional_tensor(1)
-        contract.check_verify_draft("verify_draft", tp.t, dp.t if isinstance(dp, TensorArg) else None, tok.t, par.t, u.t)
+        contract.check_verify_draft("verify_draft", tp.t, dp.v if dp is not None else None, tok.t, par.t, u.t)
         S, N, _ = tp.t.shape
         sel.return_new_tensor([S, N], torch.int32)
         sel.return_new_tensor([S], torch.int32)
         sel.return_new_tensor([S], torch.int32)
 
     def eager_execute(self, target_probs, draft_probs, tokens, parents, uniforms):
-        S, N, _ = target_probs.shape
-        new = lambda *n: torch.empty(n, dtype=torch.int32, device=target_probs.device)
-        return launch.verify_draft_out(target_probs, draft_probs, tokens, parents, uniforms, new(S, N), new(S), new(S))
+        dev = launch._dev(target_probs, tokens, parents, uniforms, *([draft_probs] if draft_probs is not None else []))
+        S, N, i32 = target_probs.size(0), target_probs.size(1), torch.int32
+        path, count, last = (torch.empty((S, N), dtype=i32, device=dev), torch.empty(S, dtype=i32, device=dev), torch.empty(S, dtype=i32, device=dev))
+        return launch._verify_draft(dev, target_probs, draft_probs, tokens, parents, uniforms, path, count, last)

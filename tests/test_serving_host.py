@@ -77,7 +77,7 @@ def test_meta_kernels_give_the_results_shapes():
     (dict(q=m(9, 4, 64), k=m(11, 2, 64), v=m(11, 2, 64)), "head dim"),
     (dict(k=m(11, 3, 128), v=m(11, 3, 128)), "query heads"),
     (dict(v=m(10, 2, 128)), "shapes differ"),
-    (dict(q=m(9, 4, 128, dt=torch.bfloat16)), "all be float16 or all bfloat16"),
+    (dict(q=m(9, 4, 128, dt=torch.bfloat16)), "all be float16 or all be bfloat16"),
     (dict(cq=m(4, dt=I64)), "cu_seqlens_q"),
     (dict(ck=m(5, dt=I32)), "cu_seqlens_k"),
     (dict(cq=m(1, dt=I32), ck=m(1, dt=I32)), "cu_seqlens_q"),
@@ -97,7 +97,7 @@ def test_varlen_refusals(change, text):
     (dict(par=m(2, 5, dt=I64)), "parents"),
     (dict(sl=m(3, dt=I32)), "rows must equal"),
     (dict(q=m(2, 5, 258, 128)), "up to 128"),
-    (dict(vc=m(6, 16, 2, 128, dt=torch.bfloat16)), "all be float16 or all bfloat16"),
+    (dict(vc=m(6, 16, 2, 128, dt=torch.bfloat16)), "all be float16 or all be bfloat16"),
 ])
 def test_tree_refusals(change, text):
     with pytest.raises(ValueError, match=text):
@@ -150,7 +150,7 @@ def test_rope_refusals(change, text):
     (dict(slots=m(5, dt=I32)), "slots"),
     (dict(kc=m(6, 16, 4, 128)[:, :, ::2], vc=m(6, 16, 4, 128)[:, :, ::2]), "contiguous"),
     (dict(f=m(65, dt=F64)), "rotary elements"),
-    (dict(v=m(5, 2, 128, dt=torch.bfloat16)), "all be float16 or all bfloat16"),
+    (dict(v=m(5, 2, 128, dt=torch.bfloat16)), "all be float16 or all be bfloat16"),
 ])
 def test_append_refusals(change, text):
     with pytest.raises(ValueError, match=text):
