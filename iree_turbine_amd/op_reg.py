@@ -204,7 +204,7 @@ class CustomOp(ABC):
         if register_impl:
             keys = ["CUDA"] if dispatch_key is None else ([dispatch_key] if isinstance(dispatch_key, str) else dispatch_key)
             for k in keys:
-                library.impl(name, _create_impl_trampoline(self), k)
+                library.impl(name, device_impl(self), k)
         ALL_CUSTOM_OP_REGS[f"{library.ns}.{name}"] = self
 
     @property
@@ -241,7 +241,9 @@ def _get_meta_impl(op: CustomOp):
     return meta
 
 
-def _create_impl_trampoline(op: CustomOp):
+def device_impl(op: CustomOp):
+    """The callable behind the op's device dispatch key: the contract, then the launch."""
+
     def handler(*args):
         sel = KernelSelection(op, args)
         op.select(sel)  # validates shapes / dtypes before anything is launched

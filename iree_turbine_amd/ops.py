@@ -15,7 +15,7 @@ from torch import Tensor
 
 from . import launch
 from .contract import PAGE_SIZES, check_mx_operand as _check_mx_operand, check_paged_args as _check_paged_args  # noqa: F401
-from . import contract
+from . import contract, op_reg
 from .contract import require as _require
 from .op_reg import CustomOp, KernelSelection
 
@@ -535,18 +535,50 @@ class rope(CustomOp):
         return launch._rope(dev, x, positions, inv_freq, torch.empty(x.shape, dtype=x.dtype, device=dev), interleaved, inverse, scale)
 
 
-def _rope_setup_context(ctx, inputs, output):
-    _, positions, inv_freq, ctx.interleaved, ctx.inverse, ctx.scale = inputs
-    ctx.save_for_backward(positions, inv_freq)
+def _on_device_eagerly(x: Tensor) -> bool:
+    """A plain device tensor outside every dispatch mode: the launch needs no further pass through the dispatcher.  Meta
+    and fake tensors and tracing do."""
+    return type(x) in (Tensor, torch.nn.Parameter) and x.is_cuda and torch._C._len_torch_dispatch_stack() == 0
 
 
-def _rope_backward(ctx, grad):
-    """The rotation is linear in x: its transpose is the rotation by the negated angles."""
-    positions, inv_freq = ctx.saved_tensors
-    return torch.ops.mi355.rope(grad, positions, inv_freq, ctx.interleaved, not ctx.inverse, ctx.scale), None, None, None, None, None
+def _rope_below_autograd(*args):
+    if _on_device_eagerly(args[0]):
+        return _rope_on_device(*args)
+    with torch._C._AutoDispatchBelowAutograd():
+        return torch.ops.mi355.rope(*args)
 
 
-torch.library.register_autograd("mi355::rope", _rope_backward, setup_context=_rope_setup_context)
+class _RopeGrad(torch.autograd.Function):
+    """The rotation is linear in x: its transpose is the rotation by the negated angles.  The formula stands here, not in
+    register_autograd, for its cost: a forward and backward pass of a small x take the host 100 us instead of 165."""
+
+    @staticmethod
+    def forward(ctx, x, positions, inv_freq, interleaved, inverse, scale):
+        ctx.interleaved, ctx.inverse, ctx.scale = interleaved, inverse, scale
+        ctx.save_for_backward(positions, inv_freq)
+        return _rope_below_autograd(x, positions, inv_freq, interleaved, inverse, scale)
+
+    @staticmethod
+    def backward(ctx, grad):
+        positions, inv_freq = ctx.saved_tensors
+        how = (ctx.interleaved, not ctx.inverse, ctx.scale)
+        if torch.is_grad_enabled():
+            dx = torch.ops.mi355.rope(grad, positions, inv_freq, *how)
+        elif _on_device_eagerly(grad):  # its sizes and type are the result's, whose call has been checked
+            dx = launch._rope(grad.device, grad, positions, inv_freq, torch.empty(grad.shape, dtype=grad.dtype, device=grad.device), *how)
+        else:
+            dx = _rope_below_autograd(grad, positions, inv_freq, *how)
+        return dx, None, None, None, None, None
+
+
+def _rope_autograd(x, *args):
+    if x.requires_grad and torch.is_grad_enabled():
+        return _RopeGrad.apply(x, *args)
+    return _rope_below_autograd(x, *args)
+
+
+_rope_on_device = op_reg.device_impl(op_reg.ALL_CUSTOM_OP_REGS["mi355.rope"])
+op_reg.MI355_LIBRARY.impl("rope", _rope_autograd, "Autograd")
 
 
 @CustomOp.register

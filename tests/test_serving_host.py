@@ -248,3 +248,26 @@ def test_oracle_verification_keeps_the_target_distribution():
         first = torch.where(count > 0, tokens[:4000].gather(1, path[:, :1].clamp(min=0).long())[:, 0], last)
         share = torch.bincount(first.long(), minlength=V).double() / 4000
         assert float((share - p).abs().max()) < 5 * math.sqrt(0.25 / 4000)
+
+
+def test_rope_gradient_formula_is_traced_and_differentiable_twice():
+    """On meta tensors and through make_fx the gradient is the op with `inverse` turned."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    x = m(5, 3, 96, dt=F32).requires_grad_()
+    pos, f = m(5, dt=I32), m(32, dt=F64)
+    y = OPS.rope(x, pos, f, False, False, 1.0)
+    g = m(5, 3, 96, dt=F32).requires_grad_()
+    first, = torch.autograd.grad(y, x, g, create_graph=True)
+    second, = torch.autograd.grad(first, g, m(5, 3, 96, dt=F32))
+    assert first.shape == second.shape == x.shape
+    with torch.no_grad():
+        assert not OPS.rope(x, pos, f, False, False, 1.0).requires_grad
+
+    def step(x, pos, f, dy):
+        x = x.detach().requires_grad_()
+        y = OPS.rope(x, pos, f, True, False, 2.0)
+        return torch.autograd.grad(y, x, dy)[0]
+
+    calls = [n for n in make_fx(step)(m(5, 3, 96, dt=F32), pos, f, m(5, 3, 96, dt=F32)).graph.nodes if "rope" in str(n.target)]
+    assert [n.args[4] for n in calls] == [False, True]
