@@ -18,6 +18,7 @@
 // V chunk c of row r -> slot c ^ (2 * (r & 7)).  As in the GEMM, the swizzle is applied on the
 // global side of the direct-to-LDS loads.
 #include "common.hpp"
+#include "tree.hpp"
 #include <math.h>
 #include <type_traits>
 
@@ -648,6 +649,18 @@ __device__ __forceinline__ int fa_find_unit(const FaVarlen& vl, int block_rows, 
   return -1;
 }
 
+// Drafted token trees over a paged cache (the TREE form of fa_fwd_d128_m16): the query rows of a (sequence, kv head) are all its
+// nodes' heads, row r = node r / group, head r % group; see paged_tree.hip for the operator.
+struct FaTree : FaPaged {
+  const int* parents;           // [batch][nodes]
+  float *part_acc, *part_ml;    // [batch][nodes][query heads][splits][128], [..][2]
+  int nodes, num_kv_heads, num_seqs, row_blocks, num_splits, chunk_tiles, ranked;
+};
+
+enum class FaForm { PLAIN, PAGED, VARLEN, TREE };
+template <FaForm F>
+using FaFormArgs = std::conditional_t<F == FaForm::VARLEN, FaVarlen, std::conditional_t<F == FaForm::TREE, FaTree, FaPaged>>;
+
 // The pipelined form on v_mfma_f32_16x16x32 (variant "..._m16").  Same tiles, rings, loads, passes and barriers as
 // fa_fwd_d128_pipe; what changes is the MFMA shape and with it every fragment layout.  On benchmark-like data a
 // 16x16x32 MFMA costs the board less energy per flop than a 32x32x16 (register-only loops with this tile's structure:
@@ -667,13 +680,19 @@ __device__ __forceinline__ int fa_find_unit(const FaVarlen& vl, int block_rows, 
 // the score MFMAs (vector work behind 48 of the trip's 64 MFMAs instead of 32).  Measured on 2 x 32 x 4096: ahead with
 // eight waves (unmasked 475 against 484 us), behind with four (causal 268 against 263); each form is built the way it
 // runs faster.
-template <bool CAUSAL, bool BF, int NW, bool SPREAD, bool PAGED = false, bool VARLEN = false>
+// QG: groups of 16 query rows per wave, 2 but for tree calls of at most 64 rows.
+template <bool CAUSAL, bool BF, int NW, bool SPREAD, FaForm FORM = FaForm::PLAIN, int QG = 2>
 __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2))) void fa_fwd_d128_m16(
     const half_t* __restrict__ Q, const half_t* __restrict__ K, const half_t* __restrict__ V, half_t* __restrict__ O, int BH,
-    int Sq_arg, int Sk_arg, float scale_log2e, int q_blocks_arg, FaLayout lay, std::conditional_t<VARLEN, FaVarlen, FaPaged> pg) {
+    int Sq_arg, int Sk_arg, float scale_log2e, int q_blocks_arg, FaLayout lay, FaFormArgs<FORM> pg) {
   extern __shared__ __attribute__((aligned(1024))) char lds[];
+  constexpr bool VARLEN = FORM == FaForm::VARLEN, TREE = FORM == FaForm::TREE, PAGED = FORM == FaForm::PAGED || TREE;
   static_assert(NW == 4 || !PAGED, "the paged form maps one page to one wave-load of a 4-wave workgroup");
-  constexpr int BLOCK_M = NW * 32, NI = 16 / NW;
+  static_assert(!TREE || !CAUSAL, "the tree form masks by ancestors");
+  // EXACT: the query fragments are the operand's own bits and scores are scaled in 32 bits, one multiplication per score;
+  // otherwise scale . log2(e) is folded into the query and rounded to 16 bits again.
+  constexpr bool EXACT = VARLEN || TREE;
+  constexpr int WAVE_M = QG * 16, BLOCK_M = NW * WAVE_M, NI = 16 / NW;
   constexpr int TILE_B = FA_BLOCK_N * 256, VBUF = 2 * TILE_B;
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -683,6 +702,7 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
   int units = CAUSAL ? (q_blocks + 1) / 2 : q_blocks;
   int bh, unit, b_idx, h_idx;
   size_t q_first = 0, k_first = 0;  // (VARLEN) the sequence's first rows
+  int split = 0, first_tile = 0;    // (TREE) the chunk of the keys, and where it begins
   if constexpr (VARLEN) {
     const int pid = blockIdx.x;
     if (pg.zero_rest) {
@@ -717,6 +737,21 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
     k_first = row;
     q_blocks = (Sq + BLOCK_M - 1) / BLOCK_M;
     bh = b_idx = 0;
+  } else if constexpr (TREE) {
+    // kv heads next to each other (they read the same pages), then a sequence's row blocks, sequences, chunks: the full
+    // chunks come first, the sequences' last ones make up the tail
+    int pid = blockIdx.x;
+    const int kvh = pid % pg.num_kv_heads;
+    pid /= pg.num_kv_heads;
+    unit = pid % pg.row_blocks;
+    pid /= pg.row_blocks;
+    b_idx = pid % pg.num_seqs;
+    split = pid / pg.num_seqs;
+    if (pg.ranked) b_idx = tree_rank(pg.seq_lens, pg.num_seqs, b_idx);
+    h_idx = kvh * lay.group;
+    bh = 0;
+    Sq = pg.nodes * lay.group;
+    q_blocks = units = pg.row_blocks;
   } else {
     const int pid = blockIdx.x;
     if (((BH / lay.group) & 7) == 0) {
@@ -735,7 +770,7 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
   if constexpr (PAGED) {
     // Sequences differ in length and workgroups are dispatched in grid order: take the sequences longest first,
     // so that the short ones make up the tail.  Thread t counts the sequences that come before sequence t.
-    const int num_seqs = BH / lay.H;
+    const int num_seqs = TREE ? 1 : BH / lay.H;
     if (num_seqs > 1 && num_seqs <= 256) {
       int* pick = reinterpret_cast<int*>(lds);
       const int t = threadIdx.x;
@@ -756,6 +791,33 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
     const int cap = (pg.max_pages * 16) << pg.page_shift;
     Sk = Sk < 0 ? 0 : (Sk > cap ? cap : Sk);
   }
+  bool single = true;  // (TREE) the sequence fits one chunk
+  int draft0 = 0;      // (TREE) position of node 0
+  if constexpr (TREE) {
+    draft0 = Sk - pg.nodes;
+    const int tiles = (Sk + FA_BLOCK_N - 1) / FA_BLOCK_N;
+    first_tile = split * pg.chunk_tiles;
+    if (first_tile >= tiles && split > 0) return;  // chunk 0 of an empty sequence writes its zeros
+    single = tiles <= pg.chunk_tiles;
+    // the ancestors of this block's rows, behind the rings
+    unsigned long long* seen = reinterpret_cast<unsigned long long*>(lds + 2 * FA_STAGE);
+    if (wave == 0) seen[lane] = tree_ancestors(pg.parents + (size_t)b_idx * pg.nodes, pg.nodes);
+    __syncthreads();
+    unsigned long long mine = 0;
+    if (threadIdx.x < BLOCK_M && unit * BLOCK_M + (int)threadIdx.x < Sq) mine = seen[(unit * BLOCK_M + threadIdx.x) / lay.group];
+    __syncthreads();
+    if (threadIdx.x < BLOCK_M) seen[threadIdx.x] = mine;
+    __syncthreads();
+  }
+  // where query row r lies behind Qb (and Ob), in elements
+  auto row_at = [&](int r, unsigned pitch) -> size_t {
+    if constexpr (TREE) {
+      const int node = r / lay.group;
+      return (size_t)node * pitch + (r - node * lay.group) * 128;
+    } else {
+      return (size_t)r * pitch;
+    }
+  };
   const int causal_off = Sk - Sq;
   const half_t* Qb = Q + (VARLEN ? q_first * lay.q_r : b_idx * lay.q_b) + h_idx * lay.q_h;
   const half_t* Kb = K + (PAGED ? 0 : VARLEN ? k_first * lay.k_r : b_idx * lay.k_b) + hk_idx * lay.k_h;
@@ -787,7 +849,7 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
   const int qb = CAUSAL ? (pass == 0 ? q_blocks - 1 - unit : unit) : unit;
   if (CAUSAL && pass == 1 && 2 * unit == q_blocks - 1) break;
   const int q0 = qb * BLOCK_M;
-  const int wq0 = q0 + wave * 32;
+  const int wq0 = q0 + wave * WAVE_M;
 
   int k_end = Sk;
   if (CAUSAL) {
@@ -796,19 +858,27 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
     int lim = last_q + causal_off + 1;
     if (lim < k_end) k_end = lim;
   }
-  const int n_tiles = k_end > 0 ? (k_end + FA_BLOCK_N - 1) / FA_BLOCK_N : 0;
+  int n_tiles = k_end > 0 ? (k_end + FA_BLOCK_N - 1) / FA_BLOCK_N : 0;
+  if constexpr (TREE) {
+    n_tiles -= first_tile;
+    n_tiles = n_tiles < pg.chunk_tiles ? n_tiles : pg.chunk_tiles;
+  }
 
   // Q fragments [query group][step over d], scale . log2(e) folded in and rounded to the 16-bit format again
-  half8 qf[2][4];
+  half8 qf[QG][4];
 #pragma unroll
-  for (int qg = 0; qg < 2; qg++) {
+  for (int qg = 0; qg < QG; qg++) {
     const int q_row = wq0 + qg * 16 + q16;
 #pragma unroll
     for (int ks = 0; ks < 4; ks++) {
       if (q_row < Sq) {
-        const half8 raw = *reinterpret_cast<const half8*>(Qb + (size_t)q_row * lay.q_r + ks * 32 + g * 8);
+        const half8 raw = *reinterpret_cast<const half8*>(Qb + row_at(q_row, lay.q_r) + ks * 32 + g * 8);
+        if constexpr (EXACT) {
+          qf[qg][ks] = raw;
+        } else {
 #pragma unroll
-        for (int e = 0; e < 8; e++) qf[qg][ks][e] = cvt16<BF>(to_f32<BF>(raw[e]) * scale_log2e);
+          for (int e = 0; e < 8; e++) qf[qg][ks][e] = cvt16<BF>(to_f32<BF>(raw[e]) * scale_log2e);
+        }
       } else {
 #pragma unroll
         for (int e = 0; e < 8; e++) qf[qg][ks][e] = (half_t)0;
@@ -866,18 +936,23 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
     }
   };
 
-  floatx4 oacc[8][2];  // [d group][query group]
+  floatx4 oacc[8][QG];  // [d group][query group]
 #pragma unroll
   for (int dg = 0; dg < 8; dg++)
 #pragma unroll
-    for (int qg = 0; qg < 2; qg++) oacc[dg][qg] = floatx4{0.f, 0.f, 0.f, 0.f};
+    for (int qg = 0; qg < QG; qg++) oacc[dg][qg] = floatx4{0.f, 0.f, 0.f, 0.f};
   // the negated running maximum of the lane's query in either group, four equal values: the addend of every score chain
-  floatx4 negm[2] = {floatx4{0.f, 0.f, 0.f, 0.f}, floatx4{0.f, 0.f, 0.f, 0.f}};
-  float l_run[2] = {0.f, 0.f};
-  float grow_thr[2] = {-INFINITY, -INFINITY};
-  constexpr float kRescaleThreshold = 8.f;
+  floatx4 negm[QG];
+  float l_run[QG], grow_thr[QG];
+#pragma unroll
+  for (int qg = 0; qg < QG; qg++) negm[qg] = floatx4{0.f, 0.f, 0.f, 0.f}, l_run[qg] = 0.f, grow_thr[qg] = -INFINITY;
+  const float score_mul = EXACT ? scale_log2e : 1.f;                // score units -> log2 units
+  const float kRescaleThreshold = EXACT ? 8.f / scale_log2e : 8.f;  // 2^8, in score units
 
-  auto wave_active = [&](int tile) { return !CAUSAL || (tile * FA_BLOCK_N <= wq0 + 31 + causal_off); };
+  auto wave_active = [&](int tile) {
+    if constexpr (TREE) return wq0 < Sq;  // a wave without rows only loads
+    else return !CAUSAL || (tile * FA_BLOCK_N <= wq0 + 31 + causal_off);
+  };
   auto kread = [&](int f, int koff) {  // K fragment f = kg * 4 + ks of the slot at koff
 #if defined(MI355_ABLATE_NO_K_READS)
     half8 stale = qf[0][f & 3];
@@ -888,24 +963,40 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
 #endif
   };
   // S^T of one tile, no softmax beside it (a pass's first tile)
-  auto scores = [&](int koff, floatx4 (*s)[2]) {
+  auto scores = [&](int koff, floatx4 (*s)[QG]) {
 #pragma unroll
     for (int f = 0; f < 16; f++) {
       const int kg = f >> 2, ks = f & 3;
       const half8 kf = kread(f, koff);
 #pragma unroll
-      for (int qg = 0; qg < 2; qg++) s[kg][qg] = mfma16_16x16x32<BF>(kf, qf[qg][ks], ks == 0 ? negm[qg] : s[kg][qg]);
+      for (int qg = 0; qg < QG; qg++) s[kg][qg] = mfma16_16x16x32<BF>(kf, qf[qg][ks], ks == 0 ? negm[qg] : s[kg][qg]);
     }
   };
 
-  auto softmax_pv = [&](int tile, auto voff_tag, floatx4 (*s)[2], int koff_next, floatx4 (*s_next)[2]) {
+  // `dropped` (TREE): bit i: the tile's 16-token block i has no page in the cache
+  auto softmax_pv = [&](int tile, int dropped, auto voff_tag, floatx4 (*s)[QG], int koff_next, floatx4 (*s_next)[QG]) {
     constexpr int VOFF = decltype(voff_tag)::value;
     {
       const int key0 = tile * FA_BLOCK_N;
+      if constexpr (TREE) {
+        if (key0 + FA_BLOCK_N > draft0 || dropped) {
+          const unsigned long long* seen = reinterpret_cast<const unsigned long long*>(lds + 2 * FA_STAGE) + wave * WAVE_M + q16;
+#pragma unroll
+          for (int qg = 0; qg < QG; qg++) {
+            const unsigned long long set = seen[qg * 16];
+#pragma unroll
+            for (int kg = 0; kg < 4; kg++) {
+              const unsigned vis = (dropped >> kg) & 1 ? 0u : tree_visible4(set, key0 + 16 * kg + 4 * g - draft0);
+#pragma unroll
+              for (int r = 0; r < 4; r++) s[kg][qg][r] = tree_hide(s[kg][qg][r], vis, r);
+            }
+          }
+        }
+      } else {
       const bool need_mask = (CAUSAL && (key0 + FA_BLOCK_N - 1 > wq0 + causal_off)) || (key0 + FA_BLOCK_N > Sk);
       if (need_mask) {
 #pragma unroll
-        for (int qg = 0; qg < 2; qg++) {
+        for (int qg = 0; qg < QG; qg++) {
           const int q_row = wq0 + qg * 16 + q16;
           const int lim = CAUSAL ? (q_row + causal_off < Sk - 1 ? q_row + causal_off : Sk - 1) : Sk - 1;  // last visible key
           const int rel = lim - key0 - 4 * g;
@@ -919,27 +1010,28 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
             }
         }
       }
+      }
     }
-    float mx[2];
+    float mx[QG];
 #pragma unroll
-    for (int qg = 0; qg < 2; qg++) {
+    for (int qg = 0; qg < QG; qg++) {
       mx[qg] = s[0][qg][0];
 #pragma unroll
       for (int kg = 0; kg < 4; kg++)
 #pragma unroll
         for (int r = 0; r < 4; r++) mx[qg] = fmaxf(mx[qg], s[kg][qg][r]);
     }
-    if (__builtin_amdgcn_ballot_w64(mx[0] > grow_thr[0] || mx[1] > grow_thr[1]) != 0) {
+    if (__builtin_amdgcn_ballot_w64(mx[0] > grow_thr[0] || mx[QG - 1] > grow_thr[QG - 1]) != 0) {
       // rare: some query's scores outgrew its maximum (or it saw its first key).  A query's keys are spread over the
       // four lanes q16 + 16 g; they take the same decision.
 #pragma unroll
-      for (int qg = 0; qg < 2; qg++) {
+      for (int qg = 0; qg < QG; qg++) {
         float mxx = fmaxf(mx[qg], __shfl_xor(mx[qg], 16));
         mxx = fmaxf(mxx, __shfl_xor(mxx, 32));
         if (mxx > grow_thr[qg]) {
           const bool fresh = grow_thr[qg] == -INFINITY;
           const float delta = fresh ? mxx : fmaxf(mxx, 0.f);  // (mxx > -inf here)
-          const float alpha = fresh ? 1.f : __builtin_amdgcn_exp2f(-delta);
+          const float alpha = fresh ? 1.f : __builtin_amdgcn_exp2f(EXACT ? -delta * score_mul : -delta);
           grow_thr[qg] = kRescaleThreshold;
           l_run[qg] *= alpha;
 #pragma unroll
@@ -960,24 +1052,27 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
     // ahead -- and one exponential of this tile, taken in the order the output MFMAs want the probabilities: key step,
     // query group, key group of the pair, r.  Every second step packs a pair; its dot2 (the row sum of what the second
     // contraction multiplies) runs one pair behind.  The empty statements tie the vector work to its step.
-    half8 pf[2][2];  // [query group][key step]
-    float psum[2] = {0.f, 0.f};
+    half8 pf[QG][2];  // [query group][key step]
+    float psum[QG];
+#pragma unroll
+    for (int qg = 0; qg < QG; qg++) psum[qg] = 0.f;
     half2v pp_prev = {(half_t)0, (half_t)0};
     // exponential e of the tile (0..31), in the order the output MFMAs want the probabilities: key step e / 16, query group
     // (e / 8) % 2, key group of the pair (e / 4) % 2, r = e % 4.  Every second one packs a pair; the pair's dot2 (the row
     // sum of what the second contraction multiplies) runs one pair behind.  The empty statements tie the work to its step.
     float e_even = 0.f;
     auto expo = [&](int e) {
-      const int st = e >> 4, eq = (e >> 3) & 1, ekg = 2 * st + ((e >> 2) & 1), r = e & 3;
+      const int st = e / (8 * QG), eq = (e >> 3) % QG, ekg = 2 * st + ((e >> 2) & 1), r = e & 3;
 #if defined(MI355_ABLATE_NO_EXP)
       const float ev = s[ekg][eq][r];
 #else
-      const float ev = __builtin_amdgcn_exp2f(s[ekg][eq][r]);
+      const float ev = __builtin_amdgcn_exp2f(EXACT ? s[ekg][eq][r] * score_mul : s[ekg][eq][r]);
 #endif
       if (e & 1) {
-        if (e > 1) psum[((e - 2) >> 3) & 1] = dot2_ones<BF>(pp_prev, psum[((e - 2) >> 3) & 1]);
+        if (e > 1) psum[((e - 2) >> 3) % QG] = dot2_ones<BF>(pp_prev, psum[((e - 2) >> 3) % QG]);
         half2v pp = cvt16x2<BF>(e_even, ev);
-        asm volatile("" : "+v"(pp), "+v"(psum[0]), "+v"(psum[1]));
+        if constexpr (QG == 2) asm volatile("" : "+v"(pp), "+v"(psum[0]), "+v"(psum[1]));
+        else asm volatile("" : "+v"(pp), "+v"(psum[0]));
         pf[eq][st][((e >> 2) & 1) * 4 + r - 1] = pp[0];
         pf[eq][st][((e >> 2) & 1) * 4 + r] = pp[1];
         pp_prev = pp;
@@ -997,8 +1092,8 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
       kf[1] = kread(1, koff_next);
       kf[2] = kread(2, koff_next);
 #pragma unroll
-      for (int i = 0; i < 32; i++) {
-        const int f = i >> 1, kg = f >> 2, ks = f & 3, qg = i & 1;
+      for (int i = 0; i < 16 * QG; i++) {
+        const int f = i / QG, kg = f >> 2, ks = f & 3, qg = i % QG;
         if (qg == 0 && f + 3 < 16) kf[(f + 3) & 3] = kread(f + 3, koff_next);
         s_next[kg][qg] = mfma16_16x16x32<BF>(kf[f & 3], qf[qg][ks], ks == 0 ? negm[qg] : s_next[kg][qg]);
         if (SPREAD) {
@@ -1042,46 +1137,68 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
       oacc[dg][0] = mfma16_16x16x32<BF>(vf, pf[0][st], oacc[dg][0]);
       if constexpr (SPREAD && f < 8) expo(16 + 2 * f);
       __builtin_amdgcn_sched_barrier(0);
-      oacc[dg][1] = mfma16_16x16x32<BF>(vf, pf[1][st], oacc[dg][1]);
-      if constexpr (SPREAD && f < 8) expo(16 + 2 * f + 1);
-      __builtin_amdgcn_sched_barrier(0);
+      if constexpr (QG == 2) {
+        oacc[dg][1] = mfma16_16x16x32<BF>(vf, pf[1][st], oacc[dg][1]);
+        if constexpr (SPREAD && f < 8) expo(16 + 2 * f + 1);
+        __builtin_amdgcn_sched_barrier(0);
+      }
       if constexpr (f == 7 || (!SPREAD && f == 0)) {  // the last pair's dot2 (it belongs to query group 1)
         if (SPREAD || f == 0) {
-          psum[1] = dot2_ones<BF>(pp_prev, psum[1]);
-          l_run[0] += psum[0];
-          l_run[1] += psum[1];
+          psum[QG - 1] = dot2_ones<BF>(pp_prev, psum[QG - 1]);
+#pragma unroll
+          for (int qg = 0; qg < QG; qg++) l_run[qg] += psum[qg];
         }
       }
     });
   };
 
-  floatx4 sa[4][2], sb[4][2];  // scores [key group][query group], two tiles
+  floatx4 sa[4][QG], sb[4][QG];  // scores [key group][query group], two tiles
   int k_ids[4] = {-1, -1, -1, -1}, v_ids[4] = {-1, -1, -1, -1};  // paged form: ids of the next K tile and the next V tile to fetch
+  // (TREE) which blocks of the present tile, the next one and the one behind have no page.  The plain paged form lets their
+  // rows read as zeros; a tree's query must not count them.
+  int drop0 = 0, drop1 = 0, drop2 = 0;
+  auto drops = [&](const int* ids) {
+    int d = 0;
+    if constexpr (TREE) {
+#pragma unroll
+      for (int i = 0; i < 4; i++) d |= (ids[i] < 0) << i;
+    }
+    return d;
+  };
   if (n_tiles > 0) {
-    load_ids(0, k_ids);
-    issue_kv(Kb, k_rb, k_voff, 0, 0, k_ids);
-    issue_kv(Vb, v_rb, v_voff, 0, VBUF, k_ids);
-    load_ids(1, v_ids);
-    if (n_tiles > 1) issue_kv(Kb, k_rb, k_voff, 1, TILE_B, v_ids);
-    load_ids(2, k_ids);  // what trip 0 issues: K(2) and V(1)
+    load_ids(first_tile, k_ids);
+    drop0 = drops(k_ids);
+    issue_kv(Kb, k_rb, k_voff, first_tile, 0, k_ids);
+    issue_kv(Vb, v_rb, v_voff, first_tile, VBUF, k_ids);
+    load_ids(first_tile + 1, v_ids);
+    drop1 = drops(v_ids);
+    if (n_tiles > 1) issue_kv(Kb, k_rb, k_voff, first_tile + 1, TILE_B, v_ids);
+    load_ids(first_tile + 2, k_ids);  // what trip 0 issues: K(2) and V(1)
+    drop2 = drops(k_ids);
     wait_vmcnt0();
     __syncthreads();
-    if (wave_active(0)) scores(0, sa);
+    if (wave_active(first_tile)) scores(0, sa);
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     __syncthreads();
   }
-  auto trip = [&](auto par_tag, int j, floatx4 (*s_cur)[2], floatx4 (*s_next)[2]) {
+  auto trip = [&](auto par_tag, int j, floatx4 (*s_cur)[QG], floatx4 (*s_next)[QG]) {
     constexpr int PAR = decltype(par_tag)::value;
     constexpr int K_CUR = PAR * TILE_B, K_NEXT = (1 - PAR) * TILE_B, V_CUR = VBUF + PAR * TILE_B, V_NEXT = VBUF + (1 - PAR) * TILE_B;
-    if (j + 2 < n_tiles) issue_kv(Kb, k_rb, k_voff, j + 2, K_CUR, k_ids);
-    if (j + 1 < n_tiles) issue_kv(Vb, v_rb, v_voff, j + 1, V_NEXT, v_ids);
+    if (j + 2 < n_tiles) issue_kv(Kb, k_rb, k_voff, first_tile + j + 2, K_CUR, k_ids);
+    if (j + 1 < n_tiles) issue_kv(Vb, v_rb, v_voff, first_tile + j + 1, V_NEXT, v_ids);
+    const int dropped = drop0;
     if constexpr (PAGED) {
       // the next trip fetches V(j+2) -- the tile whose ids K just used -- and K(j+3)
 #pragma unroll
       for (int i = 0; i < 4; i++) v_ids[i] = k_ids[i];
-      load_ids(j + 3, k_ids);
+      load_ids(first_tile + j + 3, k_ids);
+      if constexpr (TREE) {
+        drop0 = drop1;
+        drop1 = drop2;
+        drop2 = drops(k_ids);
+      }
     }
-    if (wave_active(j)) softmax_pv(j, std::integral_constant<int, V_CUR - VBUF>{}, s_cur, K_NEXT, s_next);
+    if (wave_active(first_tile + j)) softmax_pv(first_tile + j, dropped, std::integral_constant<int, V_CUR - VBUF>{}, s_cur, K_NEXT, s_next);
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
 #if !defined(MI355_ABLATE_NO_BARRIERS)
     __syncthreads();
@@ -1092,15 +1209,37 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
     if (j + 1 < n_tiles) trip(std::integral_constant<int, 1>{}, j + 1, sb, sa);
   }
 
-  {
+  if (TREE && !single) {
+    // partial results of the chunk: the unnormalised sums, their maximum in log2 units and weight
+    if constexpr (TREE) {
+      const int el = opaque_lane_id(), e16 = el & 15, eg = el >> 4;
+#pragma unroll
+      for (int qg = 0; qg < QG; qg++) {
+        float l_tot = l_run[qg] + __shfl_xor(l_run[qg], 16);
+        l_tot += __shfl_xor(l_tot, 32);
+        const int r = wq0 + qg * 16 + e16;
+        if (r < Sq) {
+          const int node = r / lay.group;
+          const size_t at = (((size_t)b_idx * pg.nodes + node) * lay.H + h_idx + (r - node * lay.group)) * pg.num_splits + split;
+          float* acc = pg.part_acc + at * 128 + 4 * eg;
+#pragma unroll
+          for (int dg = 0; dg < 8; dg++) *reinterpret_cast<floatx4*>(acc + dg * 16) = oacc[dg][qg];
+          if (eg == 0) {
+            pg.part_ml[at * 2] = grow_thr[qg] == -INFINITY ? -INFINITY : -negm[qg][0] * score_mul;
+            pg.part_ml[at * 2 + 1] = l_tot;
+          }
+        }
+      }
+    }
+  } else {
     // Output through LDS (the rings are idle: the last trip ended with a barrier): each wave assembles its 32 rows x 256
     // bytes in a private region (chunk c of row r in slot c ^ (r & 15)) from 8-byte pieces -- the lane holds d = 16 dg +
     // 4 g .. + 3 of its query in either group -- and stores whole rows, 16 bytes per lane.
     char* ep = lds + wave * 8192;
-    const int el = (CAUSAL || VARLEN) ? opaque_lane_id() : lane;  // (see fa_fwd_d128_pipe)
+    const int el = (CAUSAL || EXACT) ? opaque_lane_id() : lane;  // (see fa_fwd_d128_pipe)
     const int e16 = el & 15, eg = el >> 4;
 #pragma unroll
-    for (int qg = 0; qg < 2; qg++) {
+    for (int qg = 0; qg < QG; qg++) {
       float l_tot = l_run[qg] + __shfl_xor(l_run[qg], 16);
       l_tot += __shfl_xor(l_tot, 32);
       const float inv = l_tot > 0.f ? 1.f / l_tot : 0.f;
@@ -1113,10 +1252,10 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
     }
     const int er = el >> 4, ec = el & 15;
 #pragma unroll
-    for (int it = 0; it < 8; it++) {
+    for (int it = 0; it < WAVE_M / 4; it++) {
       const int row = it * 4 + er;
       const half8 v = *reinterpret_cast<const half8*>(ep + row * 256 + ((ec ^ (row & 15)) * 16));
-      if (wq0 + row < Sq) *reinterpret_cast<half8*>(Ob + (size_t)(wq0 + row) * lay.o_r + ec * 8) = v;
+      if (wq0 + row < Sq) *reinterpret_cast<half8*>(Ob + row_at(wq0 + row, lay.o_r) + ec * 8) = v;
     }
     if (CAUSAL) __syncthreads();  // the next pass loads K / V tiles over these regions
   }
@@ -1731,7 +1870,7 @@ static int fa_paged_prefill(const void* q, const void* k_cache, const void* v_ca
   const int BH = (int)(num_seqs * num_q_heads);
   const int q_blocks = (int)((num_new + FA_BLOCK_M - 1) / FA_BLOCK_M);
   const int lds_bytes = 2 * FA_STAGE;
-  auto kern = fa_fwd_d128_m16<true, BF, 4, false, true>;
+  auto kern = fa_fwd_d128_m16<true, BF, 4, false, FaForm::PAGED>;
   static std::atomic<uint64_t> lds_ok{0};
   if (int rc = allow_lds(reinterpret_cast<const void*>(kern), lds_bytes, lds_ok, "fa_fwd_d128_m16<paged>")) return rc;
   dim3 grid(BH * ((q_blocks + 1) / 2)), block(256);
@@ -1757,6 +1896,39 @@ extern "C" int mi355_paged_prefill_attn_bf16(const void* q, const void* k_cache,
   return fa_paged_prefill<true>(q, k_cache, v_cache, block_table, seq_lens, out, num_seqs, num_new, num_q_heads, num_kv_heads, D,
                                 page_size, max_pages_per_seq, num_pages, scale, stream);
 }
+
+namespace mi355 {
+
+// The tree form's launch: arguments checked by the caller (paged_tree.hip); chunk_steps counts 32-token steps and is even.
+template <bool BF, int QG>
+static int fa_tree_launch(const TreeArgs& a, int num_seqs, hipStream_t stream) {
+  auto kern = fa_fwd_d128_m16<false, BF, 4, false, FaForm::TREE, QG>;
+  constexpr int block_m = 64 * QG;
+  const int lds_bytes = 2 * FA_STAGE + block_m * (int)sizeof(unsigned long long);
+  static std::atomic<uint64_t> lds_ok{0};
+  if (int rc = allow_lds(reinterpret_cast<const void*>(kern), lds_bytes, lds_ok, "fa_fwd_d128_m16<tree>")) return rc;
+  const int hq = a.num_kv_heads * a.group;
+  FaLayout lay{};
+  lay.q_b = lay.o_b = (int64_t)a.nodes * hq * 128, lay.q_h = lay.o_h = 128, lay.q_r = lay.o_r = (unsigned)(hq * 128);
+  lay.k_h = lay.v_h = 128, lay.k_r = lay.v_r = (unsigned)(a.num_kv_heads * 128);
+  lay.H = hq, lay.group = a.group;
+  FaTree tr;
+  tr.block_table = a.table, tr.seq_lens = a.seq_lens, tr.max_pages = a.max_pages, tr.num_pages = a.num_pages, tr.page_shift = a.page_shift;
+  tr.parents = a.parents, tr.part_acc = a.part_acc, tr.part_ml = a.part_ml, tr.nodes = a.nodes, tr.num_kv_heads = a.num_kv_heads;
+  tr.num_seqs = num_seqs, tr.num_splits = a.num_splits, tr.chunk_tiles = a.chunk_steps / 2;
+  tr.row_blocks = (a.nodes * a.group + block_m - 1) / block_m, tr.ranked = a.ranked;
+  const int64_t wgs = (int64_t)num_seqs * a.num_kv_heads * tr.row_blocks * a.num_splits;
+  if (wgs >= (1ll << 31)) return fail(-MI355_E_SHAPE, "paged_tree_attn: too many workgroups");
+  dim3 grid((unsigned)wgs), block(256);
+  hipLaunchKernelGGL(kern, grid, block, lds_bytes, stream, a.q, a.kc, a.vc, a.out, 0, 0, 0, a.scale_log2e, 0, lay, tr);
+  return check_launch("fa_fwd_d128_m16<tree>", grid, block, lds_bytes);
+}
+int fa_tree(const TreeArgs& a, int num_seqs, bool bf16, hipStream_t stream) {
+  if (a.nodes * a.group <= 64) return bf16 ? fa_tree_launch<true, 1>(a, num_seqs, stream) : fa_tree_launch<false, 1>(a, num_seqs, stream);
+  return bf16 ? fa_tree_launch<true, 2>(a, num_seqs, stream) : fa_tree_launch<false, 2>(a, num_seqs, stream);
+}
+
+}  // namespace mi355
 
 template <bool BF>
 static int fa_varlen(const void* q, const void* k, const void* v, void* o, const int32_t* cu_q, const int32_t* cu_k, int64_t num_seqs,
@@ -1799,7 +1971,7 @@ static int fa_varlen(const void* q, const void* k, const void* v, void* o, const
   // the lengths are known on the device only: as many units as num_seqs sequences of total_q rows can have
   const int64_t units = total_q / (FA_BLOCK_M << pairs) + num_seqs;
   if (units * H >= (1ll << 31)) return fail(-MI355_E_SHAPE, "%s: too many query blocks", who);
-  auto kern = is_causal ? fa_fwd_d128_m16<true, BF, 4, false, false, true> : fa_fwd_d128_m16<false, BF, 4, false, false, true>;
+  auto kern = is_causal ? fa_fwd_d128_m16<true, BF, 4, false, FaForm::VARLEN> : fa_fwd_d128_m16<false, BF, 4, false, FaForm::VARLEN>;
   const int lds_bytes = 2 * FA_STAGE;
   static std::atomic<uint64_t> lds_ok[2] = {};
   if (int rc = allow_lds(reinterpret_cast<const void*>(kern), lds_bytes, lds_ok[is_causal ? 1 : 0], "fa_fwd_d128_m16<varlen>")) return rc;

@@ -13,69 +13,24 @@
 //
 // The table's reach is cut into num_splits chunks of equally many 32-token steps; a sequence that fits one chunk writes
 // its result directly, the others write fp32 partials that a second launch merges.
-#include "common.hpp"
+#include "tree.hpp"
 #include <math.h>
 
 namespace mi355 {
 
 constexpr int PT_WAVES = 4;
 constexpr int PT_WAVE_LDS = 2 * 8192;  // two stages of 32 V rows
-constexpr int PT_MAX_NODES = 64;
 constexpr int PT_MAX_GROUP = 128;  // query heads per kv head
 
-struct PtArgs {
-  const half_t *q, *kc, *vc;
-  const int *table, *seq_lens, *parents;
-  half_t* out;
-  float *part_acc, *part_ml;  // [S, N, Hq, splits, 128] and [.., 2]
-  int num_kv_heads, group, nodes, max_pages, num_pages, page_shift, num_splits, chunk_steps, row_blocks;
-  float scale_log2e;
-};
-
-// ancestors (and self) of node `lane` as a bit set; a parent that does not come before its node is none
-__device__ __forceinline__ unsigned long long pt_ancestors(const int* parents, int nodes) {
-  const int lane = threadIdx.x & 63;
-  int up = lane < nodes ? parents[lane] : -1;
-  up = (up >= 0 && up < lane) ? up : -1;
-  unsigned long long set = 1ull << lane;
-#pragma unroll
-  for (int i = 0; i < 6; i++) {
-    const int from = up < 0 ? lane : up;
-    const unsigned long long s = __shfl(set, from);
-    const int next = __shfl(up, from);
-    if (up >= 0) {
-      set |= s;
-      up = next;
-    }
-  }
-  return set;
-}
-
-// Which of the four positions d, .. , d + 3 (counted from the first draft) a node with ancestor set `seen` sees, as bits 0 .. 3:
-// all in front of the drafts, then the set's; the set has no bits behind the last draft.
-__device__ __forceinline__ unsigned pt_visible4(unsigned long long seen, int d) {
-  const int up = d > 0 ? (d < 63 ? d : 63) : 0, down = d < 0 ? (d > -4 ? -d : 4) : 0;
-  const unsigned w = d > 63 ? 0u : (unsigned)(seen >> up);
-  return (w << down) | ((1u << down) - 1u);
-}
-
-// v where bit r of `visible` is set, else -inf, by bit operations: the selection on a chain of conditions (dropped, behind
-// the end, a draft that is no ancestor) has been compiled to one that keeps the score.
-__device__ __forceinline__ float pt_hide(float v, unsigned visible, int r) {
-  const unsigned keep = (unsigned)((int)(visible << (31 - r)) >> 31);
-  return __builtin_bit_cast(float, (__builtin_bit_cast(unsigned, v) & keep) | (0xFF800000u & ~keep));
-}
-
 template <int C, bool BF>
-__global__ __launch_bounds__(PT_WAVES * 64) __attribute__((amdgpu_waves_per_eu(C == 4 ? 1 : 2, C == 4 ? 1 : 2))) void paged_tree_kernel(PtArgs a) {
+__global__ __launch_bounds__(PT_WAVES * 64) __attribute__((amdgpu_waves_per_eu(2, 2))) void paged_tree_kernel(TreeArgs a) {
   extern __shared__ __attribute__((aligned(1024))) char lds[];
-  constexpr int ROWS = 16 * C;
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int i16 = lane & 15, g = lane >> 4;
-  const int split = blockIdx.x / a.row_blocks, rb = blockIdx.x - split * a.row_blocks;
-  const int kvh = blockIdx.y, seq = blockIdx.z;
-  const int R = a.nodes * a.group, row0 = rb * ROWS;
+  const int kvh = blockIdx.x, split = blockIdx.z;
+  const int seq = a.ranked ? tree_rank(a.seq_lens, gridDim.y, blockIdx.y) : blockIdx.y;  // the full chunks first, the sequences' last ones in the tail
+  const int R = a.nodes * a.group;
   const int num_q_heads = a.num_kv_heads * a.group;
 
   const int reach = (a.max_pages << a.page_shift) * 16;
@@ -92,13 +47,13 @@ __global__ __launch_bounds__(PT_WAVES * 64) __attribute__((amdgpu_waves_per_eu(C
   const int n_steps = s_end - s_begin;
 
   unsigned long long* anc = reinterpret_cast<unsigned long long*>(lds);
-  if (wave == 0) anc[lane] = pt_ancestors(a.parents + (size_t)seq * a.nodes, a.nodes);
+  if (wave == 0) anc[lane] = tree_ancestors(a.parents + (size_t)seq * a.nodes, a.nodes);
   __syncthreads();
   unsigned long long seen[C];
   half8 qf[C][4];
 #pragma unroll
   for (int c = 0; c < C; c++) {
-    const int r = row0 + c * 16 + i16;
+    const int r = c * 16 + i16;
     const int node = r < R ? r / a.group : 0;
     const int head = kvh * a.group + (r < R ? r - node * a.group : 0);
     seen[c] = anc[node];
@@ -114,7 +69,10 @@ __global__ __launch_bounds__(PT_WAVES * 64) __attribute__((amdgpu_waves_per_eu(C
   }
   __syncthreads();  // the words are part of the V ring
 
-  const int* bt = a.table + (size_t)seq * a.max_pages;
+  // page ids come through the scalar cache (constant address space: the table is not written while the kernel runs): a
+  // vector load would have to be waited for in the order of the K and V loads in flight
+  typedef const int __attribute__((address_space(4)))* table_ptr_t;
+  const table_ptr_t bt = (table_ptr_t)(unsigned long long)(a.table + (size_t)seq * a.max_pages);
   char* my_lds = lds + wave * PT_WAVE_LDS;
   const size_t tok_stride = (size_t)a.num_kv_heads * 128;
   const half_t* k_lane = a.kc + (size_t)kvh * 128 + i16 * tok_stride + g * 8;
@@ -190,12 +148,12 @@ __global__ __launch_bounds__(PT_WAVES * 64) __attribute__((amdgpu_waves_per_eu(C
 #pragma unroll
           for (int ks = 0; ks < 4; ks++) s1 = mfma16_16x16x32<BF>(kf[b][1][ks], qf[c][ks], s1);
           if (edge) {
-            const unsigned vis0 = drop0 ? 0u : pt_visible4(seen[c], tok0 - draft0);
-            const unsigned vis1 = drop1 ? 0u : pt_visible4(seen[c], tok0 + 16 - draft0);
+            const unsigned vis0 = drop0 ? 0u : tree_visible4(seen[c], tok0 - draft0);
+            const unsigned vis1 = drop1 ? 0u : tree_visible4(seen[c], tok0 + 16 - draft0);
 #pragma unroll
             for (int r = 0; r < 4; r++) {
-              s0[r] = pt_hide(s0[r], vis0, r);
-              s1[r] = pt_hide(s1[r], vis1, r);
+              s0[r] = tree_hide(s0[r], vis0, r);
+              s1[r] = tree_hide(s1[r], vis1, r);
             }
           }
           float mx = fmaxf(fmaxf(fmaxf(s0[0], s0[1]), fmaxf(s0[2], s0[3])), fmaxf(fmaxf(s1[0], s1[1]), fmaxf(s1[2], s1[3])));
@@ -256,7 +214,7 @@ __global__ __launch_bounds__(PT_WAVES * 64) __attribute__((amdgpu_waves_per_eu(C
     for (int dt = 0; dt < 8; dt++) *reinterpret_cast<floatx4*>(sacc + ((wave * 16 + i16) * 128 + dt * 16 + 4 * g)) = oacc[c][dt];
     __syncthreads();
     for (int idx = threadIdx.x; idx < 16 * 128; idx += PT_WAVES * 64) {
-      const int col = idx >> 7, d = idx & 127, r = row0 + c * 16 + col;
+      const int col = idx >> 7, d = idx & 127, r = c * 16 + col;
       if (r >= R) continue;
       float m_tot = -INFINITY;
 #pragma unroll
@@ -287,61 +245,90 @@ __global__ __launch_bounds__(PT_WAVES * 64) __attribute__((amdgpu_waves_per_eu(C
   }
 }
 
-// Merge of the chunks of every row whose sequence has more than one: one wave per row, two elements per lane.
-template <bool BF>
-__global__ __launch_bounds__(64) void paged_tree_merge_kernel(PtArgs a) {
-  const size_t row = blockIdx.x;
-  const int rows_per_seq = a.nodes * a.num_kv_heads * a.group;
-  const int seq = (int)(row / rows_per_seq);
+// Merge of the chunks of every row whose sequence has more than one.  A row's 128 sums are 32 lanes of 16 bytes, so that a
+// group of 32 lanes takes a chunk at a time; GROUPS of them share a row's chunks and add up through LDS (few chunks: one group
+// per row, eight rows per workgroup; many: the whole workgroup on one row, so that a row waits for memory
+// num_splits / 8 times and not num_splits times).
+template <bool BF, int GROUPS>
+__global__ __launch_bounds__(256) void paged_tree_merge_kernel(TreeArgs a, int num_rows) {
+  constexpr int ROWS = 8 / GROUPS;
+  __shared__ floatx4 sum[8][32];
+  __shared__ float weight[8];
+  const int l32 = threadIdx.x & 31, grp = threadIdx.x >> 5;
+  const int row = blockIdx.x * ROWS + grp / GROUPS, part = grp % GROUPS;
+  const bool on = row < num_rows;
+  const int seq = (on ? row : 0) / (a.nodes * a.num_kv_heads * a.group);
   const int reach = (a.max_pages << a.page_shift) * 16;
   const int L_in = a.seq_lens[seq];
   const int L = L_in < 0 ? 0 : (L_in > reach ? reach : L_in);
   const int steps = (L + 31) >> 5;
-  if (steps <= a.chunk_steps) return;
-  const int n = (steps + a.chunk_steps - 1) / a.chunk_steps;
-  const int lane = threadIdx.x;
-  const float* ml = a.part_ml + row * a.num_splits * 2;
+  const int n = !on || steps <= a.chunk_steps ? 0 : (steps + a.chunk_steps - 1) / a.chunk_steps;
+  const float* ml = a.part_ml + (size_t)row * a.num_splits * 2;
+  const float* acc = a.part_acc + (size_t)row * a.num_splits * 128 + l32 * 4;
   float m_tot = -INFINITY;
-  for (int s = 0; s < n; s++) m_tot = fmaxf(m_tot, ml[2 * s]);
-  float a0 = 0.f, a1 = 0.f, l = 0.f;
+  for (int s = l32; s < n; s += 32) m_tot = fmaxf(m_tot, ml[2 * s]);
+#pragma unroll
+  for (int d = 16; d >= 1; d >>= 1) m_tot = fmaxf(m_tot, __shfl_xor(m_tot, d));
+  floatx4 o = {0.f, 0.f, 0.f, 0.f};
+  float l = 0.f;
   if (m_tot > -INFINITY) {
-    for (int s = 0; s < n; s++) {
+#pragma unroll 4
+    for (int s = part; s < n; s += GROUPS) {
       const float w = __builtin_amdgcn_exp2f(ml[2 * s] - m_tot);
-      const floatx2 p = *reinterpret_cast<const floatx2*>(a.part_acc + (row * a.num_splits + s) * 128 + 2 * lane);
-      a0 = __builtin_fmaf(w, p[0], a0);
-      a1 = __builtin_fmaf(w, p[1], a1);
+      const floatx4 p = *reinterpret_cast<const floatx4*>(acc + (size_t)s * 128);
       l = __builtin_fmaf(w, ml[2 * s + 1], l);
+#pragma unroll
+      for (int e = 0; e < 4; e++) o[e] = __builtin_fmaf(w, p[e], o[e]);
     }
   }
+  if constexpr (GROUPS > 1) {
+    sum[grp][l32] = o;
+    if (l32 == 0) weight[grp] = l;
+    __syncthreads();
+    if (grp % GROUPS) return;
+#pragma unroll
+    for (int k = 1; k < GROUPS; k++) {
+      const floatx4 p = sum[grp + k][l32];
+      l += weight[grp + k];
+#pragma unroll
+      for (int e = 0; e < 4; e++) o[e] += p[e];
+    }
+  }
+  if (n == 0) return;
   const float inv = l > 0.f ? 1.f / l : 0.f;
-  *reinterpret_cast<half2v*>(a.out + row * 128 + 2 * lane) = cvt16x2<BF>(a0 * inv, a1 * inv);
+  const half4 v = {cvt16<BF>(o[0] * inv), cvt16<BF>(o[1] * inv), cvt16<BF>(o[2] * inv), cvt16<BF>(o[3] * inv)};
+  *reinterpret_cast<half4*>(a.out + (size_t)row * 128 + l32 * 4) = v;
+}
+
+template <bool BF, int GROUPS>
+static int launch_merge(const TreeArgs& a, int64_t rows, hipStream_t stream) {
+  dim3 grid((unsigned)((rows * GROUPS + 7) / 8)), block(256);
+  hipLaunchKernelGGL((paged_tree_merge_kernel<BF, GROUPS>), grid, block, 0, stream, a, (int)rows);
+  return check_launch("paged_tree_merge_kernel", grid, block, 0);
 }
 
 template <int C, bool BF>
-static int launch_tree(const PtArgs& a, int num_seqs, hipStream_t stream) {
+static int launch_tree(const TreeArgs& a, int num_seqs, hipStream_t stream) {
   auto kern = paged_tree_kernel<C, BF>;
   constexpr int lds_bytes = PT_WAVES * PT_WAVE_LDS;
   static_assert(lds_bytes >= (int)((2 * PT_WAVES * 16 + PT_WAVES * 16 * 128) * sizeof(float)), "merge area must fit");
   static std::atomic<uint64_t> lds_ok{0};
   if (int rc = allow_lds(reinterpret_cast<const void*>(kern), lds_bytes, lds_ok, "paged_tree_kernel")) return rc;
-  dim3 grid(a.num_splits * a.row_blocks, a.num_kv_heads, num_seqs), block(PT_WAVES * 64);
+  dim3 grid(a.num_kv_heads, num_seqs, a.num_splits), block(PT_WAVES * 64);
   hipLaunchKernelGGL(kern, grid, block, lds_bytes, stream, a);
   return check_launch("paged_tree_kernel", grid, block, lds_bytes);
 }
 
 template <bool BF>
-static int run_tree(PtArgs a, int num_seqs, hipStream_t stream) {
+static int run_tree(TreeArgs a, int num_seqs, hipStream_t stream) {
   const int R = a.nodes * a.group;
-  const int C = R <= 16 ? 1 : R <= 32 ? 2 : 4;
-  a.row_blocks = (R + 16 * C - 1) / (16 * C);
   int rc;
-  if (C == 1) rc = launch_tree<1, BF>(a, num_seqs, stream);
-  else if (C == 2) rc = launch_tree<2, BF>(a, num_seqs, stream);
-  else rc = launch_tree<4, BF>(a, num_seqs, stream);
+  if (R <= 16) rc = launch_tree<1, BF>(a, num_seqs, stream);
+  else if (R <= 32) rc = launch_tree<2, BF>(a, num_seqs, stream);
+  else rc = fa_tree(a, num_seqs, BF, stream);
   if (rc || a.num_splits == 1) return rc;
-  dim3 grid((unsigned)((int64_t)num_seqs * R * a.num_kv_heads)), block(64);
-  hipLaunchKernelGGL(paged_tree_merge_kernel<BF>, grid, block, 0, stream, a);
-  return check_launch("paged_tree_merge_kernel", grid, block, 0);
+  const int64_t rows = (int64_t)num_seqs * R * a.num_kv_heads;
+  return a.num_splits <= 8 ? launch_merge<BF, 1>(a, rows, stream) : launch_merge<BF, 8>(a, rows, stream);
 }
 
 }  // namespace mi355
@@ -361,8 +348,8 @@ extern "C" int mi355_paged_tree_attn(const void* q, const void* k_cache, const v
   for (int sh = 0; sh <= 4; sh++)
     if (page_size == (16ll << sh)) page_shift = sh;
   if (page_shift < 0) return fail(-MI355_E_SHAPE, "%s: page size %lld not supported (16, 32, 64, 128 or 256)", fn, (long long)page_size);
-  if (num_nodes <= 0 || num_nodes > PT_MAX_NODES)
-    return fail(-MI355_E_SHAPE, "%s: %lld nodes per sequence, supported: 1 to %d", fn, (long long)num_nodes, PT_MAX_NODES);
+  if (num_nodes <= 0 || num_nodes > TREE_MAX_NODES)
+    return fail(-MI355_E_SHAPE, "%s: %lld nodes per sequence, supported: 1 to %d", fn, (long long)num_nodes, TREE_MAX_NODES);
   if (num_seqs <= 0 || num_seqs > 65535 || num_q_heads <= 0 || num_kv_heads <= 0 || num_kv_heads > 65535 || num_q_heads > 65535 ||
       max_pages_per_seq <= 0 || max_pages_per_seq > (1 << 22) || num_pages <= 0 || num_pages > (1 << 26) ||
       num_seqs * num_nodes * num_q_heads > (1ll << 30) || max_pages_per_seq * page_size > (1ll << 30))
@@ -380,10 +367,10 @@ extern "C" int mi355_paged_tree_attn(const void* q, const void* k_cache, const v
   if (num_splits > 1 && (!part_acc || !part_ml)) return fail(-MI355_E_SCRATCH, "%s: num_splits > 1 needs part_acc / part_ml scratch", fn);
   if (num_splits > 1 && !aligned16(part_acc)) return fail(-MI355_E_ALIGN, "%s: part_acc must be 16-byte aligned", fn);
   const int64_t reach_steps = (max_pages_per_seq * page_size + 31) / 32;
-  PtArgs a{(const half_t*)q, (const half_t*)k_cache, (const half_t*)v_cache, block_table, seq_lens, parents, (half_t*)out,
+  TreeArgs a{(const half_t*)q, (const half_t*)k_cache, (const half_t*)v_cache, block_table, seq_lens, parents, (half_t*)out,
            part_acc, part_ml, (int)num_kv_heads, (int)(num_q_heads / num_kv_heads), (int)num_nodes, (int)max_pages_per_seq,
-           (int)num_pages, page_shift, (int)num_splits, (int)((reach_steps + num_splits - 1) / num_splits), 1,
-           scale * 1.4426950408889634f};
+           (int)num_pages, page_shift, (int)num_splits, (int)((reach_steps + 2 * num_splits - 1) / (2 * num_splits)) * 2,
+           num_seqs > 1 && num_seqs <= 64, scale * 1.4426950408889634f};
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   return dtype == MI355_BF16 ? run_tree<true>(a, (int)num_seqs, s) : run_tree<false>(a, (int)num_seqs, s);
 }
