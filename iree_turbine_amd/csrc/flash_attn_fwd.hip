@@ -654,7 +654,7 @@ __device__ __forceinline__ int fa_find_unit(const FaVarlen& vl, int block_rows, 
 struct FaTree : FaPaged {
   const int* parents;           // [batch][nodes]
   float *part_acc, *part_ml;    // [batch][nodes][query heads][splits][128], [..][2]
-  int nodes, num_kv_heads, num_seqs, row_blocks, num_splits, chunk_tiles, ranked;
+  int nodes, num_kv_heads, num_seqs, row_blocks, num_splits, chunk_tiles;
 };
 
 enum class FaForm { PLAIN, PAGED, VARLEN, TREE };
@@ -738,16 +738,13 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
     q_blocks = (Sq + BLOCK_M - 1) / BLOCK_M;
     bh = b_idx = 0;
   } else if constexpr (TREE) {
-    // kv heads next to each other (they read the same pages), then a sequence's row blocks, sequences, chunks: the full
-    // chunks come first, the sequences' last ones make up the tail
+    // kv heads next to each other (they read the same pages), then row blocks, then pieces of work
     int pid = blockIdx.x;
     const int kvh = pid % pg.num_kv_heads;
     pid /= pg.num_kv_heads;
     unit = pid % pg.row_blocks;
-    pid /= pg.row_blocks;
-    b_idx = pid % pg.num_seqs;
-    split = pid / pg.num_seqs;
-    if (pg.ranked) b_idx = tree_rank(pg.seq_lens, pg.num_seqs, b_idx);
+    if (!tree_item(pg.seq_lens, pg.num_seqs, pg.num_splits, pg.chunk_tiles * 2, (pg.max_pages * 16) << pg.page_shift, pid / pg.row_blocks, b_idx, split))
+      return;
     h_idx = kvh * lay.group;
     bh = 0;
     Sq = pg.nodes * lay.group;
@@ -1916,8 +1913,8 @@ static int fa_tree_launch(const TreeArgs& a, int num_seqs, hipStream_t stream) {
   tr.block_table = a.table, tr.seq_lens = a.seq_lens, tr.max_pages = a.max_pages, tr.num_pages = a.num_pages, tr.page_shift = a.page_shift;
   tr.parents = a.parents, tr.part_acc = a.part_acc, tr.part_ml = a.part_ml, tr.nodes = a.nodes, tr.num_kv_heads = a.num_kv_heads;
   tr.num_seqs = num_seqs, tr.num_splits = a.num_splits, tr.chunk_tiles = a.chunk_steps / 2;
-  tr.row_blocks = (a.nodes * a.group + block_m - 1) / block_m, tr.ranked = a.ranked;
-  const int64_t wgs = (int64_t)num_seqs * a.num_kv_heads * tr.row_blocks * a.num_splits;
+  tr.row_blocks = (a.nodes * a.group + block_m - 1) / block_m;
+  const int64_t wgs = (int64_t)num_seqs * a.num_splits * a.num_kv_heads * tr.row_blocks;
   if (wgs >= (1ll << 31)) return fail(-MI355_E_SHAPE, "paged_tree_attn: too many workgroups");
   dim3 grid((unsigned)wgs), block(256);
   hipLaunchKernelGGL(kern, grid, block, lds_bytes, stream, a.q, a.kc, a.vc, a.out, 0, 0, 0, a.scale_log2e, 0, lay, tr);

@@ -28,12 +28,13 @@ __global__ __launch_bounds__(PT_WAVES * 64) __attribute__((amdgpu_waves_per_eu(2
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int i16 = lane & 15, g = lane >> 4;
-  const int kvh = blockIdx.x, split = blockIdx.z;
-  const int seq = a.ranked ? tree_rank(a.seq_lens, gridDim.y, blockIdx.y) : blockIdx.y;  // the full chunks first, the sequences' last ones in the tail
+  const int reach = (a.max_pages << a.page_shift) * 16;
+  const int kvh = blockIdx.x % a.num_kv_heads;
+  int seq, split;
+  if (!tree_item(a.seq_lens, a.num_seqs, a.num_splits, a.chunk_steps, reach, blockIdx.x / a.num_kv_heads, seq, split)) return;
   const int R = a.nodes * a.group;
   const int num_q_heads = a.num_kv_heads * a.group;
 
-  const int reach = (a.max_pages << a.page_shift) * 16;
   const int L_in = a.seq_lens[seq];
   const int L = L_in < 0 ? 0 : (L_in > reach ? reach : L_in);
   const int draft0 = L - a.nodes;  // position of node 0 (negative: the first nodes are not in the cache)
@@ -314,7 +315,7 @@ static int launch_tree(const TreeArgs& a, int num_seqs, hipStream_t stream) {
   static_assert(lds_bytes >= (int)((2 * PT_WAVES * 16 + PT_WAVES * 16 * 128) * sizeof(float)), "merge area must fit");
   static std::atomic<uint64_t> lds_ok{0};
   if (int rc = allow_lds(reinterpret_cast<const void*>(kern), lds_bytes, lds_ok, "paged_tree_kernel")) return rc;
-  dim3 grid(a.num_kv_heads, num_seqs, a.num_splits), block(PT_WAVES * 64);
+  dim3 grid((unsigned)((int64_t)num_seqs * a.num_splits * a.num_kv_heads)), block(PT_WAVES * 64);
   hipLaunchKernelGGL(kern, grid, block, lds_bytes, stream, a);
   return check_launch("paged_tree_kernel", grid, block, lds_bytes);
 }
@@ -370,7 +371,7 @@ extern "C" int mi355_paged_tree_attn(const void* q, const void* k_cache, const v
   TreeArgs a{(const half_t*)q, (const half_t*)k_cache, (const half_t*)v_cache, block_table, seq_lens, parents, (half_t*)out,
            part_acc, part_ml, (int)num_kv_heads, (int)(num_q_heads / num_kv_heads), (int)num_nodes, (int)max_pages_per_seq,
            (int)num_pages, page_shift, (int)num_splits, (int)((reach_steps + 2 * num_splits - 1) / (2 * num_splits)) * 2,
-           num_seqs > 1 && num_seqs <= 64, scale * 1.4426950408889634f};
+           (int)num_seqs, scale * 1.4426950408889634f};
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   return dtype == MI355_BF16 ? run_tree<true>(a, (int)num_seqs, s) : run_tree<false>(a, (int)num_seqs, s);
 }

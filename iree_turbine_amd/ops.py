@@ -629,6 +629,15 @@ class flash_attn_varlen_fwd(CustomOp):
         return launch._flash_attn_varlen_fwd(dev, q, k, v, cu_seqlens_q, cu_seqlens_k, out, is_causal, scale, True)
 
 
+def default_num_tree_splits(reach: int, num_seqs: int, rows: int, num_kv_heads: int) -> int:
+    """Chunks of a table's reach for paged_tree_attn: about 1024 workgroups (two rounds of what is resident; the kernels hand out
+    full chunks first) where the batch is small, of at least 512 tokens each and at most 32.  Measured: 64 sequences of
+    512-8192 tokens with 64 rows 231 / 170 / 175 / 206 us with 1 / 2 / 3 / 8 chunks; 16 of them with 128 rows 77 / 61 / 78 with
+    4 / 8 / 12; one of 32768 tokens 42 / 36 / 36 / 41 with 16 / 24 / 32 / 64."""
+    blocks = num_seqs * num_kv_heads * -(-rows // 128)
+    return max(1, min(1024 // blocks if blocks <= 1024 else 1, reach // 512, 32))
+
+
 @CustomOp.register
 class paged_tree_attn(CustomOp):
     """Attention of drafted token trees over the paged cache: q [S, N, Hq, 128], N <= 64 nodes per sequence, whose K/V are the last N
@@ -649,7 +658,7 @@ class paged_tree_attn(CustomOp):
 
     def eager_execute(self, q, k_cache, v_cache, block_table, seq_lens, parents, scale, num_kv_splits):
         if num_kv_splits <= 0:
-            num_kv_splits = default_num_kv_splits(block_table.size(1) * k_cache.size(1), q.size(0), k_cache.size(2))
+            num_kv_splits = default_num_tree_splits(block_table.size(1) * k_cache.size(1), q.size(0), q.size(1) * q.size(2) // k_cache.size(2), k_cache.size(2))
         _require(num_kv_splits <= 1024, "paged_tree_attn: num_kv_splits must be at most 1024")
         dev = launch._dev(q, k_cache, v_cache, block_table, seq_lens, parents)
         out = torch.empty(q.shape, dtype=q.dtype, device=dev)
