@@ -214,6 +214,10 @@ class CustomOp(ABC):
     @abstractmethod
     def select(self, sel: KernelSelection): ...
 
+    # check(*args): the op's contract by itself, for ops whose `select` describes a call beyond checking it.  Where it is given
+    # a launch runs it in place of `select`, whose descriptors only the Meta kernel and a spec key need.
+    check: Optional[Callable[..., None]] = None
+
     def eager_execute(self, *args):
         return NotImplemented
 
@@ -245,8 +249,10 @@ def device_impl(op: CustomOp):
     """The callable behind the op's device dispatch key: the contract, then the launch."""
 
     def handler(*args):
-        sel = KernelSelection(op, args)
-        op.select(sel)  # validates shapes / dtypes before anything is launched
+        if op.check is not None:
+            op.check(*args)
+        else:
+            op.select(KernelSelection(op, args))  # validates shapes / dtypes before anything is launched
         result = op.eager_execute(*args)
         if result is NotImplemented:
             raise NotImplementedError(f"{op.name}: no device implementation (eager_execute returned NotImplemented)")

@@ -468,14 +468,18 @@ class paged_batch_layout(CustomOp):
     signature = "paged_batch_layout(Tensor(a!) block_table, Tensor context_lens, Tensor new_lens, Tensor free_pages, int page_size, int num_tokens) -> (Tensor, Tensor, Tensor, Tensor, Tensor, Tensor)"
 
     def select(self, sel: KernelSelection):
-        bt, cl, nl, fp = (sel.arg_tensor(i) for i in range(4))
-        page, T = sel.attr_int(4).v, sel.arg_int(5).v
-        contract.check_batch_layout("paged_batch_layout", bt.t, cl.t, nl.t, fp.t, page, T)
+        _, cl, _, _ = (sel.arg_tensor(i) for i in range(4))
+        sel.attr_int(4)
+        T = sel.arg_int(5).v
+        self.check(*sel.args)
         S = cl.t.size(0)
         for n in (S, S + 1, T, T):
             sel.return_new_tensor([n], torch.int32)
         sel.return_new_tensor([T], torch.int64)
         sel.return_new_tensor([1], torch.int32)
+
+    def check(self, block_table, context_lens, new_lens, free_pages, page_size, num_tokens):
+        contract.check_batch_layout("paged_batch_layout", block_table, context_lens, new_lens, free_pages, page_size, num_tokens)
 
     def eager_execute(self, block_table, context_lens, new_lens, free_pages, page_size, num_tokens):
         dev = launch._dev(block_table, context_lens, new_lens, free_pages)
@@ -522,13 +526,16 @@ class rope(CustomOp):
     signature = "rope(Tensor x, Tensor positions, Tensor inv_freq, bool interleaved, bool inverse, float scale) -> Tensor"
 
     def select(self, sel: KernelSelection):
-        x, pos, freq = (sel.arg_tensor(i) for i in range(3))
+        x, _, _ = (sel.arg_tensor(i) for i in range(3))
         sel.attr_bool(3)
         sel.attr_bool(4)
         sel.attr_float(5)
-        contract.check_rope("rope", x.t, pos.t, freq.t)
+        self.check(*sel.args)
         x.specialize_dims(1, 2)
         sel.return_new_tensor(list(x.t.shape), x.t.dtype)
+
+    def check(self, x, positions, inv_freq, *_):
+        contract.check_rope("rope", x, positions, inv_freq)
 
     def eager_execute(self, x, positions, inv_freq, interleaved, inverse, scale):
         dev = launch._dev(x, positions, inv_freq)
@@ -591,12 +598,15 @@ class rope_kv_append(CustomOp):
     signature = "rope_kv_append(Tensor q, Tensor k_new, Tensor v_new, Tensor positions, Tensor inv_freq, Tensor(a!) k_cache, Tensor(b!) v_cache, Tensor slots, bool interleaved, float scale) -> Tensor"
 
     def select(self, sel: KernelSelection):
-        q, kn, vn, pos, freq, kc, vc, sl = (sel.arg_tensor(i) for i in range(8))
+        q = [sel.arg_tensor(i) for i in range(8)][0]
         sel.attr_bool(8)
         sel.attr_float(9)
-        contract.check_rope_append("rope_kv_append", q.t, kn.t, vn.t, pos.t, freq.t, kc.t, vc.t, sl.t)
+        self.check(*sel.args)
         q.specialize_dims(1, 2)
         sel.return_new_tensor(list(q.t.shape), q.t.dtype)
+
+    def check(self, q, k_new, v_new, positions, inv_freq, k_cache, v_cache, slots, *_):
+        contract.check_rope_append("rope_kv_append", q, k_new, v_new, positions, inv_freq, k_cache, v_cache, slots)
 
     def eager_execute(self, q, k_new, v_new, positions, inv_freq, k_cache, v_cache, slots, interleaved, scale):
         dev = launch._dev(q, k_new, v_new, positions, inv_freq, k_cache, v_cache, slots)
@@ -615,13 +625,16 @@ class flash_attn_varlen_fwd(CustomOp):
     signature = "flash_attn_varlen_fwd(Tensor q, Tensor k, Tensor v, Tensor cu_seqlens_q, Tensor cu_seqlens_k, bool is_causal, float scale) -> Tensor"
 
     def select(self, sel: KernelSelection):
-        q, k, v, cq, ck = (sel.arg_tensor(i) for i in range(5))
+        q, k, v, _, _ = (sel.arg_tensor(i) for i in range(5))
         sel.attr_bool(5)
         sel.attr_float(6)
-        contract.check_varlen_attention("flash_attn_varlen_fwd", q.t, k.t, v.t, cq.t, ck.t)
+        self.check(*sel.args)
         for d in (q, k, v):
             d.specialize_dims(1, 2)
         sel.return_new_tensor(list(q.t.shape), q.t.dtype)
+
+    def check(self, q, k, v, cu_seqlens_q, cu_seqlens_k, *_):
+        contract.check_varlen_attention("flash_attn_varlen_fwd", q, k, v, cu_seqlens_q, cu_seqlens_k)
 
     def eager_execute(self, q, k, v, cu_seqlens_q, cu_seqlens_k, is_causal, scale):
         dev = launch._dev(q, k, v, cu_seqlens_q, cu_seqlens_k)
@@ -649,17 +662,21 @@ class paged_tree_attn(CustomOp):
     signature = "paged_tree_attn(Tensor q, Tensor k_cache, Tensor v_cache, Tensor block_table, Tensor seq_lens, Tensor parents, float scale, int num_kv_splits) -> Tensor"
 
     def select(self, sel: KernelSelection):
-        q, kc, vc, bt, sl, par = (sel.arg_tensor(i) for i in range(6))
+        q = [sel.arg_tensor(i) for i in range(6)][0]
         sel.attr_float(6)
         sel.attr_int(7)
-        contract.check_tree_attention("paged_tree_attn", q.t, kc.t, vc.t, bt.t, sl.t, par.t)
+        self.check(*sel.args)
         q.specialize_dims(1, 2, 3)
         sel.return_new_tensor(list(q.t.shape), q.t.dtype)
+
+    def check(self, q, k_cache, v_cache, block_table, seq_lens, parents, scale, num_kv_splits):
+        contract.check_tree_attention("paged_tree_attn", q, k_cache, v_cache, block_table, seq_lens, parents)
+        if num_kv_splits > 1024:
+            contract.refuse("paged_tree_attn", "num_kv_splits must be at most 1024")
 
     def eager_execute(self, q, k_cache, v_cache, block_table, seq_lens, parents, scale, num_kv_splits):
         if num_kv_splits <= 0:
             num_kv_splits = default_num_tree_splits(block_table.size(1) * k_cache.size(1), q.size(0), q.size(1) * q.size(2) // k_cache.size(2), k_cache.size(2))
-        _require(num_kv_splits <= 1024, "paged_tree_attn: num_kv_splits must be at most 1024")
         dev = launch._dev(q, k_cache, v_cache, block_table, seq_lens, parents)
         out = torch.empty(q.shape, dtype=q.dtype, device=dev)
         return launch._paged_tree_attn(dev, q, k_cache, v_cache, block_table, seq_lens, parents, out, scale, num_kv_splits, None, None)
@@ -679,13 +696,16 @@ class verify_draft(CustomOp):
     signature = "verify_draft(Tensor target_probs, Tensor? draft_probs, Tensor tokens, Tensor parents, Tensor uniforms) -> (Tensor, Tensor, Tensor)"
 
     def select(self, sel: KernelSelection):
-        tp, tok, par, u = (sel.arg_tensor(i) for i in (0, 2, 3, 4))
-        dp = sel.arg_optional_tensor(1)
-        contract.check_verify_draft("verify_draft", tp.t, dp.v if dp is not None else None, tok.t, par.t, u.t)
+        tp = [sel.arg_tensor(i) for i in (0, 2, 3, 4)][0]
+        sel.arg_optional_tensor(1)
+        self.check(*sel.args)
         S, N, _ = tp.t.shape
         sel.return_new_tensor([S, N], torch.int32)
         sel.return_new_tensor([S], torch.int32)
         sel.return_new_tensor([S], torch.int32)
+
+    def check(self, target_probs, draft_probs, tokens, parents, uniforms):
+        contract.check_verify_draft("verify_draft", target_probs, draft_probs, tokens, parents, uniforms)
 
     def eager_execute(self, target_probs, draft_probs, tokens, parents, uniforms):
         dev = launch._dev(target_probs, tokens, parents, uniforms, *([draft_probs] if draft_probs is not None else []))
