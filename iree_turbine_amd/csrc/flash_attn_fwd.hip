@@ -582,12 +582,17 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
 
 
 // Packed sequences of different lengths (the VARLEN form of fa_fwd_d128_m16): the queries of sequence s are the rows
-// [cu_q[s], cu_q[s + 1]) of one token stream, its keys and values the rows [cu_k[s], cu_k[s + 1]) of another.
+// [cu_q[s], cu_q[s + 1]) of one token stream, its keys and values the rows [cu_k[s], cu_k[s + 1]) of another.  The query heads that
+// share a K/V head are packed: query row r of a (sequence, K/V head) is token r / group, head r % group, so that a block of
+// 128 rows spans 128 / group tokens -- short sequences fill their blocks (a one-token sequence is one workgroup per K/V
+// head) and less of a block's last tile is masked.
 struct FaVarlen {
   const int *cu_q, *cu_k;  // [num_seqs + 1]
   int num_seqs, total_q, total_k;
+  int group_shift;         // log2(group), -1 if the group is no power of two
   int zero_rest;           // also write zeros to the query rows in front of the first and behind the last sequence
   int pairs;               // (causal) a unit is a pair of query blocks, else one block
+  int ranked;              // hand out the units of the sequence with the most keys first (up to 64 sequences)
 };
 
 // Rows [begin, begin + len) of sequence s; offsets outside the stream are cut to it, a negative length counts as 0.
@@ -599,54 +604,52 @@ __device__ __forceinline__ int fa_seq_range(const int* cu, int s, int total, int
   return e - b;
 }
 
-// The sequence whose units hold place `loc` when every unit takes `per_unit` places (its heads), and the place inside the
-// sequence's; -1 behind the last.  Sequences come in order of falling key length as far as one wave can rank them
-// (64), so that short ones make up the tail of the grid; more than 64 come as they are.  `block_rows` query rows make a block,
-// one or two blocks a unit.  Every wave finds the place by itself, one sequence per lane.
-__device__ __forceinline__ int fa_find_unit(const FaVarlen& vl, int block_rows, int per_unit, int loc, int& inside, int& units) {
-  const int lane = threadIdx.x & 63;
-  auto units_of = [&](int s, int& key) {
-    int begin;
-    const int blocks = (fa_seq_range(vl.cu_q, s, vl.total_q, begin) + block_rows - 1) / block_rows;
-    key = fa_seq_range(vl.cu_k, s, vl.total_k, begin);
-    return vl.pairs ? (blocks + 1) >> 1 : blocks;
-  };
+// A unit's place: what the workgroup with place `loc` works on when every unit takes `per_unit` places (K/V heads).
+struct FaUnit {
+  int q_first, q_len, k_first, k_len;  // the sequence's rows
+  int inside, units;                   // place among the sequence's, and how many units those are per K/V head
+};
+
+// Finds it; false behind the last unit.  Every wave by itself, one sequence per lane and 64 at a time: in order of falling
+// key length (ranked), so that short sequences make up the tail of the grid, or as they come.
+__device__ __forceinline__ bool fa_find_unit(const FaVarlen& vl, int group, int block_rows, int per_unit, int loc, FaUnit& u) {
+  const int lane = threadIdx.x & 63, at = loc / per_unit;
   int base = 0;
-  if (vl.num_seqs <= 64) {
-    int key = -1, n = 0, before = 0;
-    if (lane < vl.num_seqs) n = units_of(lane, key);
-    for (int j = 0; j < vl.num_seqs; j++) {
-      const int kj = __builtin_amdgcn_readlane(key, j), nj = __builtin_amdgcn_readlane(n, j);
-      before += (kj > key || (kj == key && j < lane)) ? nj : 0;
-    }
-    const int at = loc / per_unit;
-    const unsigned long long hit = __builtin_amdgcn_ballot_w64(before <= at && at < before + n);
-    if (!hit) return -1;
-    const int l = __builtin_ctzll(hit);
-    inside = loc - __builtin_amdgcn_readlane(before, l) * per_unit;
-    units = __builtin_amdgcn_readlane(n, l);
-    return l;
-  }
-  const int at = loc / per_unit;
   for (int s0 = 0; s0 < vl.num_seqs; s0 += 64) {
-    int key, n = 0;
-    if (s0 + lane < vl.num_seqs) n = units_of(s0 + lane, key);
-    int incl = n;
+    int qf = 0, ql = 0, kf = 0, kl = -1, n = 0, before = 0;
+    if (s0 + lane < vl.num_seqs) {
+      ql = fa_seq_range(vl.cu_q, s0 + lane, vl.total_q, qf);
+      kl = fa_seq_range(vl.cu_k, s0 + lane, vl.total_k, kf);
+      n = (ql * group + block_rows - 1) / block_rows;
+      if (vl.pairs) n = (n + 1) >> 1;
+    }
+    if (vl.ranked) {
+#pragma unroll 4
+      for (int j = 0; j < vl.num_seqs; j++) {
+        const int kj = __builtin_amdgcn_readlane(kl, j), nj = __builtin_amdgcn_readlane(n, j);
+        before += (kj > kl || (kj == kl && j < lane)) ? nj : 0;
+      }
+    } else {
+      int incl = n;
 #pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-      const int up = __shfl_up(incl, d);
-      if (lane >= d) incl += up;
+      for (int d = 1; d < 64; d <<= 1) {
+        const int up = __shfl_up(incl, d);
+        if (lane >= d) incl += up;
+      }
+      before = base + incl - n;
+      base += __builtin_amdgcn_readlane(incl, 63);
     }
-    const unsigned long long past = __builtin_amdgcn_ballot_w64(base + incl > at);
-    if (past) {
-      const int l = __builtin_ctzll(past);
-      units = __builtin_amdgcn_readlane(n, l);
-      inside = loc - (base + __builtin_amdgcn_readlane(incl, l) - units) * per_unit;
-      return s0 + l;
+    const unsigned long long hit = __builtin_amdgcn_ballot_w64(before <= at && at < before + n);
+    if (hit) {
+      const int l = __builtin_ctzll(hit);
+      u.q_first = __builtin_amdgcn_readlane(qf, l), u.q_len = __builtin_amdgcn_readlane(ql, l);
+      u.k_first = __builtin_amdgcn_readlane(kf, l), u.k_len = __builtin_amdgcn_readlane(kl, l);
+      u.units = __builtin_amdgcn_readlane(n, l);
+      u.inside = loc - __builtin_amdgcn_readlane(before, l) * per_unit;
+      return true;
     }
-    base += __builtin_amdgcn_readlane(incl, 63);
   }
-  return -1;
+  return false;
 }
 
 // Drafted token trees over a paged cache (the TREE form of fa_fwd_d128_m16): the query rows of a (sequence, kv head) are all its
@@ -702,6 +705,7 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
   int units = CAUSAL ? (q_blocks + 1) / 2 : q_blocks;
   int bh, unit, b_idx, h_idx;
   size_t q_first = 0, k_first = 0;  // (VARLEN) the sequence's first rows
+  int seq_q = 0;                    // (VARLEN) its query tokens; Sq counts rows
   int split = 0, first_tile = 0;    // (TREE) the chunk of the keys, and where it begins
   if constexpr (VARLEN) {
     const int pid = blockIdx.x;
@@ -717,24 +721,19 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
         *reinterpret_cast<half8*>(row + q16 * 8) = half8{};
       }
     }
-    // The heads that share a K/V head sit on one XCD when the K/V heads divide over the eight; a sequence's heads follow
-    // each other, a head's units too.
-    const bool spread = (lay.H / lay.group) % 8 == 0;
-    const int xcd = pid & 7, per_unit = spread ? lay.H / 8 : lay.H;
-    int inside;
-    const int seq = fa_find_unit(pg, BLOCK_M, per_unit, spread ? pid >> 3 : pid, inside, units);
-    if (seq < 0) return;
-    h_idx = inside / units;
-    unit = inside - h_idx * units;
-    if (spread) {
-      const int kv = h_idx / lay.group;
-      h_idx = (kv * 8 + xcd) * lay.group + (h_idx - kv * lay.group);
-    }
-    int row;
-    Sq = fa_seq_range(pg.cu_q, seq, pg.total_q, row);
-    q_first = row;
-    Sk = fa_seq_range(pg.cu_k, seq, pg.total_k, row);
-    k_first = row;
+    // A K/V head's units sit on one XCD when the K/V heads divide over the eight.
+    const int kv_heads = lay.H / lay.group;
+    const bool spread = kv_heads % 8 == 0;
+    FaUnit u;
+    if (!fa_find_unit(pg, lay.group, BLOCK_M, spread ? kv_heads / 8 : kv_heads, spread ? pid >> 3 : pid, u)) return;
+    units = u.units;
+    const int kv = u.inside / units;
+    unit = u.inside - kv * units;
+    h_idx = (spread ? kv * 8 + (pid & 7) : kv) * lay.group;
+    q_first = u.q_first, k_first = u.k_first;
+    Sq = u.q_len * lay.group;
+    Sk = u.k_len;
+    seq_q = u.q_len;
     q_blocks = (Sq + BLOCK_M - 1) / BLOCK_M;
     bh = b_idx = 0;
   } else if constexpr (TREE) {
@@ -806,16 +805,21 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
     if (threadIdx.x < BLOCK_M) seen[threadIdx.x] = mine;
     __syncthreads();
   }
-  // where query row r lies behind Qb (and Ob), in elements
-  auto row_at = [&](int r, unsigned pitch) -> size_t {
-    if constexpr (TREE) {
-      const int node = r / lay.group;
-      return (size_t)node * pitch + (r - node * lay.group) * 128;
+  // (VARLEN, TREE) the token, or node, of a packed query row, and where the row lies behind Qb (and Ob), in elements
+  auto token_of = [&](int r) -> int {
+    if constexpr (VARLEN) return pg.group_shift >= 0 ? r >> pg.group_shift : r / lay.group;
+    else if constexpr (TREE) return r / lay.group;
+    else return r;
+  };
+  auto row_at = [&](int r, unsigned pitch, int64_t head_pitch) -> size_t {
+    if constexpr (VARLEN || TREE) {
+      const int tok = token_of(r);
+      return (size_t)tok * pitch + (size_t)(r - tok * lay.group) * head_pitch;
     } else {
       return (size_t)r * pitch;
     }
   };
-  const int causal_off = Sk - Sq;
+  const int causal_off = Sk - (VARLEN ? seq_q : Sq);
   const half_t* Qb = Q + (VARLEN ? q_first * lay.q_r : b_idx * lay.q_b) + h_idx * lay.q_h;
   const half_t* Kb = K + (PAGED ? 0 : VARLEN ? k_first * lay.k_r : b_idx * lay.k_b) + hk_idx * lay.k_h;
   const half_t* Vb = V + (PAGED ? 0 : VARLEN ? k_first * lay.v_r : b_idx * lay.v_b) + hk_idx * lay.v_h;
@@ -847,12 +851,13 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
   if (CAUSAL && pass == 1 && 2 * unit == q_blocks - 1) break;
   const int q0 = qb * BLOCK_M;
   const int wq0 = q0 + wave * WAVE_M;
+  const int wave_first = token_of(wq0), wave_last = token_of(wq0 + WAVE_M - 1);  // the wave's tokens
 
   int k_end = Sk;
   if (CAUSAL) {
     int last_q = q0 + BLOCK_M - 1;
     if (last_q > Sq - 1) last_q = Sq - 1;
-    int lim = last_q + causal_off + 1;
+    int lim = token_of(last_q) + causal_off + 1;
     if (lim < k_end) k_end = lim;
   }
   int n_tiles = k_end > 0 ? (k_end + FA_BLOCK_N - 1) / FA_BLOCK_N : 0;
@@ -869,7 +874,7 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
 #pragma unroll
     for (int ks = 0; ks < 4; ks++) {
       if (q_row < Sq) {
-        const half8 raw = *reinterpret_cast<const half8*>(Qb + row_at(q_row, lay.q_r) + ks * 32 + g * 8);
+        const half8 raw = *reinterpret_cast<const half8*>(Qb + row_at(q_row, lay.q_r, lay.q_h) + ks * 32 + g * 8);
         if constexpr (EXACT) {
           qf[qg][ks] = raw;
         } else {
@@ -948,7 +953,7 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
 
   auto wave_active = [&](int tile) {
     if constexpr (TREE) return wq0 < Sq;  // a wave without rows only loads
-    else return !CAUSAL || (tile * FA_BLOCK_N <= wq0 + 31 + causal_off);
+    else return !CAUSAL || (tile * FA_BLOCK_N <= wave_last + causal_off);
   };
   auto kread = [&](int f, int koff) {  // K fragment f = kg * 4 + ks of the slot at koff
 #if defined(MI355_ABLATE_NO_K_READS)
@@ -990,12 +995,13 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
           }
         }
       } else {
-      const bool need_mask = (CAUSAL && (key0 + FA_BLOCK_N - 1 > wq0 + causal_off)) || (key0 + FA_BLOCK_N > Sk);
+      const bool need_mask = (CAUSAL && (key0 + FA_BLOCK_N - 1 > wave_first + causal_off)) || (key0 + FA_BLOCK_N > Sk);
       if (need_mask) {
 #pragma unroll
         for (int qg = 0; qg < QG; qg++) {
           const int q_row = wq0 + qg * 16 + q16;
-          const int lim = CAUSAL ? (q_row + causal_off < Sk - 1 ? q_row + causal_off : Sk - 1) : Sk - 1;  // last visible key
+          const int q_tok = token_of(q_row);
+          const int lim = CAUSAL ? (q_tok + causal_off < Sk - 1 ? q_tok + causal_off : Sk - 1) : Sk - 1;  // last visible key
           const int rel = lim - key0 - 4 * g;
 #pragma unroll
           for (int kg = 0; kg < 4; kg++)
@@ -1252,7 +1258,7 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
     for (int it = 0; it < WAVE_M / 4; it++) {
       const int row = it * 4 + er;
       const half8 v = *reinterpret_cast<const half8*>(ep + row * 256 + ((ec ^ (row & 15)) * 16));
-      if (wq0 + row < Sq) *reinterpret_cast<half8*>(Ob + row_at(wq0 + row, lay.o_r) + ec * 8) = v;
+      if (wq0 + row < Sq) *reinterpret_cast<half8*>(Ob + row_at(wq0 + row, lay.o_r, lay.o_h) + ec * 8) = v;
     }
     if (CAUSAL) __syncthreads();  // the next pass loads K / V tiles over these regions
   }
@@ -1960,19 +1966,26 @@ static int fa_varlen(const void* q, const void* k, const void* v, void* o, const
   lay.v_h = v_strides[1], lay.v_r = (unsigned)v_strides[0];
   lay.o_h = o_strides[1], lay.o_r = (unsigned)o_strides[0];
   lay.H = (int)H, lay.group = (int)(H / Hkv);
+  const int64_t group = H / Hkv, rows = total_q * group;
+  if (rows >= (1ll << 31)) return fail(-MI355_E_SHAPE, "%s: too many query rows per key/value head", who);
+  int group_shift = -1;
+  for (int sh = 0; sh < 16; sh++)
+    if (group == (1ll << sh)) group_shift = sh;
   // With the mask, a pair of blocks (the i-th from the end and the i-th from the start) is the same work everywhere in a sequence,
   // and half as many workgroups; where even single blocks would not fill the chip twice (512 workgroups are resident), they
   // are handed out singly.
-  const int pairs = is_causal && total_q / FA_BLOCK_M * H >= 2048;
-  const FaVarlen vl{cu_q, cu_k, (int)num_seqs, (int)total_q, (int)total_k, zero_rest, pairs};
-  // the lengths are known on the device only: as many units as num_seqs sequences of total_q rows can have
-  const int64_t units = total_q / (FA_BLOCK_M << pairs) + num_seqs;
-  if (units * H >= (1ll << 31)) return fail(-MI355_E_SHAPE, "%s: too many query blocks", who);
+  const int pairs = is_causal && rows / FA_BLOCK_M * Hkv >= 2048;
+  // Ranking costs every workgroup some 20 ns per sequence: worth it where sequences are long or few.
+  const int ranked = num_seqs > 1 && num_seqs <= 64 && total_k / num_seqs >= 16 * num_seqs;
+  const FaVarlen vl{cu_q, cu_k, (int)num_seqs, (int)total_q, (int)total_k, group_shift, zero_rest, pairs, ranked};
+  // the lengths are known on the device only: as many units as num_seqs sequences of total_q tokens can have
+  const int64_t units = rows / (FA_BLOCK_M << pairs) + num_seqs;
+  if (units * Hkv >= (1ll << 31)) return fail(-MI355_E_SHAPE, "%s: too many query blocks", who);
   auto kern = is_causal ? fa_fwd_d128_m16<true, BF, 4, false, FaForm::VARLEN> : fa_fwd_d128_m16<false, BF, 4, false, FaForm::VARLEN>;
   const int lds_bytes = 2 * FA_STAGE;
   static std::atomic<uint64_t> lds_ok[2] = {};
   if (int rc = allow_lds(reinterpret_cast<const void*>(kern), lds_bytes, lds_ok[is_causal ? 1 : 0], "fa_fwd_d128_m16<varlen>")) return rc;
-  dim3 grid((unsigned)(units * H)), block(256);
+  dim3 grid((unsigned)(units * Hkv)), block(256);
   hipLaunchKernelGGL(kern, grid, block, lds_bytes, reinterpret_cast<hipStream_t>(stream), (const half_t*)q, (const half_t*)k,
                      (const half_t*)v, (half_t*)o, (int)H, 0, 0, scale * 1.4426950408889634f, 0, lay, vl);
   return check_launch("fa_fwd_d128_m16<varlen>", grid, block, lds_bytes);
