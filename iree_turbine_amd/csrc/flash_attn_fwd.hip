@@ -683,7 +683,7 @@ using FaFormArgs = std::conditional_t<F == FaForm::VARLEN, FaVarlen, std::condit
 // the score MFMAs (vector work behind 48 of the trip's 64 MFMAs instead of 32).  Measured on 2 x 32 x 4096: ahead with
 // eight waves (unmasked 475 against 484 us), behind with four (causal 268 against 263); each form is built the way it
 // runs faster.
-// QG: groups of 16 query rows per wave, 2 but for tree calls of at most 64 rows.
+// QG: groups of 16 query rows per wave, 2 but for packed and tree calls with few rows.
 template <bool CAUSAL, bool BF, int NW, bool SPREAD, FaForm FORM = FaForm::PLAIN, int QG = 2>
 __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2))) void fa_fwd_d128_m16(
     const half_t* __restrict__ Q, const half_t* __restrict__ K, const half_t* __restrict__ V, half_t* __restrict__ O, int BH,
@@ -1974,17 +1974,23 @@ static int fa_varlen(const void* q, const void* k, const void* v, void* o, const
   // With the mask, a pair of blocks (the i-th from the end and the i-th from the start) is the same work everywhere in a sequence,
   // and half as many workgroups; where even single blocks would not fill the chip twice (512 workgroups are resident), they
   // are handed out singly.
-  const int pairs = is_causal && rows / FA_BLOCK_M * Hkv >= 2048;
+  const int64_t blocks = rows / FA_BLOCK_M * Hkv;
+  const int pairs = is_causal && blocks >= 2048;
+  // Blocks of 64 rows where those of 128 would not fill the chip: twice the workgroups, each with half the work per key tile.
+  // One prompt of 1024 tokens (32 query heads over 8) 23 against 29 us, 32 of 16 tokens 8.0 against 9.7; where the chip
+  // is full the 64-row blocks are bound by LDS reads: 8 prompts of 256 tokens 22 against 20, one of 4096 164 against 134.
+  const int qg = blocks < 512 ? 1 : 2, block_m = 64 * qg;
   // Ranking costs every workgroup some 20 ns per sequence: worth it where sequences are long or few.
   const int ranked = num_seqs > 1 && num_seqs <= 64 && total_k / num_seqs >= 16 * num_seqs;
   const FaVarlen vl{cu_q, cu_k, (int)num_seqs, (int)total_q, (int)total_k, group_shift, zero_rest, pairs, ranked};
   // the lengths are known on the device only: as many units as num_seqs sequences of total_q tokens can have
-  const int64_t units = rows / (FA_BLOCK_M << pairs) + num_seqs;
+  const int64_t units = rows / (block_m << pairs) + num_seqs;
   if (units * Hkv >= (1ll << 31)) return fail(-MI355_E_SHAPE, "%s: too many query blocks", who);
-  auto kern = is_causal ? fa_fwd_d128_m16<true, BF, 4, false, FaForm::VARLEN> : fa_fwd_d128_m16<false, BF, 4, false, FaForm::VARLEN>;
+  auto kern = qg == 1 ? (is_causal ? fa_fwd_d128_m16<true, BF, 4, false, FaForm::VARLEN, 1> : fa_fwd_d128_m16<false, BF, 4, false, FaForm::VARLEN, 1>)
+                      : (is_causal ? fa_fwd_d128_m16<true, BF, 4, false, FaForm::VARLEN, 2> : fa_fwd_d128_m16<false, BF, 4, false, FaForm::VARLEN, 2>);
   const int lds_bytes = 2 * FA_STAGE;
-  static std::atomic<uint64_t> lds_ok[2] = {};
-  if (int rc = allow_lds(reinterpret_cast<const void*>(kern), lds_bytes, lds_ok[is_causal ? 1 : 0], "fa_fwd_d128_m16<varlen>")) return rc;
+  static std::atomic<uint64_t> lds_ok[4] = {};
+  if (int rc = allow_lds(reinterpret_cast<const void*>(kern), lds_bytes, lds_ok[(is_causal ? 1 : 0) + 2 * (qg - 1)], "fa_fwd_d128_m16<varlen>")) return rc;
   dim3 grid((unsigned)(units * Hkv)), block(256);
   hipLaunchKernelGGL(kern, grid, block, lds_bytes, reinterpret_cast<hipStream_t>(stream), (const half_t*)q, (const half_t*)k,
                      (const half_t*)v, (half_t*)o, (int)H, 0, 0, scale * 1.4426950408889634f, 0, lay, vl);
