@@ -173,7 +173,7 @@ int mi355_flash_attn_fwd_strided_bf16(const void* q, const void* k, const void* 
  * and a sequence that ends before it begins is empty, so no contents make the kernel leave its operands.  Lengths are
  * read on the device only: nothing has to be known on the host, and a captured launch serves any lengths.
  * Rows of o outside every sequence are left as they are; with zero_rest != 0 those in front of the first and behind
- * the last sequence are set to zero.  total_q, total_k <= 2^24, num_seqs <= 65535.
+ * the last sequence are set to zero.  total_q, total_k <= 2^24, total_q * H / Hkv <= 2^30, num_seqs <= 65535.
  * A weight of zero times a non-finite V row of the same sequence is NaN, as in the formula.
  * Replaces: the SDPA root of mi355_flash_attn_fwd for a ragged batch, which the reference can only pad
  * (tests/dynamo/llama_test.py:285-290 builds one rectangular mask).
@@ -366,11 +366,13 @@ int mi355_paged_prefill_attn_bf16(const void* q, const void* k_cache, const void
  * seq_lens:    [num_seqs] int32, cut to [0, max_pages_per_seq * page_size]; shorter than num_nodes: the first nodes are not
  *              in the cache and nobody sees them
  * parents:     [num_seqs, num_nodes] int32; a value outside [0, n) for node n: it has no ancestors (a root)
- * A query that sees nothing gives zeros.  1 <= num_nodes <= 64, num_q_heads / num_kv_heads <= 128, D == 128, page_size 16, 32, 64,
+ * A query that sees nothing gives zeros.  The V rows of all drafts have to hold numbers, also of branches that a query does
+ * not see (a weight of zero times a non-finite value is NaN): a sequence with fewer drafts than num_nodes writes its
+ * padding too.  1 <= num_nodes <= 64, num_q_heads / num_kv_heads <= 128, D == 128, page_size 16, 32, 64,
  * 128 or 256, 1 <= num_splits <= 1024.  A chain (parents[n] = n - 1) is the causal mask among the drafts.
  * num_splits cuts the table's reach into that many chunks, each by its own workgroups; num_splits > 1 needs
  * part_acc [num_seqs, num_nodes, num_q_heads, num_splits, D] and part_ml [.., num_splits, 2], fp32, written before they are
- * read in the same call.  No counterpart in the reference; the mask generalises tests/dynamo/llama_test.py:285-290.
+ * read in the same call, and at most 2^23 query rows (num_seqs * num_nodes * num_q_heads).  No counterpart in the reference; the mask generalises tests/dynamo/llama_test.py:285-290.
  */
 int mi355_paged_tree_attn(const void* q, const void* k_cache, const void* v_cache,
                           const int32_t* block_table, const int32_t* seq_lens, const int32_t* parents, void* out,
@@ -429,7 +431,7 @@ int mi355_paged_batch_layout(int32_t* block_table, const int32_t* context_lens, 
  * x, out: [tokens, heads, D] of dtype (MI355_F16 | MI355_BF16 | MI355_F32); *_strides {token, head} in elements, the D elements
  * of a row contiguous; in place (out == x, same strides) is allowed.  positions: int32 [tokens].  inv_freq: fp64
  * (freq_is_f64 != 0) or fp32 [rotary_dim / 2].  Angles are formed in 64 bits, the products in 32, rounded once.
- * rotary_dim even, <= D and <= 1024.  Rows on 16-byte borders with rotary_dim / 2 and D - rotary_dim multiples of 16
+ * rotary_dim even, <= D and <= 1024; fewer than 2^24 tokens.  Rows on 16-byte borders with rotary_dim / 2 and D - rotary_dim multiples of 16
  * bytes' elements run with wide loads; others element by element.
  * No counterpart among the reference's kernels.
  */
@@ -441,8 +443,8 @@ int mi355_rope(const void* x, void* out, const int32_t* positions, const void* i
 /*
  * The serving form: q rotated into q_out [tokens, num_q_heads, 128] (contiguous), k_new rotated and v_new as it is into the
  * rows slots[token] of k_cache / v_cache ([num_slots, num_kv_heads, 128]: the caches' pages and places flattened).
- * A slot outside [0, num_slots): the token's key and value go nowhere.  Slots must differ from each other (of two
- * tokens with one slot, either may be found there).  q, k_new, v_new: [tokens, heads, 128] with {token, head} strides;
+ * A slot outside [0, num_slots): the token's key and value go nowhere.  The others must differ from each other (what a slot
+ * that is given twice holds is not defined); fewer than 2^24 tokens.  q, k_new, v_new: [tokens, heads, 128] with {token, head} strides;
  * dtype MI355_F16 | MI355_BF16.  Slots as mi355_paged_batch_layout gives them.
  * Replaces: the cache update of tests/dynamo/llama_test.py:160-167 with the rotation in front of it.
  */

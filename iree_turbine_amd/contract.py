@@ -186,8 +186,8 @@ def check_varlen_attention(op: str, q: Tensor, k: Tensor, v: Tensor, cu_q: Tenso
         refuse(op, "k and v shapes differ")
     if hkv == 0 or h == 0 or h % hkv or h > 65535:
         refuse(op, f"{h} query heads over {hkv} key/value heads")
-    if not (0 < tq <= 1 << 24 and 0 < tk <= 1 << 24):
-        refuse(op, f"q and k need 1 to 2^24 rows, got {tq} and {tk}")
+    if not (0 < tq <= 1 << 24 and 0 < tk <= 1 << 24 and tq * (h // hkv) <= 1 << 30):
+        refuse(op, f"q and k need 1 to 2^24 rows (q times the query heads of a key head 2^30), got {tq} and {tk}")
     if cu_q.dim() != 1 or not 2 <= cu_q.size(0) <= 65536:
         refuse(op, "cu_seqlens_q must be int32 [num_seqs + 1] with 1 to 65535 sequences")
     _check_int32(op, "cu_seqlens_q", cu_q, cu_q.size(0))
@@ -253,7 +253,7 @@ def check_rope(op: str, x: Tensor, positions: Tensor, inv_freq: Tensor) -> None:
     if x.dim() != 3 or x.dtype not in ROPE_DTYPES:
         refuse(op, f"x must be [tokens, heads, D] in float16, bfloat16 or float32, got {x.dtype} {tuple(x.shape)}")
     T, H, D = x.shape
-    if not (T > 0 and 0 < H <= 65535 and 0 < D <= 65536 and H * D <= 1 << 30):
+    if not (0 < T < 1 << 24 and 0 < H <= 65535 and 0 < D <= 65536 and H * D <= 1 << 30):
         refuse(op, f"bad size {tuple(x.shape)}")
     check_rope_angles(op, positions, inv_freq, T, D)
 
@@ -279,8 +279,8 @@ def check_rope_append(op: str, q: Tensor, k_new: Tensor, v_new: Tensor, position
         refuse(op, f"head dim must be 128, got {D} and {Dk}")
     if not (0 < hq <= 65535 and 0 < hkv <= 65535):
         refuse(op, f"bad head counts {hq} and {hkv}")
-    if T == 0 or Tk != T:
-        refuse(op, f"empty or unequal tokens ({T} and {Tk})")
+    if not 0 < T < 1 << 24 or Tk != T:
+        refuse(op, f"no, too many or unequal tokens ({T} and {Tk})")
     if hkv != k_cache.size(2):
         refuse(op, "k_new and k_cache disagree on the number of kv heads")
     if not (k_cache.is_contiguous() and v_cache.is_contiguous()):

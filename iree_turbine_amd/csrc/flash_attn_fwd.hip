@@ -1921,7 +1921,7 @@ static int fa_tree_launch(const TreeArgs& a, int num_seqs, hipStream_t stream) {
   tr.num_seqs = num_seqs, tr.num_splits = a.num_splits, tr.chunk_tiles = a.chunk_steps / 2;
   tr.row_blocks = (a.nodes * a.group + block_m - 1) / block_m;
   const int64_t wgs = (int64_t)num_seqs * a.num_splits * a.num_kv_heads * tr.row_blocks;
-  if (wgs >= (1ll << 31)) return fail(-MI355_E_SHAPE, "paged_tree_attn: too many workgroups");
+  if (wgs >= (1ll << 24)) return fail(-MI355_E_SHAPE, "paged_tree_attn: too many workgroups");  // 2^32 threads
   dim3 grid((unsigned)wgs), block(256);
   hipLaunchKernelGGL(kern, grid, block, lds_bytes, stream, a.q, a.kc, a.vc, a.out, 0, 0, 0, a.scale_log2e, 0, lay, tr);
   return check_launch("fa_fwd_d128_m16<tree>", grid, block, lds_bytes);
@@ -1967,7 +1967,7 @@ static int fa_varlen(const void* q, const void* k, const void* v, void* o, const
   lay.o_h = o_strides[1], lay.o_r = (unsigned)o_strides[0];
   lay.H = (int)H, lay.group = (int)(H / Hkv);
   const int64_t group = H / Hkv, rows = total_q * group;
-  if (rows >= (1ll << 31)) return fail(-MI355_E_SHAPE, "%s: too many query rows per key/value head", who);
+  if (rows > (1ll << 30)) return fail(-MI355_E_SHAPE, "%s: %lld query rows per key/value head, at most 2^30", who, (long long)rows);
   int group_shift = -1;
   for (int sh = 0; sh < 16; sh++)
     if (group == (1ll << sh)) group_shift = sh;
@@ -1985,7 +1985,7 @@ static int fa_varlen(const void* q, const void* k, const void* v, void* o, const
   const FaVarlen vl{cu_q, cu_k, (int)num_seqs, (int)total_q, (int)total_k, group_shift, zero_rest, pairs, ranked};
   // the lengths are known on the device only: as many units as num_seqs sequences of total_q tokens can have
   const int64_t units = rows / (block_m << pairs) + num_seqs;
-  if (units * Hkv >= (1ll << 31)) return fail(-MI355_E_SHAPE, "%s: too many query blocks", who);
+  if (units * Hkv >= (1ll << 24)) return fail(-MI355_E_SHAPE, "%s: too many query blocks", who);  // 2^32 threads
   auto kern = qg == 1 ? (is_causal ? fa_fwd_d128_m16<true, BF, 4, false, FaForm::VARLEN, 1> : fa_fwd_d128_m16<false, BF, 4, false, FaForm::VARLEN, 1>)
                       : (is_causal ? fa_fwd_d128_m16<true, BF, 4, false, FaForm::VARLEN, 2> : fa_fwd_d128_m16<false, BF, 4, false, FaForm::VARLEN, 2>);
   const int lds_bytes = 2 * FA_STAGE;

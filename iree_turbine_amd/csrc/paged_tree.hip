@@ -315,7 +315,9 @@ static int launch_tree(const TreeArgs& a, int num_seqs, hipStream_t stream) {
   static_assert(lds_bytes >= (int)((2 * PT_WAVES * 16 + PT_WAVES * 16 * 128) * sizeof(float)), "merge area must fit");
   static std::atomic<uint64_t> lds_ok{0};
   if (int rc = allow_lds(reinterpret_cast<const void*>(kern), lds_bytes, lds_ok, "paged_tree_kernel")) return rc;
-  dim3 grid((unsigned)((int64_t)num_seqs * a.num_splits * a.num_kv_heads)), block(PT_WAVES * 64);
+  const int64_t wgs = (int64_t)num_seqs * a.num_splits * a.num_kv_heads;
+  if (wgs >= (1ll << 24)) return fail(-MI355_E_SHAPE, "paged_tree_attn: too many workgroups");  // 2^32 threads
+  dim3 grid((unsigned)wgs), block(PT_WAVES * 64);
   hipLaunchKernelGGL(kern, grid, block, lds_bytes, stream, a);
   return check_launch("paged_tree_kernel", grid, block, lds_bytes);
 }
@@ -353,7 +355,7 @@ extern "C" int mi355_paged_tree_attn(const void* q, const void* k_cache, const v
     return fail(-MI355_E_SHAPE, "%s: %lld nodes per sequence, supported: 1 to %d", fn, (long long)num_nodes, TREE_MAX_NODES);
   if (num_seqs <= 0 || num_seqs > 65535 || num_q_heads <= 0 || num_kv_heads <= 0 || num_kv_heads > 65535 || num_q_heads > 65535 ||
       max_pages_per_seq <= 0 || max_pages_per_seq > (1 << 22) || num_pages <= 0 || num_pages > (1 << 26) ||
-      num_seqs * num_nodes * num_q_heads > (1ll << 30) || max_pages_per_seq * page_size > (1ll << 30))
+      num_seqs * num_nodes * num_q_heads > (num_splits > 1 ? 1ll << 23 : 1ll << 30) || max_pages_per_seq * page_size > (1ll << 30))
     return fail(-MI355_E_SHAPE, "%s: bad sizes seqs=%lld nodes=%lld hq=%lld hkv=%lld max_pages=%lld num_pages=%lld", fn,
                 (long long)num_seqs, (long long)num_nodes, (long long)num_q_heads, (long long)num_kv_heads,
                 (long long)max_pages_per_seq, (long long)num_pages);

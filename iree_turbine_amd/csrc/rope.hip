@@ -197,7 +197,7 @@ extern "C" int mi355_rope(const void* x, void* out, const int32_t* positions, co
                           int interleaved, int inverse, float scale, int dtype, void* stream) {
   const char* fn = "rope";
   if (!x || !out || !positions || !inv_freq || !x_strides || !out_strides) return fail(-MI355_E_NULL, "%s: null pointer", fn);
-  if (tokens <= 0 || tokens > 0x7fffffffll || heads <= 0 || heads > 65535 || D <= 0 || D > 65536 || rotary_dim <= 0 || rotary_dim > D ||
+  if (tokens <= 0 || tokens >= (1ll << 24) || heads <= 0 || heads > 65535 || D <= 0 || D > 65536 || rotary_dim <= 0 || rotary_dim > D ||
       rotary_dim % 2 || rotary_dim > 2 * RP_MAX_PAIRS || heads * D > (1ll << 30))
     return fail(-MI355_E_SHAPE, "%s: bad sizes tokens=%lld heads=%lld D=%lld rotary_dim=%lld (even, at most D and %d)", fn,
                 (long long)tokens, (long long)heads, (long long)D, (long long)rotary_dim, 2 * RP_MAX_PAIRS);
@@ -236,7 +236,7 @@ extern "C" int mi355_rope_kv_append(const void* q, const void* k_new, const void
       !v_strides)
     return fail(-MI355_E_NULL, "%s: null pointer", fn);
   if (D != 128) return fail(-MI355_E_SHAPE, "%s: head dim %lld not supported (only 128)", fn, (long long)D);
-  if (tokens <= 0 || tokens > 0x7fffffffll || num_q_heads <= 0 || num_kv_heads <= 0 || num_q_heads > 65535 || num_kv_heads > 65535 ||
+  if (tokens <= 0 || tokens >= (1ll << 24) || num_q_heads <= 0 || num_kv_heads <= 0 || num_q_heads > 65535 || num_kv_heads > 65535 ||
       rotary_dim <= 0 || rotary_dim > D || rotary_dim % 2 || num_slots <= 0 || num_slots > (1ll << 34))
     return fail(-MI355_E_SHAPE, "%s: bad sizes tokens=%lld hq=%lld hkv=%lld rotary_dim=%lld slots=%lld", fn, (long long)tokens,
                 (long long)num_q_heads, (long long)num_kv_heads, (long long)rotary_dim, (long long)num_slots);

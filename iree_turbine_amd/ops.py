@@ -593,7 +593,7 @@ class rope_kv_append(CustomOp):
     """One pass over a step's projections: q [T, Hq, 128] rotated (the result), k_new [T, Hkv, 128] rotated and v_new as it is into
     the rows `slots` int64 [T] of k_cache, v_cache [P, page, Hkv, 128] (page * page_size + place, as paged_batch_layout gives
     them; -1 or anything outside the cache: that token is not stored).  q, k_new, v_new may be slices of a packed
-    projection.  Slots must differ.  Angles, layouts and `scale` as in `rope`."""
+    projection.  Slots inside the cache must differ.  Angles, layouts and `scale` as in `rope`."""
 
     signature = "rope_kv_append(Tensor q, Tensor k_new, Tensor v_new, Tensor positions, Tensor inv_freq, Tensor(a!) k_cache, Tensor(b!) v_cache, Tensor slots, bool interleaved, float scale) -> Tensor"
 
@@ -656,7 +656,7 @@ class paged_tree_attn(CustomOp):
     """Attention of drafted token trees over the paged cache: q [S, N, Hq, 128], N <= 64 nodes per sequence, whose K/V are the last N
     tokens of the cache (seq_lens int32 [S] counts them); parents int32 [S, N] (a value outside [0, n) for node n: a root).
     Node n sees every token in front of the drafts, its ancestors and itself; with parents[n] = n - 1 this is
-    paged_prefill_attn of N new tokens.  num_kv_splits <= 0 picks a default from the table width; scale <= 0 selects
+    paged_prefill_attn of N new tokens.  All N positions' V rows have to hold numbers (write padding too).  num_kv_splits <= 0 picks a default from the table width; scale <= 0 selects
     1/sqrt(D).  Returns [S, N, Hq, 128]."""
 
     signature = "paged_tree_attn(Tensor q, Tensor k_cache, Tensor v_cache, Tensor block_table, Tensor seq_lens, Tensor parents, float scale, int num_kv_splits) -> Tensor"
