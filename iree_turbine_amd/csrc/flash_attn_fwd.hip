@@ -938,16 +938,21 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
     }
   };
 
+  // the j-th key tile that this workgroup walks
+  auto tile_at = [&](int j) -> int {
+    if constexpr (TREE) return first_tile + j;
+    else return j;
+  };
   floatx4 oacc[8][QG];  // [d group][query group]
 #pragma unroll
   for (int dg = 0; dg < 8; dg++)
 #pragma unroll
     for (int qg = 0; qg < QG; qg++) oacc[dg][qg] = floatx4{0.f, 0.f, 0.f, 0.f};
   // the negated running maximum of the lane's query in either group, four equal values: the addend of every score chain
-  floatx4 negm[QG];
-  float l_run[QG], grow_thr[QG];
-#pragma unroll
-  for (int qg = 0; qg < QG; qg++) negm[qg] = floatx4{0.f, 0.f, 0.f, 0.f}, l_run[qg] = 0.f, grow_thr[qg] = -INFINITY;
+  floatx4 negm[QG] = {};
+  float l_run[QG] = {};
+  float grow_thr[QG];
+  grow_thr[0] = grow_thr[QG - 1] = -INFINITY;
   const float score_mul = EXACT ? scale_log2e : 1.f;                // score units -> log2 units
   const float kRescaleThreshold = EXACT ? 8.f / scale_log2e : 8.f;  // 2^8, in score units
 
@@ -1169,39 +1174,39 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
     return d;
   };
   if (n_tiles > 0) {
-    load_ids(first_tile, k_ids);
+    load_ids(tile_at(0), k_ids);
     drop0 = drops(k_ids);
-    issue_kv(Kb, k_rb, k_voff, first_tile, 0, k_ids);
-    issue_kv(Vb, v_rb, v_voff, first_tile, VBUF, k_ids);
-    load_ids(first_tile + 1, v_ids);
+    issue_kv(Kb, k_rb, k_voff, tile_at(0), 0, k_ids);
+    issue_kv(Vb, v_rb, v_voff, tile_at(0), VBUF, k_ids);
+    load_ids(tile_at(1), v_ids);
     drop1 = drops(v_ids);
-    if (n_tiles > 1) issue_kv(Kb, k_rb, k_voff, first_tile + 1, TILE_B, v_ids);
-    load_ids(first_tile + 2, k_ids);  // what trip 0 issues: K(2) and V(1)
+    if (n_tiles > 1) issue_kv(Kb, k_rb, k_voff, tile_at(1), TILE_B, v_ids);
+    load_ids(tile_at(2), k_ids);  // what trip 0 issues: K(2) and V(1)
     drop2 = drops(k_ids);
     wait_vmcnt0();
     __syncthreads();
-    if (wave_active(first_tile)) scores(0, sa);
+    if (wave_active(tile_at(0))) scores(0, sa);
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     __syncthreads();
   }
   auto trip = [&](auto par_tag, int j, floatx4 (*s_cur)[QG], floatx4 (*s_next)[QG]) {
     constexpr int PAR = decltype(par_tag)::value;
     constexpr int K_CUR = PAR * TILE_B, K_NEXT = (1 - PAR) * TILE_B, V_CUR = VBUF + PAR * TILE_B, V_NEXT = VBUF + (1 - PAR) * TILE_B;
-    if (j + 2 < n_tiles) issue_kv(Kb, k_rb, k_voff, first_tile + j + 2, K_CUR, k_ids);
-    if (j + 1 < n_tiles) issue_kv(Vb, v_rb, v_voff, first_tile + j + 1, V_NEXT, v_ids);
+    if (j + 2 < n_tiles) issue_kv(Kb, k_rb, k_voff, tile_at(j + 2), K_CUR, k_ids);
+    if (j + 1 < n_tiles) issue_kv(Vb, v_rb, v_voff, tile_at(j + 1), V_NEXT, v_ids);
     const int dropped = drop0;
     if constexpr (PAGED) {
       // the next trip fetches V(j+2) -- the tile whose ids K just used -- and K(j+3)
 #pragma unroll
       for (int i = 0; i < 4; i++) v_ids[i] = k_ids[i];
-      load_ids(first_tile + j + 3, k_ids);
+      load_ids(tile_at(j + 3), k_ids);
       if constexpr (TREE) {
         drop0 = drop1;
         drop1 = drop2;
         drop2 = drops(k_ids);
       }
     }
-    if (wave_active(first_tile + j)) softmax_pv(first_tile + j, dropped, std::integral_constant<int, V_CUR - VBUF>{}, s_cur, K_NEXT, s_next);
+    if (wave_active(tile_at(j))) softmax_pv(tile_at(j), dropped, std::integral_constant<int, V_CUR - VBUF>{}, s_cur, K_NEXT, s_next);
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
 #if !defined(MI355_ABLATE_NO_BARRIERS)
     __syncthreads();
