@@ -17,6 +17,7 @@ namespace mi355 {
 
 constexpr int RP_THREADS = 256;
 constexpr int RP_MAX_PAIRS = 512;  // R / 2
+constexpr int RP_ANGLES = 1024;    // angles per workgroup: its tokens times R / 2
 
 // One operand: where a token's head rows lie, in elements; the D elements of a row are contiguous.
 struct RopeRows {
@@ -25,15 +26,6 @@ struct RopeRows {
   long long src_token, src_head, dst_token, dst_head;
   int heads;
 };
-
-template <typename T>
-__device__ __forceinline__ float rp_load(T v) {
-  return (float)v;
-}
-template <typename T>
-__device__ __forceinline__ T rp_store(float v) {
-  return (T)v;
-}
 
 // (cos, sin) of pos * freq, both times `mul`
 __device__ __forceinline__ floatx2 rp_angle(int pos, double freq, float mul, float sin_mul) {
@@ -44,138 +36,175 @@ __device__ __forceinline__ floatx2 rp_angle(int pos, double freq, float mul, flo
   return floatx2{c * mul, s * sin_mul};
 }
 
-// One work item of a head row: item i < n_pair rotates W pairs, the others copy W elements (halves) or 2 W (interleaved:
-// W pairs are 2 W neighbours).  W = 1: no alignment is assumed.
-template <typename T, bool INTER, int W>
-__device__ __forceinline__ void rp_item(const T* __restrict__ src, T* __restrict__ dst, int item, int n_pair, int half,
-                                        const floatx2* cs) {
-  constexpr int WI = INTER ? 2 * W : W;  // elements at one place
-  struct alignas(W == 1 ? sizeof(T) : WI * sizeof(T)) Pack { T v[WI]; };
-  if (item >= n_pair) {
-    const int at = 2 * half + (item - n_pair) * W;
-    if constexpr (INTER) {
-      // the rest of the row is cut into W elements, half a place each
-      struct alignas(W == 1 ? sizeof(T) : W * sizeof(T)) Half { T v[W]; };
-      *reinterpret_cast<Half*>(dst + at) = *reinterpret_cast<const Half*>(src + at);
+// A head row as work items of V elements (16 bytes, 8 bytes, or one element, which assumes no alignment): n_pair items of W
+// pairs each (two places of V elements for halves), then items that copy V elements of the rest.
+template <typename T, bool INTER, int V>
+struct RopeItems {
+  static constexpr int W = INTER ? (V + 1) / 2 : V;       // pairs
+  static constexpr int P = INTER ? 2 * W : W;             // elements at one place
+  struct alignas(V * sizeof(T)) Place { T v[P]; };
+  struct alignas(V * sizeof(T)) Rest { T v[V]; };
+  int n_pair, per_row, half;
+
+  __device__ __forceinline__ RopeItems(int half_, int D) : n_pair(half_ / W), per_row(half_ / W + (D - 2 * half_) / V), half(half_) {}
+  static bool fits(int half, int D) { return half % W == 0 && (D - 2 * half) % V == 0; }
+
+  static __device__ __forceinline__ void copy(const T* src, T* dst, int at) {
+    *reinterpret_cast<Rest*>(dst + at) = *reinterpret_cast<const Rest*>(src + at);
+  }
+  __device__ __forceinline__ void run(const T* __restrict__ src, T* __restrict__ dst, int item, const floatx2* cs) const {
+    if (item >= n_pair) {
+      copy(src, dst, 2 * half + (item - n_pair) * V);
+    } else if constexpr (INTER) {
+      Place x = *reinterpret_cast<const Place*>(src + item * P);
+#pragma unroll
+      for (int e = 0; e < W; e++) {
+        const floatx2 r = cs[item * W + e];
+        const float a = (float)x.v[2 * e], b = (float)x.v[2 * e + 1];
+        x.v[2 * e] = (T)(a * r[0] - b * r[1]);
+        x.v[2 * e + 1] = (T)(a * r[1] + b * r[0]);
+      }
+      *reinterpret_cast<Place*>(dst + item * P) = x;
     } else {
-      *reinterpret_cast<Pack*>(dst + at) = *reinterpret_cast<const Pack*>(src + at);
-    }
-    return;
-  }
-  if constexpr (INTER) {
-    const int at = item * WI;
-    Pack x = *reinterpret_cast<const Pack*>(src + at);
+      const int at = item * W;
+      Place x = *reinterpret_cast<const Place*>(src + at), y = *reinterpret_cast<const Place*>(src + at + half);
 #pragma unroll
-    for (int e = 0; e < W; e++) {
-      const floatx2 r = cs[item * W + e];
-      const float a = rp_load(x.v[2 * e]), b = rp_load(x.v[2 * e + 1]);
-      x.v[2 * e] = rp_store<T>(a * r[0] - b * r[1]);
-      x.v[2 * e + 1] = rp_store<T>(a * r[1] + b * r[0]);
+      for (int e = 0; e < W; e++) {
+        const floatx2 r = cs[at + e];
+        const float a = (float)x.v[e], b = (float)y.v[e];
+        x.v[e] = (T)(a * r[0] - b * r[1]);
+        y.v[e] = (T)(a * r[1] + b * r[0]);
+      }
+      *reinterpret_cast<Place*>(dst + at) = x;
+      *reinterpret_cast<Place*>(dst + at + half) = y;
     }
-    *reinterpret_cast<Pack*>(dst + at) = x;
-  } else {
-    const int at = item * W;
-    Pack x = *reinterpret_cast<const Pack*>(src + at), y = *reinterpret_cast<const Pack*>(src + at + half);
-#pragma unroll
-    for (int e = 0; e < W; e++) {
-      const floatx2 r = cs[at + e];
-      const float a = rp_load(x.v[e]), b = rp_load(y.v[e]);
-      x.v[e] = rp_store<T>(a * r[0] - b * r[1]);
-      y.v[e] = rp_store<T>(a * r[1] + b * r[0]);
-    }
-    *reinterpret_cast<Pack*>(dst + at) = x;
-    *reinterpret_cast<Pack*>(dst + at + half) = y;
   }
+};
+
+// The angles of a workgroup's tokens, `half` of them each.
+template <typename F>
+__device__ __forceinline__ void rope_angles(floatx2* cs, const int* __restrict__ positions, const F* __restrict__ freq, long long tok0,
+                                            int tokens, int half, float mul, float sin_mul) {
+  for (int i = threadIdx.x; i < tokens * half; i += RP_THREADS) {
+    const int t = i / half;
+    cs[i] = rp_angle(positions[tok0 + t], (double)freq[i - t * half], mul, sin_mul);
+  }
+  __syncthreads();
 }
 
-// One token per workgroup: its angles into LDS, then its head rows.
-template <typename T, typename F, bool INTER, int W>
+// `per_wg` neighbouring tokens per workgroup.
+template <typename T, typename F, bool INTER, int V>
 __global__ __launch_bounds__(RP_THREADS) void rope_kernel(RopeRows x, const int* __restrict__ positions,
                                                           const F* __restrict__ freq, int half, int D, float mul,
-                                                          float sin_mul) {
-  __shared__ floatx2 cs[RP_MAX_PAIRS];
-  const long long tok = blockIdx.x;
-  const int pos = positions[tok];
-  for (int i = threadIdx.x; i < half; i += RP_THREADS) cs[i] = rp_angle(pos, (double)freq[i], mul, sin_mul);
-  __syncthreads();
-  const int n_pair = half / W, per_row = n_pair + (D - 2 * half) / W;
-  const T* src = static_cast<const T*>(x.src) + tok * x.src_token;
-  T* dst = static_cast<T*>(x.dst) + tok * x.dst_token;
-  for (int i = threadIdx.x; i < x.heads * per_row; i += RP_THREADS) {
-    const int h = i / per_row;
-    rp_item<T, INTER, W>(src + h * x.src_head, dst + h * x.dst_head, i - h * per_row, n_pair, half, cs);
+                                                          float sin_mul, int num_tokens, int per_wg) {
+  __shared__ floatx2 cs[RP_ANGLES];
+  const long long tok0 = (long long)blockIdx.x * per_wg;
+  const int tokens = num_tokens - tok0 < per_wg ? (int)(num_tokens - tok0) : per_wg;
+  rope_angles(cs, positions, freq, tok0, tokens, half, mul, sin_mul);
+  const RopeItems<T, INTER, V> items(half, D);
+  const int per_token = x.heads * items.per_row;
+  for (int i = threadIdx.x; i < tokens * per_token; i += RP_THREADS) {
+    const int row = i / items.per_row, t = tokens == 1 ? 0 : row / x.heads, h = row - t * x.heads;
+    items.run(static_cast<const T*>(x.src) + (tok0 + t) * x.src_token + h * x.src_head,
+              static_cast<T*>(x.dst) + (tok0 + t) * x.dst_token + h * x.dst_head, i - row * items.per_row, cs + t * half);
   }
 }
 
 // The serving form: queries rotated into q_out, keys rotated and values copied into the cache rows that `slots` names
 // (a slot outside [0, num_slots): the token's key and value are dropped).
-template <typename T, typename F, bool INTER, int W>
+template <typename T, typename F, bool INTER, int V>
 __global__ __launch_bounds__(RP_THREADS) void rope_append_kernel(RopeRows q, RopeRows k, RopeRows v,
                                                                  const int* __restrict__ positions,
                                                                  const F* __restrict__ freq, const long long* __restrict__ slots,
-                                                                 long long num_slots, int half, float mul) {
+                                                                 long long num_slots, int half, float mul, int num_tokens, int per_wg) {
   constexpr int D = 128;
-  __shared__ floatx2 cs[D / 2];
-  const long long tok = blockIdx.x;
-  const int pos = positions[tok];
-  const long long slot = slots[tok];
-  if ((int)threadIdx.x < half) cs[threadIdx.x] = rp_angle(pos, (double)freq[threadIdx.x], mul, mul);
-  __syncthreads();
-  const int n_pair = half / W, per_row = n_pair + (D - 2 * half) / W;
-  const bool keep = slot >= 0 && slot < num_slots;
-  const int rows = q.heads + (keep ? k.heads : 0);
-  for (int i = threadIdx.x; i < rows * per_row; i += RP_THREADS) {
-    const int h = i / per_row, item = i - h * per_row;
-    if (h < q.heads)
-      rp_item<T, INTER, W>(static_cast<const T*>(q.src) + tok * q.src_token + h * q.src_head,
-                           static_cast<T*>(q.dst) + tok * q.dst_token + h * q.dst_head, item, n_pair, half, cs);
-    else
-      rp_item<T, INTER, W>(static_cast<const T*>(k.src) + tok * k.src_token + (h - q.heads) * k.src_head,
-                           static_cast<T*>(k.dst) + slot * k.dst_token + (h - q.heads) * k.dst_head, item, n_pair, half, cs);
+  __shared__ floatx2 cs[RP_ANGLES];
+  const long long tok0 = (long long)blockIdx.x * per_wg;
+  const int tokens = num_tokens - tok0 < per_wg ? (int)(num_tokens - tok0) : per_wg;
+  rope_angles(cs, positions, freq, tok0, tokens, half, mul, mul);
+  typedef RopeItems<T, INTER, V> Items;
+  const Items items(half, D);
+  const int turned = q.heads + k.heads;
+  for (int i = threadIdx.x; i < tokens * turned * items.per_row; i += RP_THREADS) {
+    const int row = i / items.per_row, item = i - row * items.per_row, t = tokens == 1 ? 0 : row / turned, h = row - t * turned;
+    const long long tok = tok0 + t;
+    if (h < q.heads) {
+      items.run(static_cast<const T*>(q.src) + tok * q.src_token + h * q.src_head,
+                static_cast<T*>(q.dst) + tok * q.dst_token + h * q.dst_head, item, cs + t * half);
+    } else {
+      const long long slot = slots[tok];
+      if (slot >= 0 && slot < num_slots)
+        items.run(static_cast<const T*>(k.src) + tok * k.src_token + (h - q.heads) * k.src_head,
+                  static_cast<T*>(k.dst) + slot * k.dst_token + (h - q.heads) * k.dst_head, item, cs + t * half);
+    }
   }
-  if (!keep) return;
-  const T* vs = static_cast<const T*>(v.src) + tok * v.src_token;
-  T* vd = static_cast<T*>(v.dst) + slot * v.dst_token;
-  struct alignas(W == 1 ? sizeof(T) : W * sizeof(T)) Pack { T e[W]; };
-  for (int i = threadIdx.x; i < v.heads * (D / W); i += RP_THREADS) {
-    const int h = i / (D / W), e = (i - h * (D / W)) * W;
-    *reinterpret_cast<Pack*>(vd + h * v.dst_head + e) = *reinterpret_cast<const Pack*>(vs + h * v.src_head + e);
+  constexpr int pieces = D / V;
+  for (int i = threadIdx.x; i < tokens * v.heads * pieces; i += RP_THREADS) {
+    const int row = i / pieces, t = tokens == 1 ? 0 : row / v.heads, h = row - t * v.heads;
+    const long long tok = tok0 + t, slot = slots[tok];
+    if (slot >= 0 && slot < num_slots)
+      Items::copy(static_cast<const T*>(v.src) + tok * v.src_token + h * v.src_head,
+                  static_cast<T*>(v.dst) + slot * v.dst_token + h * v.dst_head, (i - row * pieces) * V);
   }
 }
 
-// whether every row of `x` starts on a 16-byte border
-static bool rows16(const RopeRows& x, int elem) {
-  const long long unit = 16 / elem;
-  return aligned16(x.src) && aligned16(x.dst) && x.src_token % unit == 0 && x.src_head % unit == 0 && x.dst_token % unit == 0 &&
-         x.dst_head % unit == 0;
+// whether every row of `x` starts on a border of `unit` elements
+static bool rows_on(const RopeRows& x, int unit, int elem) {
+  const uintptr_t bytes = (uintptr_t)unit * elem;
+  return reinterpret_cast<uintptr_t>(x.src) % bytes == 0 && reinterpret_cast<uintptr_t>(x.dst) % bytes == 0 && x.src_token % unit == 0 &&
+         x.src_head % unit == 0 && x.dst_token % unit == 0 && x.dst_head % unit == 0;
 }
 
+// Tokens per workgroup: one, unless a token has less than an item per thread (16384 tokens of one head of 128: 14 us with
+// four tokens, 23 with one; of 32 heads 102 with four, 96 with one), as long as that leaves the chip full of workgroups.
+static int rope_per_wg(int64_t tokens, int64_t items_per_token, int half) {
+  int64_t n = RP_THREADS / items_per_token;
+  n = n < tokens / 2048 ? n : tokens / 2048;
+  n = n < RP_ANGLES / half ? n : RP_ANGLES / half;
+  return n < 1 ? 1 : (int)n;
+}
+
+template <typename T, typename F, bool INTER, int V>
+static int rope_launch_as(const RopeRows& x, const int* pos, const F* freq, int half, int D, float mul, float sin_mul, int64_t tokens,
+                          hipStream_t s) {
+  const int per_wg = rope_per_wg(tokens, (int64_t)x.heads * D / RopeItems<T, INTER, V>::P, half);
+  dim3 grid((unsigned)((tokens + per_wg - 1) / per_wg)), block(RP_THREADS);
+  hipLaunchKernelGGL((rope_kernel<T, F, INTER, V>), grid, block, 0, s, x, pos, freq, half, D, mul, sin_mul, (int)tokens, per_wg);
+  return check_launch("rope_kernel", grid, block, 0);
+}
+
+// The widest accesses that the rows, the rotated part and the rest allow.  A head of 80 with 40 rotated elements has 8-byte ones.
 template <typename T, typename F, bool INTER>
 static int rope_launch(const RopeRows& x, const int* pos, const F* freq, int half, int D, float mul, float sin_mul, int64_t tokens,
                        hipStream_t s) {
-  constexpr int V = 16 / sizeof(T);           // elements of 16 bytes
-  constexpr int W = INTER ? V / 2 : V;        // pairs (or elements of a half) per item
-  dim3 grid((unsigned)tokens), block(RP_THREADS);
-  const bool wide = rows16(x, sizeof(T)) && half % W == 0 && (D - 2 * half) % W == 0;
-  if (wide)
-    hipLaunchKernelGGL((rope_kernel<T, F, INTER, W>), grid, block, 0, s, x, pos, freq, half, D, mul, sin_mul);
-  else
-    hipLaunchKernelGGL((rope_kernel<T, F, INTER, 1>), grid, block, 0, s, x, pos, freq, half, D, mul, sin_mul);
-  return check_launch("rope_kernel", grid, block, 0);
+  constexpr int V16 = 16 / sizeof(T), V8 = V16 / 2;
+  if (rows_on(x, V16, sizeof(T)) && RopeItems<T, INTER, V16>::fits(half, D))
+    return rope_launch_as<T, F, INTER, V16>(x, pos, freq, half, D, mul, sin_mul, tokens, s);
+  if (rows_on(x, V8, sizeof(T)) && RopeItems<T, INTER, V8>::fits(half, D))
+    return rope_launch_as<T, F, INTER, V8>(x, pos, freq, half, D, mul, sin_mul, tokens, s);
+  return rope_launch_as<T, F, INTER, 1>(x, pos, freq, half, D, mul, sin_mul, tokens, s);
+}
+
+template <typename T, typename F, bool INTER, int V>
+static int rope_append_as(const RopeRows& q, const RopeRows& k, const RopeRows& v, const int* pos, const F* freq, const int64_t* slots,
+                          long long num_slots, int half, float mul, int64_t tokens, hipStream_t s) {
+  const int per_wg = rope_per_wg(tokens, (int64_t)(q.heads + 2 * k.heads) * 128 / RopeItems<T, INTER, V>::P, half);
+  dim3 grid((unsigned)((tokens + per_wg - 1) / per_wg)), block(RP_THREADS);
+  hipLaunchKernelGGL((rope_append_kernel<T, F, INTER, V>), grid, block, 0, s, q, k, v, pos, freq, reinterpret_cast<const long long*>(slots),
+                     num_slots, half, mul, (int)tokens, per_wg);
+  return check_launch("rope_append_kernel", grid, block, 0);
 }
 
 template <typename T, typename F, bool INTER>
 static int rope_append_launch(const RopeRows& q, const RopeRows& k, const RopeRows& v, const int* pos, const F* freq,
                               const int64_t* slots, long long num_slots, int half, float mul, int64_t tokens, hipStream_t s) {
-  constexpr int V = 16 / sizeof(T), W = INTER ? V / 2 : V;
-  dim3 grid((unsigned)tokens), block(RP_THREADS);
-  const bool wide = rows16(q, sizeof(T)) && rows16(k, sizeof(T)) && rows16(v, sizeof(T)) && half % W == 0;
-  const long long* sl = reinterpret_cast<const long long*>(slots);
-  if (wide)
-    hipLaunchKernelGGL((rope_append_kernel<T, F, INTER, W>), grid, block, 0, s, q, k, v, pos, freq, sl, num_slots, half, mul);
-  else
-    hipLaunchKernelGGL((rope_append_kernel<T, F, INTER, 1>), grid, block, 0, s, q, k, v, pos, freq, sl, num_slots, half, mul);
-  return check_launch("rope_append_kernel", grid, block, 0);
+  constexpr int V16 = 16 / sizeof(T), V8 = V16 / 2;
+  auto on = [&](int unit) { return rows_on(q, unit, sizeof(T)) && rows_on(k, unit, sizeof(T)) && rows_on(v, unit, sizeof(T)); };
+  if (on(V16) && RopeItems<T, INTER, V16>::fits(half, 128))
+    return rope_append_as<T, F, INTER, V16>(q, k, v, pos, freq, slots, num_slots, half, mul, tokens, s);
+  if (on(V8) && RopeItems<T, INTER, V8>::fits(half, 128))
+    return rope_append_as<T, F, INTER, V8>(q, k, v, pos, freq, slots, num_slots, half, mul, tokens, s);
+  return rope_append_as<T, F, INTER, 1>(q, k, v, pos, freq, slots, num_slots, half, mul, tokens, s);
 }
 
 }  // namespace mi355

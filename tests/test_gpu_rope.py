@@ -24,7 +24,7 @@ def _freq(R, **kw):
 
 @pytest.mark.parametrize("inter", [False, True])
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32])
-@pytest.mark.parametrize("T,H,D,R", [(1, 1, 128, 128), (5, 3, 128, 64), (33, 7, 96, 96), (4, 2, 80, 48), (3, 5, 66, 22), (7, 1, 2, 2), (2, 2, 1100, 1024), (9, 32, 64, 10)])
+@pytest.mark.parametrize("T,H,D,R", [(1, 1, 128, 128), (5, 3, 128, 64), (33, 7, 96, 96), (4, 2, 80, 48), (3, 5, 66, 22), (7, 1, 2, 2), (2, 2, 1100, 1024), (9, 32, 64, 10), (70, 2, 80, 40), (3000, 1, 8, 8), (5000, 2, 72, 24)])
 def test_rope(dev, T, H, D, R, dtype, inter):
     from oracle import serving
 
