@@ -174,7 +174,7 @@ int mi355_flash_attn_fwd_strided_bf16(const void* q, const void* k, const void* 
  * read on the device only: nothing has to be known on the host, and a captured launch serves any lengths.
  * Rows of o outside every sequence are left as they are; with zero_rest != 0 those in front of the first and behind
  * the last sequence are set to zero.  total_q, total_k <= 2^24, total_q * H / Hkv <= 2^30, num_seqs <= 65535.
- * A weight of zero times a non-finite V row of the same sequence is NaN, as in the formula.
+ * With the mask, keys and values that a query does not see do not reach it, whatever they hold (NaN and infinities too).
  * Replaces: the SDPA root of mi355_flash_attn_fwd for a ragged batch, which the reference can only pad
  * (tests/dynamo/llama_test.py:285-290 builds one rectangular mask).
  */
@@ -366,13 +366,14 @@ int mi355_paged_prefill_attn_bf16(const void* q, const void* k_cache, const void
  * seq_lens:    [num_seqs] int32, cut to [0, max_pages_per_seq * page_size]; shorter than num_nodes: the first nodes are not
  *              in the cache and nobody sees them
  * parents:     [num_seqs, num_nodes] int32; a value outside [0, n) for node n: it has no ancestors (a root)
- * A query that sees nothing gives zeros.  The V rows of all drafts have to hold numbers, also of branches that a query does
- * not see (a weight of zero times a non-finite value is NaN): a sequence with fewer drafts than num_nodes writes its
- * padding too.  1 <= num_nodes <= 64, num_q_heads / num_kv_heads <= 128, D == 128, page_size 16, 32, 64,
+ * A query that sees nothing gives zeros; what it does not see does not reach it, whatever is there (drafts that were never
+ * written, other branches, the rest of the last page).
+ * 1 <= num_nodes <= 64, num_q_heads / num_kv_heads <= 128, D == 128, page_size 16, 32, 64,
  * 128 or 256, 1 <= num_splits <= 1024.  A chain (parents[n] = n - 1) is the causal mask among the drafts.
  * num_splits cuts the table's reach into that many chunks, each by its own workgroups; num_splits > 1 needs
  * part_acc [num_seqs, num_nodes, num_q_heads, num_splits, D] and part_ml [.., num_splits, 2], fp32, written before they are
- * read in the same call, and at most 2^23 query rows (num_seqs * num_nodes * num_q_heads).  No counterpart in the reference; the mask generalises tests/dynamo/llama_test.py:285-290.
+ * read in the same call, and at most 2^23 query rows (num_seqs * num_nodes * num_q_heads).  No counterpart in the
+ * reference; the mask generalises tests/dynamo/llama_test.py:285-290.
  */
 int mi355_paged_tree_attn(const void* q, const void* k_cache, const void* v_cache,
                           const int32_t* block_table, const int32_t* seq_lens, const int32_t* parents, void* out,

@@ -4,15 +4,21 @@
 // sees every token in front of the drafts, itself and its ancestors.  With G query heads per kv head there are R = N * G
 // query rows (row r: node r / G, head r % G of the group) that read the same keys and values: they share one pass.
 //
-// The op is HBM bound up to about 160 rows (a K and a V row are 512 bytes and 512 flop per query row), so the kernel is
-// the one-token decode kernel's: every wave streams its own steps of 32 tokens -- K straight into MFMA operand
-// registers, V through a private LDS ring by direct-to-LDS loads, both one step ahead -- and no wave waits for another
-// before the end.  What differs: a step's K and V serve C column groups of 16 query rows (C = 1, 2 or 4; more rows than
-// 64 take further workgroups, which find the pages in the caches), and scores of draft positions are masked by the
-// node's set of ancestors, a 64-bit word per node made from the parents once per workgroup by pointer doubling.
+// The op is HBM bound up to about 250 rows (a K and a V row are 512 bytes and 512 flop per query row; 1.29 PFLOP/s against 5 TB/s).
+// Up to 32 rows are this file's kernel, built as the one-token decode kernel is: every wave streams its own steps of 32
+// tokens -- K straight into MFMA operand registers, V through a private LDS ring by direct-to-LDS loads, both one step
+// ahead -- and no wave waits for another before the end.  What differs: a step's K and V serve C = 1 or 2 column groups
+// of 16 query rows, and scores of draft positions are masked by the node's set of ancestors, a 64-bit word per node made
+// from the parents once per workgroup by pointer doubling.  More rows are the prefill kernel's TREE form, whose waves
+// split the rows and share a tile: with four column groups here every wave read every V fragment for itself, and 64
+// sequences of 512 to 8192 tokens with 64 rows took 317 us, on the TREE form 208 (and 175 with today's order of work).
 //
 // The table's reach is cut into num_splits chunks of equally many 32-token steps; a sequence that fits one chunk writes
-// its result directly, the others write fp32 partials that a second launch merges.
+// its result directly, the others write fp32 partials that a second launch merges (two launches wherever the table's reach
+// is cut: the lengths are not known on the host).  Full chunks are handed out before shorter ones, see tree.hpp.
+//
+// Measured (8 K/V heads, 64 rows, bf16): one sequence of 32768 tokens 37 us (3.6 TB/s; merging included), 64 of 512 to 8192
+// tokens 175 us (4.3 TB/s of the 5.0 that a copy reaches).  Looking masked steps over for non-finite values is 1 to 5 of these.
 #include "tree.hpp"
 #include <math.h>
 
@@ -21,6 +27,23 @@ namespace mi355 {
 constexpr int PT_WAVES = 4;
 constexpr int PT_WAVE_LDS = 2 * 8192;  // two stages of 32 V rows
 constexpr int PT_MAX_GROUP = 128;  // query heads per kv head
+
+// bits 0 .. n - 1, at most four of them
+__device__ __forceinline__ unsigned pt_first4(int n) { return n >= 4 ? 15u : n <= 0 ? 0u : (1u << n) - 1u; }
+
+// The entries of v whose bit of `there` is set, zeros for the others and, unless the step is clean, for infinities and NaN.  By
+// bit operations, as in tree_hide: conditional assignments to the vector's elements have been compiled to ones that keep them.
+template <bool BF>
+__device__ __forceinline__ half4 pt_keep(half4 v, unsigned there, bool clean) {
+  uint2 w = __builtin_bit_cast(uint2, v);
+  auto keep = [&](unsigned two, unsigned bits) {
+    unsigned m = ((bits & 1u) | (bits & 2u) << 15) * 0xFFFFu;
+    if (!clean) m &= ~((tree_nonfinite2<BF>(two) >> 15) * 0xFFFFu);
+    return two & m;
+  };
+  w.x = keep(w.x, there), w.y = keep(w.y, there >> 2);
+  return __builtin_bit_cast(half4, w);
+}
 
 template <int C, bool BF>
 __global__ __launch_bounds__(PT_WAVES * 64) __attribute__((amdgpu_waves_per_eu(2, 2))) void paged_tree_kernel(TreeArgs a) {
@@ -179,16 +202,51 @@ __global__ __launch_bounds__(PT_WAVES * 64) __attribute__((amdgpu_waves_per_eu(2
           for (int dt = 0; dt < 8; dt++) oacc[c][dt] = oacc[c][dt] * alpha;
         }
         const char* vst = my_lds + b * 8192;
+        // What a query does not see does not reach it, whatever it holds: a weight of zero times a non-finite V entry would be
+        // NaN.  In the steps with masked tokens such entries are added by themselves to the queries that see them (the
+        // sums become infinity or NaN, whatever the weight) and left out of the product.
+        bool clean = true;
+        unsigned there0 = 15, there1 = 15;  // which of the lane's tokens are in the cache
+        if (edge) {
+          there0 = drop0 ? 0u : pt_first4(L - tok0);
+          there1 = drop1 ? 0u : pt_first4(L - tok0 - 16);
+          unsigned any = 0;
+#pragma unroll
+          for (int i = 0; i < 8; i++) {
+            const uint4 x = *reinterpret_cast<const uint4*>(vst + (i * 64 + lane) * 16);
+            any |= tree_nonfinite2<BF>(x.x) | tree_nonfinite2<BF>(x.y) | tree_nonfinite2<BF>(x.z) | tree_nonfinite2<BF>(x.w);
+          }
+          clean = __builtin_amdgcn_ballot_w64(any != 0) == 0;
+          if (!clean) {
+#pragma unroll 1
+            for (int j = 0; j < 32; j++) {
+              const int t = pa * 16 + j;
+              if (t >= L || (j < 16 ? drop0 : drop1)) continue;
+              unsigned sees[C];
+#pragma unroll
+              for (int c = 0; c < C; c++) sees[c] = 0u - (tree_visible4(seen[c], t - draft0) & 1u);
+#pragma unroll
+              for (int dt = 0; dt < 8; dt++) {
+                const int row = j & 15, chunk = (2 * dt + (g >> 1)) ^ (2 * (row & 7));
+                uint2 v = *reinterpret_cast<const uint2*>(vst + (j >> 4) * 4096 + row * 256 + chunk * 16 + (g & 1) * 8);
+                v.x &= (tree_nonfinite2<BF>(v.x) >> 15) * 0xFFFFu, v.y &= (tree_nonfinite2<BF>(v.y) >> 15) * 0xFFFFu;
+#pragma unroll
+                for (int c = 0; c < C; c++) {
+                  const unsigned x = v.x & sees[c], y = v.y & sees[c];
+                  const floatx4 add = {tree_value<BF>(x & 0xFFFFu), tree_value<BF>(x >> 16), tree_value<BF>(y & 0xFFFFu), tree_value<BF>(y >> 16)};
+                  oacc[c][dt] = oacc[c][dt] + add;
+                }
+              }
+            }
+          }
+        }
 #pragma unroll
         for (int dt = 0; dt < 8; dt++) {
           half4 lo = lds_read_tr16(vst + (vr_base ^ (dt * 32)));
           half4 hi = lds_read_tr16(vst + 4096 + (vr_base ^ (dt * 32)));
-          if (edge) {  // tokens at or beyond L may hold anything (NaN included): 0 * garbage must stay 0
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-              if (drop0 || tok0 + e >= L) lo[e] = (half_t)0;
-              if (drop1 || tok0 + 16 + e >= L) hi[e] = (half_t)0;
-            }
+          if (edge) {  // 0 * garbage must stay 0
+            lo = pt_keep<BF>(lo, there0, clean);
+            hi = pt_keep<BF>(hi, there1, clean);
           }
           const half8 vf = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
 #pragma unroll
@@ -221,19 +279,17 @@ __global__ __launch_bounds__(PT_WAVES * 64) __attribute__((amdgpu_waves_per_eu(2
 #pragma unroll
       for (int w = 0; w < PT_WAVES; w++) m_tot = fmaxf(m_tot, sm[w * 16 + col]);
       float acc = 0.f, lt = 0.f;
-      if (m_tot > -INFINITY) {
 #pragma unroll
-        for (int w = 0; w < PT_WAVES; w++) {
-          const float mw = sm[w * 16 + col];
-          const float wgt = mw > -INFINITY ? __builtin_amdgcn_exp2f((mw - m_tot) * a.scale_log2e) : 0.f;
-          acc += wgt * sacc[(w * 16 + col) * 128 + d];
-          lt += wgt * sl[w * 16 + col];
-        }
+      for (int w = 0; w < PT_WAVES; w++) {
+        // (no maximum: zeros, or a row of scores that are not numbers; either is passed on as it is)
+        const float wgt = m_tot > -INFINITY ? __builtin_amdgcn_exp2f((sm[w * 16 + col] - m_tot) * a.scale_log2e) : 1.f;
+        acc += wgt * sacc[(w * 16 + col) * 128 + d];
+        lt += wgt * sl[w * 16 + col];
       }
       const int node = r / a.group;
       const size_t row = ((size_t)seq * a.nodes + node) * num_q_heads + kvh * a.group + (r - node * a.group);
       if (single) {
-        a.out[row * 128 + d] = cvt16<BF>(lt > 0.f ? acc / lt : 0.f);
+        a.out[row * 128 + d] = cvt16<BF>(lt == 0.f ? 0.f : acc / lt);
       } else {
         const size_t at = row * a.num_splits + split;
         a.part_acc[at * 128 + d] = acc;
@@ -272,15 +328,13 @@ __global__ __launch_bounds__(256) void paged_tree_merge_kernel(TreeArgs a, int n
   for (int d = 16; d >= 1; d >>= 1) m_tot = fmaxf(m_tot, __shfl_xor(m_tot, d));
   floatx4 o = {0.f, 0.f, 0.f, 0.f};
   float l = 0.f;
-  if (m_tot > -INFINITY) {
 #pragma unroll 4
-    for (int s = part; s < n; s += GROUPS) {
-      const float w = __builtin_amdgcn_exp2f(ml[2 * s] - m_tot);
-      const floatx4 p = *reinterpret_cast<const floatx4*>(acc + (size_t)s * 128);
-      l = __builtin_fmaf(w, ml[2 * s + 1], l);
+  for (int s = part; s < n; s += GROUPS) {
+    const float w = m_tot > -INFINITY ? __builtin_amdgcn_exp2f(ml[2 * s] - m_tot) : 1.f;  // (see the kernel's own merge)
+    const floatx4 p = *reinterpret_cast<const floatx4*>(acc + (size_t)s * 128);
+    l = __builtin_fmaf(w, ml[2 * s + 1], l);
 #pragma unroll
-      for (int e = 0; e < 4; e++) o[e] = __builtin_fmaf(w, p[e], o[e]);
-    }
+    for (int e = 0; e < 4; e++) o[e] = __builtin_fmaf(w, p[e], o[e]);
   }
   if constexpr (GROUPS > 1) {
     sum[grp][l32] = o;
@@ -296,7 +350,7 @@ __global__ __launch_bounds__(256) void paged_tree_merge_kernel(TreeArgs a, int n
     }
   }
   if (n == 0) return;
-  const float inv = l > 0.f ? 1.f / l : 0.f;
+  const float inv = l == 0.f ? 0.f : 1.f / l;
   const half4 v = {cvt16<BF>(o[0] * inv), cvt16<BF>(o[1] * inv), cvt16<BF>(o[2] * inv), cvt16<BF>(o[3] * inv)};
   *reinterpret_cast<half4*>(a.out + (size_t)row * 128 + l32 * 4) = v;
 }

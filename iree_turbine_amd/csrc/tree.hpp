@@ -51,6 +51,18 @@ __device__ __forceinline__ float tree_hide(float v, unsigned visible, int r) {
   return __builtin_bit_cast(float, (__builtin_bit_cast(unsigned, v) & keep) | (0xFF800000u & ~keep));
 }
 
+// Bits 15 and 31 where the low and the high of two 16-bit numbers are infinite or NaN (an exponent of all ones).
+template <bool BF>
+__device__ __forceinline__ unsigned tree_nonfinite2(unsigned two) {
+  return BF ? ((two & 0x7F807F80u) + 0x00800080u) & 0x80008000u : ((two & 0x7C007C00u) + 0x04000400u) & 0x80008000u;
+}
+
+// The 16-bit number of these bits.
+template <bool BF>
+__device__ __forceinline__ float tree_value(unsigned bits) {
+  return BF ? __builtin_bit_cast(float, bits << 16) : (float)__builtin_bit_cast(half_t, (unsigned short)bits);
+}
+
 // Piece of work number `item` of a call whose sequences are cut into chunks of `chunk_steps` 32-token steps: its sequence and chunk;
 // false behind the last.  Up to 64 sequences (one per lane, every wave by itself): all full chunks first, then the
 // sequences' last chunks, the longest first, so that the short ones make up the tail.  Nothing empty lies between: workgroups

@@ -656,8 +656,9 @@ class paged_tree_attn(CustomOp):
     """Attention of drafted token trees over the paged cache: q [S, N, Hq, 128], N <= 64 nodes per sequence, whose K/V are the last N
     tokens of the cache (seq_lens int32 [S] counts them); parents int32 [S, N] (a value outside [0, n) for node n: a root).
     Node n sees every token in front of the drafts, its ancestors and itself; with parents[n] = n - 1 this is
-    paged_prefill_attn of N new tokens.  All N positions' V rows have to hold numbers (write padding too).  num_kv_splits <= 0 picks a default from the table width; scale <= 0 selects
-    1/sqrt(D).  Returns [S, N, Hq, 128]."""
+    paged_prefill_attn of N new tokens.  What a node does not see does not reach it, whatever it holds (padding may stay
+    unwritten).  num_kv_splits <= 0 picks a default from the table width; scale <= 0 selects 1/sqrt(D).  Returns
+    [S, N, Hq, 128]."""
 
     signature = "paged_tree_attn(Tensor q, Tensor k_cache, Tensor v_cache, Tensor block_table, Tensor seq_lens, Tensor parents, float scale, int num_kv_splits) -> Tensor"
 

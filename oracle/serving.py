@@ -63,13 +63,12 @@ def rope_ref(x, positions, inv_freq, interleaved: bool, inverse: bool = False, s
     return out, slack + rounding
 
 
-def attention_ref(q, k, v, visible, scale: float | None = None, q_rounded: bool = False):
+def attention_ref(q, k, v, visible, scale: float | None = None):
     """(result, bound) in float64 for q [n, Hq, D], k, v [m, Hkv, D], visible bool [n, m]; a query that sees nothing: zeros.
 
     The bound, with h = half a step of the 16-bit type and f = 2^-24: a score of D products summed in 32 bits is off by
-    at most D f (scale |q| . |k|), its product with the scale and the subtraction of the maximum by 4 f (|s| + |max|), and
-    by h (scale |q| . |k|) more where the kernel rounds the scaled query to 16 bits; with d the largest of these, weights
-    move by a factor e^(2 d) at most; each weight is rounded to 16 bits once (h) and again where its sum is taken from the
+    at most D f (scale |q| . |k|), its product with the scale and the subtraction of the maximum by 4 f (|s| + |max|); with
+    d the largest of these, weights move by a factor e^(2 d) at most; each weight is rounded to 16 bits once (h) and again where its sum is taken from the
     rounded ones (h); the accumulation over m keys adds (m + 64) f; the result is rounded once (h)."""
     n, hq, D = q.shape
     m, hkv = k.shape[0], k.shape[1]
@@ -86,7 +85,7 @@ def attention_ref(q, k, v, visible, scale: float | None = None, q_rounded: bool 
         s = torch.where(visible, s, -math.inf)
         mag = torch.where(visible, (qq.abs() @ kk.abs().t()) * scale, 0.0)
         top = s.amax(-1, keepdim=True)
-        off = mag * (D * f + (h if q_rounded else 0.0)) + 4 * f * torch.where(visible, s.abs() + top.abs(), 0.0)
+        off = mag * D * f + 4 * f * torch.where(visible, s.abs() + top.abs(), 0.0)
         d = off.amax(-1, keepdim=True)
         w = torch.exp(s - torch.where(top == -math.inf, 0.0, top))
         w = w / torch.where(w.sum(-1, keepdim=True) > 0, w.sum(-1, keepdim=True), 1.0)
@@ -97,7 +96,7 @@ def attention_ref(q, k, v, visible, scale: float | None = None, q_rounded: bool 
     return out, bound
 
 
-def varlen_ref(q, k, v, cu_q, cu_k, is_causal: bool, scale: float | None = None, q_rounded: bool = False):
+def varlen_ref(q, k, v, cu_q, cu_k, is_causal: bool, scale: float | None = None):
     out = torch.zeros(q.shape, dtype=torch.float64)
     bound = torch.zeros_like(out)
     cq, ck = [x.tolist() for x in (cu_q, cu_k)]
@@ -107,7 +106,7 @@ def varlen_ref(q, k, v, cu_q, cu_k, is_causal: bool, scale: float | None = None,
         visible = torch.ones(b - a, max(d - c, 0), dtype=torch.bool)
         if is_causal:
             visible = visible.tril(d - c - (b - a))
-        out[a:b], bound[a:b] = attention_ref(q[a:b], k[c:d], v[c:d], visible, scale, q_rounded)
+        out[a:b], bound[a:b] = attention_ref(q[a:b], k[c:d], v[c:d], visible, scale)
     return out, bound
 
 

@@ -89,6 +89,37 @@ def test_bad_pages_are_dropped(dev, splits):
     assert torch.equal(got[2].cpu(), torch.zeros(6, 8, 128).bfloat16())
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("N,hq,hkv", [(4, 4, 2), (7, 8, 2), (12, 8, 2), (40, 8, 2)], ids=["16 rows", "32 rows", "64 rows", "160 rows"])
+@pytest.mark.parametrize("splits", [1, 3])
+def test_other_branches_do_not_leak(dev, splits, N, hq, hkv, dtype):
+    """A draft that was never written (NaN and infinities in its place) changes nothing for nodes of other branches; its
+    descendants see it: infinity where its value is infinite, NaN where its key is NaN."""
+    from oracle import serving
+
+    announce(f"tree other branches N={N} hq={hq} {dtype} splits={splits}")
+    lens = [150 + N, N, 64 + N]
+    q, kc, vc, table, sl = _inputs(3, lens, N, hq, hkv, 16, dtype)
+    par = torch.tensor([[-1, 0, 0, 1] + [1] * (N - 4)] * 3, dtype=torch.int32)  # node 2 has no children, node 3 is node 1's
+    place = lambda s, n: (int(table[s, (lens[s] - N + n) // 16]), (lens[s] - N + n) % 16)
+    want, bound = serving.tree_ref(q, torch.nan_to_num(kc, 0.0), torch.nan_to_num(vc, 0.0), table, sl, par)
+    for s in range(3):
+        p, at = place(s, 2)
+        kc[p, at], vc[p, at] = float("nan"), float("inf")
+        p, at = place(s, 3)
+        vc[p, at, 0, 9], vc[p, at, hkv - 1, 100] = float("-inf"), float("nan")
+    got = torch.ops.mi355.paged_tree_attn(*(t.to(dev) for t in (q, kc, vc, table, sl, par)), 0.0, splits).cpu()
+    others = [n for n in range(N) if n not in (2, 3)]
+    off = (got[:, others].double() - want[:, others]).abs() - bound[:, others]
+    assert torch.isfinite(got[:, others]).all() and float(off.max()) <= 0
+    assert bool(got[:, 2].isnan().all())
+    g = hq // hkv
+    assert bool((got[:, 3, :g, 9] == float("-inf")).all()) and bool(got[:, 3, hq - g:, 100].isnan().all())
+    clear = torch.ones(128, dtype=torch.bool)
+    clear[[9, 100]] = False
+    assert float(((got[:, 3].double() - want[:, 3]).abs() - bound[:, 3])[..., clear].max()) <= 0
+
+
 def test_chain_is_paged_prefill(dev):
     """A chain is the causal mask: the prefill op's result within the two kernels' rounding; single nodes are decode."""
     announce("tree chain against prefill and decode")

@@ -27,7 +27,7 @@ def _run(dev, lq, lk, hq, hkv, causal, dtype, scale=0.0, spread=1.0, pad=0):
     k, v = ((torch.randn(max(1, sum(lk) + pad), hkv, 128)).to(dtype) for _ in range(2))
     cq, ck = _cu(lq), _cu(lk)
     got = torch.ops.mi355.flash_attn_varlen_fwd(q.to(dev), k.to(dev), v.to(dev), cq.to(dev), ck.to(dev), causal, scale)
-    want, bound = serving.varlen_ref(q, k, v, cq, ck, causal, scale or None, q_rounded=True)
+    want, bound = serving.varlen_ref(q, k, v, cq, ck, causal, scale or None)
     _inside(got, want, bound)
     return got
 
@@ -92,7 +92,7 @@ def test_neighbours_do_not_leak(dev, causal):
     got = torch.ops.mi355.flash_attn_varlen_fwd(q.to(dev), k.to(dev), v.to(dev), cu.to(dev), cu.to(dev), causal, 0.0)
     clean = torch.ones(T, dtype=torch.bool)
     clean[76:109] = False
-    want, bound = serving.varlen_ref(q, torch.nan_to_num(k, 0.0, 0.0), torch.nan_to_num(v, 0.0, 0.0, 0.0), cu, cu, causal, q_rounded=True)
+    want, bound = serving.varlen_ref(q, torch.nan_to_num(k, 0.0, 0.0), torch.nan_to_num(v, 0.0, 0.0, 0.0), cu, cu, causal)
     _inside(got.cpu()[clean], want[clean], bound[clean])
     outside = torch.ones(T, dtype=torch.bool)
     outside[6:int(cu[-1])] = False
@@ -101,6 +101,40 @@ def test_neighbours_do_not_leak(dev, causal):
     launch.flash_attn_varlen_fwd_out(q.to(dev), k.to(dev), v.to(dev), cu.to(dev), cu.to(dev), o, causal, 0.0)
     assert torch.equal(o.cpu()[outside], torch.full((15, 4, 128), 7.0).half())
     assert torch.equal(o.cpu()[~outside & clean], got.cpu()[~outside & clean])
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("lens,hq,hkv", [([150, 40, 5], 4, 2), ([700], 8, 8), ([2048, 300], 32, 8)], ids=["64 rows", "one", "128 rows"])
+def test_later_tokens_do_not_leak(dev, lens, hq, hkv, dtype):
+    """A token whose key and value hold NaN or infinities changes nothing for the queries in front of it, also in the tile
+    that both lie in; queries that see an infinite value get an infinity in its column, one that sees a NaN gets NaN."""
+    from oracle import serving
+
+    announce(f"varlen later tokens lens={lens} {dtype}")
+    cu = _cu(lens)
+    q, k, v = (torch.randn(sum(lens), h, 128).to(dtype) for h in (hq, hkv, hkv))
+    bad = [min(9, lens[0] - 1), lens[0] - 1]
+    kb, vb = k.clone(), v.clone()
+    kb[bad[1]] = float("nan")
+    vb[bad[1]] = float("inf")
+    vb[bad[0], 0, 5], vb[bad[0], 0, 77], vb[bad[0], hkv - 1, 127] = float("inf"), float("-inf"), float("nan")
+    args = [t.to(dev) for t in (q, kb, vb, cu, cu)]
+    got = torch.ops.mi355.flash_attn_varlen_fwd(*args, True, 0.0).cpu()
+    want, bound = serving.varlen_ref(q[:300], k[:300], v[:300], torch.tensor([0, min(300, lens[0])]), torch.tensor([0, min(300, lens[0])]), True)
+    front = got[: bad[0]].double()
+    assert torch.isfinite(front).all() and bool(((front - want[: bad[0]]).abs() <= bound[: bad[0]]).all())
+    seen = got[bad[0] : bad[1]]
+    g = hq // hkv
+    if len(seen):
+        assert bool((seen[:, :g, 5] == float("inf")).all()) and bool((seen[:, :g, 77] == float("-inf")).all()) and bool(seen[:, hq - g :, 127].isnan().all())
+        clear = torch.ones(128, dtype=torch.bool)
+        clear[[5, 77, 127]] = False
+        n = min(bad[1], len(want))
+        off = (got[bad[0] : n].double() - want[bad[0] : n]).abs() - bound[bad[0] : n]
+        assert float(off[..., clear].max()) <= 0
+    assert bool(got[bad[1]].isnan().all())
+    other = torch.ops.mi355.flash_attn_varlen_fwd(*(t.to(dev) for t in (q, k, v, cu, cu)), True, 0.0).cpu()
+    assert torch.equal(got[lens[0]:], other[lens[0]:])
 
 
 def test_offsets_outside_the_stream(dev):
