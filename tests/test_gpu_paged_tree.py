@@ -61,6 +61,16 @@ def test_tree(dev, N, hq, hkv, page, dtype, splits):
     _check(dev, _inputs(N, lens, N, hq, hkv, page, dtype), _parents(N, 5, N, 4), splits)
 
 
+@pytest.mark.parametrize("splits", [1, 3, 0])
+@pytest.mark.parametrize("S,N,hq", [(64, 3, 4), (65, 3, 4), (70, 12, 8), (64, 12, 8)])
+def test_many_sequences(dev, S, N, hq, splits):
+    """Up to 64 sequences are handed out by falling size, more chunk by chunk; lengths from none to several chunks."""
+    announce(f"tree sequences={S} N={N} hq={hq} splits={splits}")
+    rng = random.Random(S + N)
+    lens = [rng.choice([0, 1, N, 31, 32, 33, rng.randrange(N, 700)]) for _ in range(S)]
+    _check(dev, _inputs(S, lens, N, hq, 2, 16, torch.bfloat16), _parents(S, S, N, 3), splits)
+
+
 @pytest.mark.parametrize("splits", [1, 3])
 def test_tree_lengths_on_the_borders(dev, splits):
     """Drafts that start inside a 16-token block, across pages, sequences shorter than their drafts, empty and wild lengths."""
