@@ -21,7 +21,13 @@ def require(cond: bool, msg: str) -> None:
 
 
 def same_half_dtype(tensors) -> bool:
-    return tensors[0].dtype in HALF_DTYPES and all(t.dtype == tensors[0].dtype for t in tensors)
+    dtype = tensors[0].dtype
+    if dtype not in HALF_DTYPES:
+        return False
+    for t in tensors:  # (not a generator: a microsecond of every call)
+        if t.dtype != dtype:
+            return False
+    return True
 
 
 def check_gemm_operands(op: str, a: Tensor, b: Tensor, dtypes=HALF_DTYPES, what: str = "float16 or both bfloat16") -> None:

@@ -539,7 +539,7 @@ class rope(CustomOp):
 
     def eager_execute(self, x, positions, inv_freq, interleaved, inverse, scale):
         dev = launch._dev(x, positions, inv_freq)
-        return launch._rope(dev, x, positions, inv_freq, torch.empty(x.shape, dtype=x.dtype, device=dev), interleaved, inverse, scale)
+        return launch._rope(dev, x, positions, inv_freq, x.new_empty(x.shape), interleaved, inverse, scale)
 
 
 def _on_device_eagerly(x: Tensor) -> bool:
@@ -572,7 +572,7 @@ class _RopeGrad(torch.autograd.Function):
         if torch.is_grad_enabled():
             dx = torch.ops.mi355.rope(grad, positions, inv_freq, *how)
         elif _on_device_eagerly(grad):  # its sizes and type are the result's, whose call has been checked
-            dx = launch._rope(grad.device, grad, positions, inv_freq, torch.empty(grad.shape, dtype=grad.dtype, device=grad.device), *how)
+            dx = launch._rope(grad.device, grad, positions, inv_freq, grad.new_empty(grad.shape), *how)
         else:
             dx = _rope_below_autograd(grad, positions, inv_freq, *how)
         return dx, None, None, None, None, None
@@ -610,7 +610,7 @@ class rope_kv_append(CustomOp):
 
     def eager_execute(self, q, k_new, v_new, positions, inv_freq, k_cache, v_cache, slots, interleaved, scale):
         dev = launch._dev(q, k_new, v_new, positions, inv_freq, k_cache, v_cache, slots)
-        out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+        out = q.new_empty(q.shape)
         return launch._rope_kv_append(dev, q, k_new, v_new, positions, inv_freq, k_cache, v_cache, slots, out, interleaved, scale)
 
 
@@ -638,7 +638,7 @@ class flash_attn_varlen_fwd(CustomOp):
 
     def eager_execute(self, q, k, v, cu_seqlens_q, cu_seqlens_k, is_causal, scale):
         dev = launch._dev(q, k, v, cu_seqlens_q, cu_seqlens_k)
-        out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+        out = q.new_empty(q.shape)
         return launch._flash_attn_varlen_fwd(dev, q, k, v, cu_seqlens_q, cu_seqlens_k, out, is_causal, scale, True)
 
 
@@ -679,7 +679,7 @@ class paged_tree_attn(CustomOp):
         if num_kv_splits <= 0:
             num_kv_splits = default_num_tree_splits(block_table.size(1) * k_cache.size(1), q.size(0), q.size(1) * q.size(2) // k_cache.size(2), k_cache.size(2))
         dev = launch._dev(q, k_cache, v_cache, block_table, seq_lens, parents)
-        out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+        out = q.new_empty(q.shape)
         return launch._paged_tree_attn(dev, q, k_cache, v_cache, block_table, seq_lens, parents, out, scale, num_kv_splits, None, None)
 
 
