@@ -26,6 +26,7 @@ namespace mi355 {
 
 constexpr int PT_WAVES = 4;
 constexpr int PT_WAVE_LDS = 2 * 8192;  // two stages of 32 V rows
+constexpr int PT_ACC_ROW = 132;  // words per row of sums in the waves' merge: rows on the same banks took 1.4 us of a call
 constexpr int PT_MAX_GROUP = 128;  // query heads per kv head
 
 // bits 0 .. n - 1, at most four of them
@@ -259,7 +260,7 @@ __global__ __launch_bounds__(PT_WAVES * 64) __attribute__((amdgpu_waves_per_eu(2
   // ---- merge the four waves through LDS, one column group at a time ----
   float* sm = reinterpret_cast<float*>(lds);  // [wave][16]
   float* sl = sm + PT_WAVES * 16;
-  float* sacc = sl + PT_WAVES * 16;           // [wave][16][128]
+  float* sacc = sl + PT_WAVES * 16;           // [wave][16][PT_ACC_ROW]
 #pragma unroll
   for (int c = 0; c < C; c++) {
     float l = l_run[c] + __shfl_xor(l_run[c], 16);
@@ -270,29 +271,35 @@ __global__ __launch_bounds__(PT_WAVES * 64) __attribute__((amdgpu_waves_per_eu(2
       sl[wave * 16 + i16] = l;
     }
 #pragma unroll
-    for (int dt = 0; dt < 8; dt++) *reinterpret_cast<floatx4*>(sacc + ((wave * 16 + i16) * 128 + dt * 16 + 4 * g)) = oacc[c][dt];
+    for (int dt = 0; dt < 8; dt++) *reinterpret_cast<floatx4*>(sacc + ((wave * 16 + i16) * PT_ACC_ROW + dt * 16 + 4 * g)) = oacc[c][dt];
     __syncthreads();
-    for (int idx = threadIdx.x; idx < 16 * 128; idx += PT_WAVES * 64) {
-      const int col = idx >> 7, d = idx & 127, r = c * 16 + col;
+#pragma unroll
+    for (int idx = threadIdx.x; idx < 16 * 32; idx += PT_WAVES * 64) {  // 32 lanes of four columns per row
+      const int col = idx >> 5, d = (idx & 31) * 4, r = c * 16 + col;
       if (r >= R) continue;
       float m_tot = -INFINITY;
 #pragma unroll
       for (int w = 0; w < PT_WAVES; w++) m_tot = fmaxf(m_tot, sm[w * 16 + col]);
-      float acc = 0.f, lt = 0.f;
+      floatx4 acc = {0.f, 0.f, 0.f, 0.f};
+      float lt = 0.f;
 #pragma unroll
       for (int w = 0; w < PT_WAVES; w++) {
         // (no maximum: zeros, or a row of scores that are not numbers; either is passed on as it is)
         const float wgt = m_tot > -INFINITY ? __builtin_amdgcn_exp2f((sm[w * 16 + col] - m_tot) * a.scale_log2e) : 1.f;
-        acc += wgt * sacc[(w * 16 + col) * 128 + d];
-        lt += wgt * sl[w * 16 + col];
+        const floatx4 p = *reinterpret_cast<const floatx4*>(sacc + (w * 16 + col) * PT_ACC_ROW + d);
+#pragma unroll
+        for (int e = 0; e < 4; e++) acc[e] = __builtin_fmaf(wgt, p[e], acc[e]);
+        lt = __builtin_fmaf(wgt, sl[w * 16 + col], lt);
       }
       const int node = r / a.group;
       const size_t row = ((size_t)seq * a.nodes + node) * num_q_heads + kvh * a.group + (r - node * a.group);
       if (single) {
-        a.out[row * 128 + d] = cvt16<BF>(lt == 0.f ? 0.f : acc / lt);
+        const float inv = lt == 0.f ? 0.f : 1.f / lt;
+        const half4 v = {cvt16<BF>(acc[0] * inv), cvt16<BF>(acc[1] * inv), cvt16<BF>(acc[2] * inv), cvt16<BF>(acc[3] * inv)};
+        *reinterpret_cast<half4*>(a.out + row * 128 + d) = v;
       } else {
         const size_t at = row * a.num_splits + split;
-        a.part_acc[at * 128 + d] = acc;
+        *reinterpret_cast<floatx4*>(a.part_acc + at * 128 + d) = acc;
         if (d == 0) {
           a.part_ml[at * 2] = m_tot * a.scale_log2e;
           a.part_ml[at * 2 + 1] = lt;
@@ -366,7 +373,7 @@ template <int C, bool BF>
 static int launch_tree(const TreeArgs& a, int num_seqs, hipStream_t stream) {
   auto kern = paged_tree_kernel<C, BF>;
   constexpr int lds_bytes = PT_WAVES * PT_WAVE_LDS;
-  static_assert(lds_bytes >= (int)((2 * PT_WAVES * 16 + PT_WAVES * 16 * 128) * sizeof(float)), "merge area must fit");
+  static_assert(lds_bytes >= (int)((2 * PT_WAVES * 16 + PT_WAVES * 16 * PT_ACC_ROW) * sizeof(float)), "merge area must fit");
   static std::atomic<uint64_t> lds_ok{0};
   if (int rc = allow_lds(reinterpret_cast<const void*>(kern), lds_bytes, lds_ok, "paged_tree_kernel")) return rc;
   const int64_t wgs = (int64_t)num_seqs * a.num_splits * a.num_kv_heads;
