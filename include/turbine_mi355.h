@@ -175,16 +175,22 @@ int mi355_flash_attn_fwd_strided_bf16(const void* q, const void* k, const void* 
  * Rows of o outside every sequence are left as they are; with zero_rest != 0 those in front of the first and behind
  * the last sequence are set to zero.  total_q, total_k <= 2^24, total_q * H / Hkv <= 2^30, num_seqs <= 65535.
  * With the mask, keys and values that a query does not see do not reach it, whatever they hold (NaN and infinities too).
+ * Calls with few query rows and many keys cut the keys into chunks and join their results in a second launch: that takes the
+ * workspace that mi355_flash_attn_varlen_workspace_bytes names (0: none wanted), scratch that is written before it is read
+ * in the same call; without one, or with a smaller one, the call runs uncut.  16-byte aligned.
  * Replaces: the SDPA root of mi355_flash_attn_fwd for a ragged batch, which the reference can only pad
  * (tests/dynamo/llama_test.py:285-290 builds one rectangular mask).
  */
+int64_t mi355_flash_attn_varlen_workspace_bytes(int64_t num_seqs, int64_t total_q, int64_t total_k, int64_t H, int64_t Hkv,
+                                                int is_causal);
 int mi355_flash_attn_varlen_fwd(const void* q, const void* k, const void* v, void* o,
                                 const int32_t* cu_seqlens_q, const int32_t* cu_seqlens_k,
                                 int64_t num_seqs, int64_t total_q, int64_t total_k,
                                 int64_t H, int64_t Hkv, int64_t D,
                                 const int64_t* q_strides, const int64_t* k_strides,
                                 const int64_t* v_strides, const int64_t* o_strides,
-                                float scale, int is_causal, int zero_rest, int dtype, void* stream);
+                                float scale, int is_causal, int zero_rest, int dtype, void* workspace, int64_t workspace_bytes,
+                                void* stream);
 
 /*
  * Paged GQA decode attention, one query token per sequence.

@@ -88,9 +88,10 @@ _PROTOS = {
     "mi355_kv_cache_append": (c_int, [c_void_p] * 6 + [c_int64] * 7 + [c_void_p]),
     "mi355_paged_prefill_attn": (c_int, [c_void_p] * 6 + [c_int64] * 8 + [c_float, c_void_p]),
     "mi355_paged_prefill_attn_bf16": (c_int, [c_void_p] * 6 + [c_int64] * 8 + [c_float, c_void_p]),
+    "mi355_flash_attn_varlen_workspace_bytes": (c_int64, [c_int64] * 5 + [c_int]),
     "mi355_flash_attn_varlen_fwd": (
         c_int,
-        [c_void_p] * 6 + [c_int64] * 6 + [ctypes.POINTER(c_int64)] * 4 + [c_float, c_int, c_int, c_int, c_void_p],
+        [c_void_p] * 6 + [c_int64] * 6 + [ctypes.POINTER(c_int64)] * 4 + [c_float, c_int, c_int, c_int, c_void_p, c_int64, c_void_p],
     ),
     "mi355_paged_tree_attn": (c_int, [c_void_p] * 9 + [c_int64] * 9 + [c_float, c_int, c_void_p]),
     "mi355_verify_draft_workspace_bytes": (c_int64, [c_int64] * 3),

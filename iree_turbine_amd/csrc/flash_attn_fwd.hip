@@ -593,7 +593,22 @@ struct FaVarlen {
   int zero_rest;           // also write zeros to the query rows in front of the first and behind the last sequence
   int pairs;               // (causal) a unit is a pair of query blocks, else one block
   int ranked;              // hand out the units of the sequence with the most keys first (up to 64 sequences)
+  int chunks;              // a block's keys are cut into up to so many chunks, a workgroup each (1: they are not)
+  float *part_acc, *part_ml;  // (chunks > 1) [total_q][query heads][chunks][128], [..][2]
 };
+
+// How the key tiles of one block of query rows are cut: `count` chunks of `tiles` each (the last may have fewer), none
+// shorter than FA_MIN_CHUNK but by that.  The workgroups and the kernel that joins their results agree on it.
+constexpr int FA_MIN_CHUNK = 4, FA_MAX_CHUNKS = 16;
+struct FaChunks { int count, tiles; };
+__device__ __forceinline__ FaChunks fa_chunks(int n_tiles, int most) {
+  int c = (n_tiles + FA_MIN_CHUNK - 1) / FA_MIN_CHUNK;
+  c = c < 1 ? 1 : (c > most ? most : c);
+  FaChunks ch;
+  ch.tiles = (n_tiles + c - 1) / c;
+  ch.count = n_tiles > 0 ? (n_tiles + ch.tiles - 1) / ch.tiles : 1;
+  return ch;
+}
 
 // Rows [begin, begin + len) of sequence s; offsets outside the stream are cut to it, a negative length counts as 0.
 __device__ __forceinline__ int fa_seq_range(const int* cu, int s, int total, int& begin) {
@@ -659,9 +674,9 @@ struct FaTree : FaPaged {
   int nodes, num_kv_heads, num_seqs, row_blocks, num_splits, chunk_tiles;
 };
 
-enum class FaForm { PLAIN, PAGED, VARLEN, TREE };
+enum class FaForm { PLAIN, PAGED, VARLEN, CHUNKED, TREE };  // CHUNKED: VARLEN with keys cut into chunks
 template <FaForm F>
-using FaFormArgs = std::conditional_t<F == FaForm::VARLEN, FaVarlen, std::conditional_t<F == FaForm::TREE, FaTree, FaPaged>>;
+using FaFormArgs = std::conditional_t<F == FaForm::VARLEN || F == FaForm::CHUNKED, FaVarlen, std::conditional_t<F == FaForm::TREE, FaTree, FaPaged>>;
 
 // The pipelined form on v_mfma_f32_16x16x32 (variant "..._m16").  Same tiles, rings, loads, passes and barriers as
 // fa_fwd_d128_pipe; what changes is the MFMA shape and with it every fragment layout.  On benchmark-like data a
@@ -688,7 +703,7 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
     const half_t* __restrict__ Q, const half_t* __restrict__ K, const half_t* __restrict__ V, half_t* __restrict__ O, int BH,
     int Sq_arg, int Sk_arg, float scale_log2e, int q_blocks_arg, FaLayout lay, FaFormArgs<FORM> pg) {
   extern __shared__ __attribute__((aligned(1024))) char lds[];
-  constexpr bool VARLEN = FORM == FaForm::VARLEN, TREE = FORM == FaForm::TREE, PAGED = FORM == FaForm::PAGED || TREE;
+  constexpr bool VARLEN = FORM == FaForm::VARLEN || FORM == FaForm::CHUNKED, TREE = FORM == FaForm::TREE, PAGED = FORM == FaForm::PAGED || TREE;
   static_assert(NW == 4 || !PAGED, "the paged form maps one page to one wave-load of a 4-wave workgroup");
   static_assert(!TREE || !CAUSAL, "the tree form masks by ancestors");
   // EXACT: the query fragments are the operand's own bits and scores are scaled in 32 bits, one multiplication per score;
@@ -698,6 +713,8 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
   // be NaN, so tiles with masked keys are looked over first (clean_v).  That costs 1 us of 26 for 32 short prompts, 0.6 % for
   // long ones and 3 % for trees of 64 rows.
   constexpr bool CLEAN = (VARLEN && CAUSAL) || TREE;
+  // CHUNKS: the keys may be cut into chunks, each for a workgroup of its own.
+  constexpr bool CHUNKS = TREE || FORM == FaForm::CHUNKED;
   constexpr int WAVE_M = QG * 16, BLOCK_M = NW * WAVE_M, NI = 16 / NW;
   constexpr int TILE_B = FA_BLOCK_N * 256, VBUF = 2 * TILE_B;
   const int lane = threadIdx.x & 63;
@@ -709,7 +726,7 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
   int bh, unit, b_idx, h_idx;
   size_t q_first = 0, k_first = 0;  // (VARLEN) the sequence's first rows
   int seq_q = 0;                    // (VARLEN) its query tokens; Sq counts rows
-  int split = 0, first_tile = 0;    // (TREE) the chunk of the keys, and where it begins
+  int split = 0, first_tile = 0;    // (CHUNKS) the chunk of the keys, and where it begins
   if constexpr (VARLEN) {
     const int pid = blockIdx.x;
     if (pg.zero_rest) {
@@ -728,10 +745,16 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
     const int kv_heads = lay.H / lay.group;
     const bool spread = kv_heads % 8 == 0;
     FaUnit u;
-    if (!fa_find_unit(pg, lay.group, BLOCK_M, spread ? kv_heads / 8 : kv_heads, spread ? pid >> 3 : pid, u)) return;
+    int per_unit = spread ? kv_heads / 8 : kv_heads;
+    if constexpr (CHUNKS) per_unit *= pg.chunks;
+    if (!fa_find_unit(pg, lay.group, BLOCK_M, per_unit, spread ? pid >> 3 : pid, u)) return;
     units = u.units;
-    const int kv = u.inside / units;
+    int kv = u.inside / units;
     unit = u.inside - kv * units;
+    if constexpr (CHUNKS) {
+      split = kv % pg.chunks;
+      kv /= pg.chunks;
+    }
     h_idx = (spread ? kv * 8 + (pid & 7) : kv) * lay.group;
     q_first = u.q_first, k_first = u.k_first;
     Sq = u.q_len * lay.group;
@@ -790,7 +813,7 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
     const int cap = (pg.max_pages * 16) << pg.page_shift;
     Sk = Sk < 0 ? 0 : (Sk > cap ? cap : Sk);
   }
-  bool single = true;  // (TREE) the sequence fits one chunk
+  bool single = true;  // (CHUNKS) there is one chunk only
   int draft0 = 0;      // (TREE) position of node 0
   if constexpr (TREE) {
     draft0 = Sk - pg.nodes;
@@ -872,6 +895,13 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
   if constexpr (TREE) {
     n_tiles -= first_tile;
     n_tiles = n_tiles < pg.chunk_tiles ? n_tiles : pg.chunk_tiles;
+  } else if constexpr (CHUNKS) {
+    const FaChunks ch = fa_chunks(n_tiles, pg.chunks);
+    if (split >= ch.count) return;
+    single = ch.count == 1;
+    first_tile = split * ch.tiles;
+    n_tiles -= first_tile;
+    n_tiles = n_tiles < ch.tiles ? n_tiles : ch.tiles;
   }
 
   // Q fragments [query group][step over d], scale . log2(e) folded in and rounded to the 16-bit format again
@@ -948,7 +978,7 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
 
   // the j-th key tile that this workgroup walks
   auto tile_at = [&](int j) -> int {
-    if constexpr (TREE) return first_tile + j;
+    if constexpr (CHUNKS) return first_tile + j;
     else return j;
   };
   floatx4 oacc[8][QG];  // [d group][query group]
@@ -1290,9 +1320,9 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
     if (j + 1 < n_tiles) trip(std::integral_constant<int, 1>{}, j + 1, sb, sa);
   }
 
-  if (TREE && !single) {
+  if (CHUNKS && !single) {
     // partial results of the chunk: the unnormalised sums, their maximum in log2 units and weight
-    if constexpr (TREE) {
+    if constexpr (CHUNKS) {
       const int el = opaque_lane_id(), e16 = el & 15, eg = el >> 4;
 #pragma unroll
       for (int qg = 0; qg < QG; qg++) {
@@ -1300,8 +1330,10 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
         l_tot += __shfl_xor(l_tot, 32);
         const int r = wq0 + qg * 16 + e16;
         if (r < Sq) {
-          const int node = r / lay.group;
-          const size_t at = (((size_t)b_idx * pg.nodes + node) * lay.H + h_idx + (r - node * lay.group)) * pg.num_splits + split;
+          const int tok = token_of(r);  // or node
+          size_t at;
+          if constexpr (TREE) at = (((size_t)b_idx * pg.nodes + tok) * lay.H + h_idx + (r - tok * lay.group)) * pg.num_splits + split;
+          else at = ((q_first + tok) * lay.H + h_idx + (r - tok * lay.group)) * pg.chunks + split;
           float* acc = pg.part_acc + at * 128 + 4 * eg;
 #pragma unroll
           for (int dg = 0; dg < 8; dg++) *reinterpret_cast<floatx4*>(acc + dg * 16) = oacc[dg][qg];
@@ -1341,6 +1373,62 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
     if (CAUSAL) __syncthreads();  // the next pass loads K / V tiles over these regions
   }
   }  // pass
+}
+
+// Joins the chunks of packed sequences' rows (up to 64 sequences): 32 lanes of 16 bytes per row, two rows per wave.  Rows of
+// one chunk were written by the attention kernel, rows outside every sequence are left alone.
+template <bool BF>
+__global__ __launch_bounds__(256) void fa_varlen_join(FaVarlen vl, FaLayout lay, half_t* __restrict__ O, int causal) {
+  const int lane = threadIdx.x & 63, l32 = lane & 31;
+  const long long rows = (long long)vl.total_q * lay.H;
+  const long long first = ((long long)blockIdx.x * 4 + (threadIdx.x >> 6)) * 2;  // the wave's rows: this one and the next
+  int qf = 0, ql = 0, kf = 0, kl = 0;
+  if (lane < vl.num_seqs) {
+    ql = fa_seq_range(vl.cu_q, lane, vl.total_q, qf);
+    kl = fa_seq_range(vl.cu_k, lane, vl.total_k, kf);
+  }
+  int seq = -1, tok = 0, head = 0;
+#pragma unroll
+  for (int h = 0; h < 2; h++) {
+    const long long r = first + h < rows ? first + h : rows - 1;
+    const int t = (int)(r / lay.H);
+    const unsigned long long hit = __builtin_amdgcn_ballot_w64(qf <= t && t < qf + ql);
+    if ((lane >> 5) == h) {
+      seq = first + h < rows && hit ? __builtin_ctzll(hit) : -1;
+      tok = t;
+      head = (int)(r - (long long)t * lay.H);
+    }
+  }
+  const int from = seq < 0 ? 0 : seq;
+  const int q_first = __shfl(qf, from), q_len = __shfl(ql, from), k_len = __shfl(kl, from);
+  if (seq < 0) return;
+  // the row's block, its key tiles and their chunks, as in the attention kernel
+  const int row = (tok - q_first) * lay.group + head % lay.group;
+  int last = row / 64 * 64 + 63;
+  last = last < q_len * lay.group ? last : q_len * lay.group - 1;
+  int k_end = causal ? last / lay.group + (k_len - q_len) + 1 : k_len;
+  k_end = k_end < k_len ? k_end : k_len;
+  const int n = fa_chunks(k_end > 0 ? (k_end + FA_BLOCK_N - 1) / FA_BLOCK_N : 0, vl.chunks).count;
+  if (n == 1) return;
+  const size_t at = ((size_t)tok * lay.H + head) * vl.chunks;
+  const float* ml = vl.part_ml + at * 2;
+  const float* acc = vl.part_acc + at * 128 + l32 * 4;
+  float m_tot = -INFINITY;
+  for (int c = 0; c < n; c++) m_tot = fmaxf(m_tot, ml[2 * c]);
+  floatx4 o = {0.f, 0.f, 0.f, 0.f};
+  float l = 0.f;
+#pragma unroll 4
+  for (int c = 0; c < n; c++) {
+    // (no maximum: zeros, or a row of scores that are not numbers; either is passed on as it is)
+    const float w = m_tot > -INFINITY ? __builtin_amdgcn_exp2f(ml[2 * c] - m_tot) : 1.f;
+    const floatx4 p = *reinterpret_cast<const floatx4*>(acc + (size_t)c * 128);
+    l = __builtin_fmaf(w, ml[2 * c + 1], l);
+#pragma unroll
+    for (int e = 0; e < 4; e++) o[e] = __builtin_fmaf(w, p[e], o[e]);
+  }
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  const half4 v = {cvt16<BF>(o[0] * inv), cvt16<BF>(o[1] * inv), cvt16<BF>(o[2] * inv), cvt16<BF>(o[3] * inv)};
+  *reinterpret_cast<half4*>(O + (size_t)tok * lay.o_r + (size_t)head * lay.o_h + l32 * 4) = v;
 }
 
 // Persistent form of fa_fwd_d128_pipe ("walk"): one workgroup per CU slot runs its passes (a pass = one block of
@@ -2011,11 +2099,46 @@ int fa_tree(const TreeArgs& a, int num_seqs, bool bf16, hipStream_t stream) {
 
 }  // namespace mi355
 
+// How a packed call is laid out.  The lengths are known on the device only; sizes are what decides.
+struct FaVarlenPlan { int qg, pairs, ranked, chunks; };
+static FaVarlenPlan fa_varlen_plan(int64_t num_seqs, int64_t total_q, int64_t total_k, int64_t H, int64_t Hkv, int is_causal) {
+  FaVarlenPlan p;
+  const int64_t rows = total_q * (H / Hkv), blocks = rows / FA_BLOCK_M * Hkv;
+  // With the mask, a pair of blocks (the i-th from the end and the i-th from the start) is the same work everywhere in a sequence,
+  // and half as many workgroups; where even single blocks would not fill the chip twice (512 workgroups are resident), they
+  // are handed out singly.
+  p.pairs = is_causal && blocks >= 2048;
+  // Blocks of 64 rows where those of 128 would not fill the chip: twice the workgroups, each with half the work per key tile.
+  // One prompt of 1024 tokens (32 query heads over 8) 23 against 29 us, 32 of 16 tokens 8.0 against 9.7; where the chip
+  // is full the 64-row blocks are bound by LDS reads: 8 prompts of 256 tokens 22 against 20, one of 4096 164 against 134.
+  p.qg = blocks < 512 ? 1 : 2;
+  // Ranking costs every workgroup some 20 ns per sequence: worth it where sequences are long or few.
+  p.ranked = num_seqs > 1 && num_seqs <= 64 && total_k / num_seqs >= 16 * num_seqs;
+  // Few blocks that walk many keys: the number of chunks whose estimate is the smallest, in us: 3.5 for a workgroup and 0.85 for
+  // each of its key tiles, twice and more where there are more workgroups than the 512 resident ones; and for the
+  // joining 4 and the partial results written and read at 3.5 TB/s.  One to four sequences of 8192 keys and up to 128 new
+  // tokens 116-134 us without, 20-92 with; 4 x 128 tokens in front of 1024 keys (16 query heads over 1) 20 without, 25 with 4.
+  p.chunks = 1;
+  if (p.qg == 1 && num_seqs <= 64) {
+    const double full = (double)(rows / 64 + num_seqs) * Hkv / 512, tiles = (double)total_k / num_seqs / FA_BLOCK_N;
+    double best = 0;
+    for (int c = 1; c <= FA_MAX_CHUNKS; c++) {
+      if (c > 1 && tiles < FA_MIN_CHUNK * c) break;
+      const double t = (full * c > 1 ? full * c : 1.0) * (3.5 + 0.85 * tiles / c) + (c > 1 ? 4 + (double)total_q * H * c * 1040 / 3.5e6 : 0.0);
+      if (c == 1 || t < best) best = t, p.chunks = c;
+    }
+  }
+  return p;
+}
+static int64_t fa_varlen_scratch(const FaVarlenPlan& p, int64_t total_q, int64_t H) {
+  return p.chunks == 1 ? 0 : total_q * H * p.chunks * (128 + 2) * (int64_t)sizeof(float);
+}
+
 template <bool BF>
 static int fa_varlen(const void* q, const void* k, const void* v, void* o, const int32_t* cu_q, const int32_t* cu_k, int64_t num_seqs,
                      int64_t total_q, int64_t total_k, int64_t H, int64_t Hkv, int64_t D, const int64_t* q_strides,
                      const int64_t* k_strides, const int64_t* v_strides, const int64_t* o_strides, float scale, int is_causal,
-                     int zero_rest, void* stream) {
+                     int zero_rest, void* workspace, int64_t workspace_bytes, void* stream) {
   const char* who = BF ? "flash_attn_varlen_fwd_bf16" : "flash_attn_varlen_fwd";
   if (!q || !k || !v || !o || !cu_q || !cu_k || !q_strides || !k_strides || !v_strides || !o_strides)
     return fail(-MI355_E_NULL, "%s: null pointer", who);
@@ -2049,42 +2172,52 @@ static int fa_varlen(const void* q, const void* k, const void* v, void* o, const
   int group_shift = -1;
   for (int sh = 0; sh < 16; sh++)
     if (group == (1ll << sh)) group_shift = sh;
-  // With the mask, a pair of blocks (the i-th from the end and the i-th from the start) is the same work everywhere in a sequence,
-  // and half as many workgroups; where even single blocks would not fill the chip twice (512 workgroups are resident), they
-  // are handed out singly.
-  const int64_t blocks = rows / FA_BLOCK_M * Hkv;
-  const int pairs = is_causal && blocks >= 2048;
-  // Blocks of 64 rows where those of 128 would not fill the chip: twice the workgroups, each with half the work per key tile.
-  // One prompt of 1024 tokens (32 query heads over 8) 23 against 29 us, 32 of 16 tokens 8.0 against 9.7; where the chip
-  // is full the 64-row blocks are bound by LDS reads: 8 prompts of 256 tokens 22 against 20, one of 4096 164 against 134.
-  const int qg = blocks < 512 ? 1 : 2, block_m = 64 * qg;
-  // Ranking costs every workgroup some 20 ns per sequence: worth it where sequences are long or few.
-  const int ranked = num_seqs > 1 && num_seqs <= 64 && total_k / num_seqs >= 16 * num_seqs;
-  const FaVarlen vl{cu_q, cu_k, (int)num_seqs, (int)total_q, (int)total_k, group_shift, zero_rest, pairs, ranked};
+  FaVarlenPlan plan = fa_varlen_plan(num_seqs, total_q, total_k, H, Hkv, is_causal);
+  if (!workspace || workspace_bytes < fa_varlen_scratch(plan, total_q, H)) plan.chunks = 1;
+  if (plan.chunks > 1 && !aligned16(workspace)) return fail(-MI355_E_ALIGN, "%s: workspace must be 16-byte aligned", who);
+  const int qg = plan.qg, block_m = 64 * qg;
+  float* part = plan.chunks > 1 ? (float*)workspace : nullptr;
+  const FaVarlen vl{cu_q, cu_k, (int)num_seqs, (int)total_q, (int)total_k, group_shift, zero_rest, plan.pairs, plan.ranked, plan.chunks, part,
+                    part ? part + total_q * H * plan.chunks * 128 : nullptr};
   // the lengths are known on the device only: as many units as num_seqs sequences of total_q tokens can have
-  const int64_t units = rows / (block_m << pairs) + num_seqs;
-  if (units * Hkv >= (1ll << 24)) return fail(-MI355_E_SHAPE, "%s: too many query blocks", who);  // 2^32 threads
-  auto kern = qg == 1 ? (is_causal ? fa_fwd_d128_m16<true, BF, 4, false, FaForm::VARLEN, 1> : fa_fwd_d128_m16<false, BF, 4, false, FaForm::VARLEN, 1>)
-                      : (is_causal ? fa_fwd_d128_m16<true, BF, 4, false, FaForm::VARLEN, 2> : fa_fwd_d128_m16<false, BF, 4, false, FaForm::VARLEN, 2>);
+  const int64_t units = rows / (block_m << plan.pairs) + num_seqs;
+  if (units * Hkv * plan.chunks >= (1ll << 24)) return fail(-MI355_E_SHAPE, "%s: too many query blocks", who);  // 2^32 threads
+  const bool cut = plan.chunks > 1;
+  auto kern = cut       ? (is_causal ? fa_fwd_d128_m16<true, BF, 4, false, FaForm::CHUNKED, 1> : fa_fwd_d128_m16<false, BF, 4, false, FaForm::CHUNKED, 1>)
+              : qg == 1 ? (is_causal ? fa_fwd_d128_m16<true, BF, 4, false, FaForm::VARLEN, 1> : fa_fwd_d128_m16<false, BF, 4, false, FaForm::VARLEN, 1>)
+                        : (is_causal ? fa_fwd_d128_m16<true, BF, 4, false, FaForm::VARLEN, 2> : fa_fwd_d128_m16<false, BF, 4, false, FaForm::VARLEN, 2>);
   const int lds_bytes = 2 * FA_STAGE + 16;
-  static std::atomic<uint64_t> lds_ok[4] = {};
-  if (int rc = allow_lds(reinterpret_cast<const void*>(kern), lds_bytes, lds_ok[(is_causal ? 1 : 0) + 2 * (qg - 1)], "fa_fwd_d128_m16<varlen>")) return rc;
-  dim3 grid((unsigned)(units * Hkv)), block(256);
-  hipLaunchKernelGGL(kern, grid, block, lds_bytes, reinterpret_cast<hipStream_t>(stream), (const half_t*)q, (const half_t*)k,
-                     (const half_t*)v, (half_t*)o, (int)H, 0, 0, scale * 1.4426950408889634f, 0, lay, vl);
-  return check_launch("fa_fwd_d128_m16<varlen>", grid, block, lds_bytes);
+  static std::atomic<uint64_t> lds_ok[6] = {};
+  if (int rc = allow_lds(reinterpret_cast<const void*>(kern), lds_bytes, lds_ok[(is_causal ? 1 : 0) + 2 * (cut ? 2 : qg - 1)], "fa_fwd_d128_m16<varlen>")) return rc;
+  dim3 grid((unsigned)(units * Hkv * plan.chunks)), block(256);
+  hipStream_t on = reinterpret_cast<hipStream_t>(stream);
+  hipLaunchKernelGGL(kern, grid, block, lds_bytes, on, (const half_t*)q, (const half_t*)k, (const half_t*)v, (half_t*)o, (int)H, 0, 0,
+                     scale * 1.4426950408889634f, 0, lay, vl);
+  int rc = check_launch("fa_fwd_d128_m16<varlen>", grid, block, lds_bytes);
+  if (rc || !cut) return rc;
+  dim3 join((unsigned)((total_q * H + 7) / 8));
+  hipLaunchKernelGGL(fa_varlen_join<BF>, join, block, 0, on, vl, lay, (half_t*)o, is_causal);
+  return check_launch("fa_varlen_join", join, block, 0);
+}
+
+extern "C" int64_t mi355_flash_attn_varlen_workspace_bytes(int64_t num_seqs, int64_t total_q, int64_t total_k, int64_t H, int64_t Hkv,
+                                                          int is_causal) {
+  if (num_seqs <= 0 || num_seqs > 65535 || total_q <= 0 || total_k <= 0 || total_q > (1 << 24) || total_k > (1 << 24) || H <= 0 ||
+      H > 65535 || Hkv <= 0 || H % Hkv != 0)
+    return 0;
+  return fa_varlen_scratch(fa_varlen_plan(num_seqs, total_q, total_k, H, Hkv, is_causal), total_q, H);
 }
 
 extern "C" int mi355_flash_attn_varlen_fwd(const void* q, const void* k, const void* v, void* o, const int32_t* cu_seqlens_q,
                                            const int32_t* cu_seqlens_k, int64_t num_seqs, int64_t total_q, int64_t total_k, int64_t H,
                                            int64_t Hkv, int64_t D, const int64_t* q_strides, const int64_t* k_strides,
                                            const int64_t* v_strides, const int64_t* o_strides, float scale, int is_causal,
-                                           int zero_rest, int dtype, void* stream) {
+                                           int zero_rest, int dtype, void* workspace, int64_t workspace_bytes, void* stream) {
   if (dtype == MI355_BF16)
     return fa_varlen<true>(q, k, v, o, cu_seqlens_q, cu_seqlens_k, num_seqs, total_q, total_k, H, Hkv, D, q_strides, k_strides, v_strides,
-                           o_strides, scale, is_causal, zero_rest, stream);
+                           o_strides, scale, is_causal, zero_rest, workspace, workspace_bytes, stream);
   if (dtype == MI355_F16)
     return fa_varlen<false>(q, k, v, o, cu_seqlens_q, cu_seqlens_k, num_seqs, total_q, total_k, H, Hkv, D, q_strides, k_strides, v_strides,
-                            o_strides, scale, is_causal, zero_rest, stream);
+                            o_strides, scale, is_causal, zero_rest, workspace, workspace_bytes, stream);
   return fail(-MI355_E_DTYPE, "flash_attn_varlen_fwd: dtype %d (MI355_F16 or MI355_BF16)", dtype);
 }

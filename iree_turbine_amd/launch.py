@@ -358,11 +358,16 @@ def _flash_attn_varlen_fwd(dev, q, k, v, cu_q, cu_k, o, is_causal, scale, zero_r
     if os_ is None or (o.size(1) > 1 and os_[1] == 0):
         raise ValueError(f"{op}: output rows must be contiguous, 16-byte aligned and not overlapping")
     cu_q, cu_k = cu_q.contiguous(), cu_k.contiguous()
+    lib = _lib.load()
+    S, (Tq, H, _), (Tk, Hkv, _) = cu_q.size(0) - 1, q.shape, k.shape
+    ws_bytes = lib.mi355_flash_attn_varlen_workspace_bytes(S, Tq, Tk, H, Hkv, is_causal)
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes else None
     with _on(dev):
-        rc = _lib.load().mi355_flash_attn_varlen_fwd(
-            q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), cu_q.data_ptr(), cu_k.data_ptr(), cu_q.size(0) - 1, q.size(0),
-            k.size(0), q.size(1), k.size(1), 128, _Strides(*qs), _Strides(*ks), _Strides(*vs), _Strides(*os_),
-            _default_scale(scale, 128), is_causal, zero_rest, _lib.dtype_code(q.dtype), _lib.raw_stream(dev))
+        rc = lib.mi355_flash_attn_varlen_fwd(
+            q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), cu_q.data_ptr(), cu_k.data_ptr(), S, Tq,
+            Tk, H, Hkv, 128, _Strides(*qs), _Strides(*ks), _Strides(*vs), _Strides(*os_),
+            _default_scale(scale, 128), is_causal, zero_rest, _lib.dtype_code(q.dtype), ws.data_ptr() if ws_bytes else None, ws_bytes,
+            _lib.raw_stream(dev))
     if rc:
         _lib.check(rc, f"{op} {q.dtype} q={tuple(q.shape)} k={tuple(k.shape)} seqs={cu_q.shape[0] - 1} causal={is_causal}")
     return o

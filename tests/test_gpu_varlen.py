@@ -1,5 +1,7 @@
 """GPU parity: attention over packed sequences against the 64-bit oracle, within the bound that it derives."""
 
+import ctypes
+
 import pytest
 import torch
 
@@ -58,6 +60,75 @@ def test_keys_in_front_and_missing(dev, dtype, causal):
 def test_head_layouts(dev, hq, hkv):
     announce(f"varlen hq={hq} hkv={hkv}")
     _run(dev, [100, 1, 40, 190], [100, 1, 40, 190], hq, hkv, True, torch.float16)
+
+
+CUT = [([1], [4000], 4, 1), ([1, 1, 1], [1500, 2, 2600], 16, 2), ([33, 0, 7, 64], [1900, 300, 0, 1300], 16, 1), ([130], [2500], 8, 8),
+       ([5, 16, 2, 40, 9], [900, 1033, 1024, 1088, 640], 5, 1), ([1100, 3], [1100, 1600], 8, 2), ([300], [200], 2, 2), ([700, 600], [700, 600], 3, 3), ([20] * 64, [600] * 64, 4, 1)]
+
+
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("lq,lk,hq,hkv", CUT, ids=lambda x: str(x)[:30])
+def test_keys_cut_into_chunks(dev, lq, lk, hq, hkv, dtype, causal):
+    """Few query rows and many keys: every block's keys in up to 16 chunks, joined; the same bits on every call, rows outside
+    left alone, and without a workspace the uncut call within the rounding."""
+    from iree_turbine_amd import _lib, launch
+    from oracle import serving
+
+    announce(f"varlen chunks lq={lq[:5]} lk={lk[:5]} hq={hq} {dtype} causal={causal}")
+    T, Tk = sum(lq) + 5, sum(lk) + 3
+    lib = _lib.load()
+    assert (lib.mi355_flash_attn_varlen_workspace_bytes(len(lq), T, Tk, hq, hkv, causal) > 0) == (lk not in ([200], [700, 600], [600] * 64))
+    q, k, v = (torch.randn(t, h, 128).to(dtype) for t, h in ((T, hq), (Tk, hkv), (Tk, hkv)))
+    cq, ck = _cu(lq, first=2), _cu(lk, first=1)
+    k[int(ck[-1]):], v[int(ck[-1]):], k[0], v[0] = float("nan"), float("inf"), float("inf"), float("nan")
+    args = [t.to(dev) for t in (q, k, v, cq, ck)]
+    want, bound = serving.varlen_ref(q, torch.nan_to_num(k, 0.0, 0.0, 0.0), torch.nan_to_num(v, 0.0, 0.0, 0.0), cq, ck, causal)
+    got = torch.ops.mi355.flash_attn_varlen_fwd(*args, causal, 0.0)
+    _inside(got, want, bound)
+    o = torch.full((T, 2 * hq, 128), 7.0, dtype=dtype, device=dev)
+    launch.flash_attn_varlen_fwd_out(*args, o[:, hq:], causal, 0.0)
+    inside = slice(int(cq[0]), int(cq[-1]))
+    assert torch.equal(o[inside, hq:], got[inside])
+    o[inside, hq:] = 7.0
+    assert torch.equal(o, torch.full_like(o, 7.0))
+    st = lambda t: (ctypes.c_int64 * 2)(t.stride(0), t.stride(1))
+    plain = torch.zeros_like(got)
+    rc = lib.mi355_flash_attn_varlen_fwd(*(t.data_ptr() for t in (*args[:3], plain, *args[3:])), len(lq), T, Tk, hq, hkv, 128, *(st(t) for t in (*args[:3], plain)),
+                                         128**-0.5, causal, 0, _lib.dtype_code(dtype), None, 0, _lib.raw_stream(dev))
+    assert rc == 0
+    _inside(plain, want, bound)
+
+
+def test_chunks_on_two_streams_and_captured(dev):
+    """Calls at once and two captured ones keep scratch of their own."""
+    announce("varlen chunks streams and capture")
+    q, k, v = (torch.randn(t, h, 128).half().to(dev) for t, h in ((40, 8), (6000, 2), (6000, 2)))
+    cq, ck = _cu([30, 2, 8]).to(dev), _cu([3000, 2000, 1000]).to(dev)
+    call = lambda: torch.ops.mi355.flash_attn_varlen_fwd(q, k, v, cq, ck, True, 0.0)
+    want = call()
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(dev) for _ in range(2)]
+    outs, graphs = [], []
+    for s in streams:
+        with torch.cuda.stream(s):
+            outs += [call() for _ in range(5)]
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, want) for o in outs)
+    for _ in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = call()
+        graphs.append((g, out))
+    for lens in ([3000, 2000, 1000], [0, 4000, 2000], [100, 5000, 64]):
+        ck.copy_(_cu(lens))
+        torch.cuda.synchronize()
+        for s, (g, _) in zip(streams, graphs):
+            with torch.cuda.stream(s):
+                g.replay()
+        torch.cuda.synchronize()
+        eager = call()
+        assert all(torch.equal(out, eager) for _, out in graphs)
 
 
 @pytest.mark.parametrize("S", [63, 64, 65, 130, 300])

@@ -166,10 +166,14 @@ def test_c_entries_refuse_bad_arguments_without_a_gpu():
     lib = _lib.load()
     st = strides(512, 128)
     va = lambda **c: lib.mi355_flash_attn_varlen_fwd(*{**dict(q=16, k=16, v=16, o=16, cq=16, ck=16, S=2, tq=9, tk=9, H=4, Hkv=2, D=128, qs=st, ks=st, vs=st, os=st,
-                                                              scale=1.0, causal=1, zero=0, dtype=1, stream=None), **c}.values())
+                                                              scale=1.0, causal=1, zero=0, dtype=1, ws=None, wb=0, stream=None), **c}.values())
     assert va(q=None) == -1 and va(D=64) == -2 and va(o=24) == -3 and va(dtype=0) == -4 and va(S=0) == -2 and va(Hkv=3) == -2
     assert va(qs=strides(513, 128)) == -3 and va(ks=strides(64, 128)) == -2 and va(os=strides(512, 0)) == -2 and va(scale=math.nan) == -2
     assert va(tk=1 << 25) == -2
+    cut = lib.mi355_flash_attn_varlen_workspace_bytes
+    assert cut(4, 80, 6000, 16, 1, 1) > 0 and cut(4, 80, 200, 16, 1, 1) == 0 and cut(4, 8000, 8000, 32, 8, 1) == 0 and cut(65, 80, 60000, 16, 1, 1) == 0
+    assert cut(0, 80, 6000, 16, 1, 1) == 0 and cut(4, 80, 6000, 16, 3, 1) == 0
+    assert va(S=4, tq=80, tk=6000, H=16, Hkv=1, ws=24, wb=cut(4, 80, 6000, 16, 1, 1), qs=strides(2048, 128)) == -3
     ta = lambda **c: lib.mi355_paged_tree_attn(*{**dict(q=16, k=16, v=16, bt=16, sl=16, par=16, out=16, pa=None, pm=None, S=2, N=5, hq=8, hkv=2, D=128, page=16, mp=4,
                                                         P=9, splits=1, scale=1.0, dtype=1, stream=None), **c}.values())
     assert ta(par=None) == -1 and ta(N=65) == -2 and ta(splits=2) == -5 and ta(page=48) == -2 and ta(hq=9) == -2 and ta(dtype=0) == -4
