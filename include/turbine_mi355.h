@@ -438,8 +438,8 @@ int mi355_paged_batch_layout(int32_t* block_table, const int32_t* context_lens, 
  * x, out: [tokens, heads, D] of dtype (MI355_F16 | MI355_BF16 | MI355_F32); *_strides {token, head} in elements, the D elements
  * of a row contiguous; in place (out == x, same strides) is allowed.  positions: int32 [tokens].  inv_freq: fp64
  * (freq_is_f64 != 0) or fp32 [rotary_dim / 2].  Angles are formed in 64 bits, the products in 32, rounded once.
- * rotary_dim even, <= D and <= 1024; fewer than 2^24 tokens.  Rows on 16-byte borders with rotary_dim / 2 and D - rotary_dim multiples of 16
- * bytes' elements run with wide loads; others element by element.
+ * rotary_dim even, <= D and <= 1024; fewer than 2^24 tokens.  Rows on 16- or 8-byte borders whose rotated halves and
+ * rest are whole accesses of that size run with them; others element by element.
  * No counterpart among the reference's kernels.
  */
 int mi355_rope(const void* x, void* out, const int32_t* positions, const void* inv_freq, int freq_is_f64,

@@ -1,5 +1,6 @@
 """MI355X-native dense kernels (fp16 NT GEMM, flash-attention prefill, paged GQA decode attention,
-block-scaled MXFP4 GEMM) behind iree-turbine's operator surface.
+block-scaled MXFP4 GEMM, and the operators of a serving step around the paged cache: batch layout, rotary
+positions, packed and tree attention, draft verification) behind iree-turbine's operator surface.
 
 Importing the package registers `torch.ops.mi355.*`.  The kernels live in
 csrc/libturbine_mi355.so (hand-written HIP for gfx950); there is no other implementation.

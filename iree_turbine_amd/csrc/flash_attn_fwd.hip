@@ -674,6 +674,10 @@ struct FaTree : FaPaged {
   int nodes, num_kv_heads, num_seqs, row_blocks, num_splits, chunk_tiles;
 };
 
+// Measured, causal, the packed forms: 32 prompts of 1 to 300 tokens (32 query heads over 8) 26 us, bound by the
+// workgroups' fixed cost (offsets, query rows and first tiles, one after the other: a single prompt of 16 tokens takes 6.6 us,
+// an empty launch 3.6); 12 of 100 to 700 tokens behind up
+// to 1500 (16 heads over one) 41 us; 4 of 1500 to 8192 1.07 to 1.11 ms, 1.02 to 1.06 PFLOP/s, the rate of the rectangular form.
 enum class FaForm { PLAIN, PAGED, VARLEN, CHUNKED, TREE };  // CHUNKED: VARLEN with keys cut into chunks
 template <FaForm F>
 using FaFormArgs = std::conditional_t<F == FaForm::VARLEN || F == FaForm::CHUNKED, FaVarlen, std::conditional_t<F == FaForm::TREE, FaTree, FaPaged>>;

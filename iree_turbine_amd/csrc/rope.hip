@@ -8,7 +8,10 @@
 // [-1/2, 1/2] turns there, and only the remainder goes to 32 bits.  That costs R/2 short 64-bit computations per token,
 // shared by all its heads through LDS.  The rotation itself is done in 32 bits and rounded once.
 //
-// The op reads and writes every element once (HBM bound): 16 bytes per lane where rows allow it.
+// The op reads and writes every element once (HBM bound): 16 bytes per lane where rows allow it, 8 where only those fit
+// (16384 tokens x 8 heads of 80 elements, 40 of them turned: 37 us, 59 element by element), else one element.
+// Measured: 16384 tokens x 32 x 128 bf16 48 us (5.6 TB/s), 8000 tokens with the append 32 us of which a part comes out of the
+// memory-side cache (cold: 43 us, 4.6 TB/s), 64 tokens with the append 4 us (a launch and two trips to memory).
 #include "common.hpp"
 #include <math.h>
 #include <type_traits>
