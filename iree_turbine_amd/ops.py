@@ -544,12 +544,12 @@ class rope(CustomOp):
 
 def _on_device_eagerly(x: Tensor) -> bool:
     """A plain device tensor outside every dispatch mode: the launch needs no further pass through the dispatcher.  Meta
-    and fake tensors and tracing do."""
-    return type(x) in (Tensor, torch.nn.Parameter) and x.is_cuda and torch._C._len_torch_dispatch_stack() == 0
+    and fake tensors and tracing do, and lazily negated or zero ones, whose memory is not yet what they stand for."""
+    return type(x) in (Tensor, torch.nn.Parameter) and x.is_cuda and torch._C._len_torch_dispatch_stack() == 0 and not x.is_neg() and not x._is_zerotensor()
 
 
 def _rope_below_autograd(*args):
-    if _on_device_eagerly(args[0]):
+    if _on_device_eagerly(args[0]) and not args[2].is_neg():
         return _rope_on_device(*args)
     with torch._C._AutoDispatchBelowAutograd():
         return torch.ops.mi355.rope(*args)

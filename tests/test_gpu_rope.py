@@ -192,3 +192,28 @@ def test_rope_in_place_on_a_stream_and_captured(dev):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(z, torch.ops.mi355.rope(xd, pd, fd, False, False, 1.0))
+
+
+def test_lazily_negated_operands_and_gradients(dev):
+    """Tensors that carry torch's negation as a flag (the imaginary part of a conjugate) are read with their sign, and so are
+    the gradients that come back through one; a gradient of zeros that has no memory gives zeros."""
+    announce("rope of lazily negated tensors")
+    z = torch.randn(5, 2, 64, dtype=torch.complex64, device=dev)
+    x = z.conj().imag
+    assert x.is_neg()
+    pos, f = torch.arange(5, dtype=torch.int32, device=dev), _freq(64, device=dev)[0].float()
+    call = lambda t, g=f: torch.ops.mi355.rope(t, pos, g, False, False, 1.0)
+    want = call(x.resolve_neg().clone())
+    assert torch.equal(call(x), want)
+    neg_f = torch.complex(f, -f).conj().imag  # f again, negated twice
+    assert neg_f.is_neg() and torch.equal(call(x, neg_f), call(x.resolve_neg().clone(), neg_f.resolve_neg().clone()))
+    leaf = torch.randn(5, 2, 64, device=dev, requires_grad=True)
+    y = call(leaf)
+    g = torch.randn(5, 2, 64, dtype=torch.complex64, device=dev).conj().imag
+    assert torch.equal(torch.autograd.grad(y, leaf, g, retain_graph=True)[0], torch.autograd.grad(y, leaf, g.resolve_neg().clone(), retain_graph=True)[0])
+    zero = torch._efficientzerotensor((5, 2, 64), device=dev)
+    assert torch.equal(torch.autograd.grad(y, leaf, zero)[0], torch.zeros_like(leaf))
+    # x itself required to have a gradient while lazily negated
+    w = z.clone().requires_grad_()
+    v = w.conj().imag
+    torch.testing.assert_close(torch.autograd.grad(call(v), w, want)[0], torch.autograd.grad(call(-w.imag), w, want)[0], rtol=0, atol=0)
