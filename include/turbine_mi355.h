@@ -381,6 +381,9 @@ int mi355_paged_prefill_attn_bf16(const void* q, const void* k_cache, const void
  * read in the same call, and at most 2^23 query rows (num_seqs * num_nodes * num_q_heads).  No counterpart in the
  * reference; the mask generalises tests/dynamo/llama_test.py:285-290.
  */
+/* A default for num_splits, from sizes alone. */
+int64_t mi355_paged_tree_default_splits(int64_t num_seqs, int64_t num_nodes, int64_t num_q_heads, int64_t num_kv_heads,
+                                        int64_t page_size, int64_t max_pages_per_seq);
 int mi355_paged_tree_attn(const void* q, const void* k_cache, const void* v_cache,
                           const int32_t* block_table, const int32_t* seq_lens, const int32_t* parents, void* out,
                           float* part_acc, float* part_ml,

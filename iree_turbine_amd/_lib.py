@@ -10,6 +10,8 @@ The reference reaches HIP the same way, through ctypes on libamdhip64
 from __future__ import annotations
 
 import ctypes
+import importlib.machinery
+import importlib.util
 import threading
 from ctypes import c_char_p, c_float, c_int, c_int64, c_void_p
 from pathlib import Path
@@ -17,12 +19,14 @@ from pathlib import Path
 import torch  # noqa: F401  (must be imported first: it loads the HIP runtime this library links to)
 
 LIB_PATH = Path(__file__).resolve().parent / "csrc" / "libturbine_mi355.so"
+HOST_PATH = LIB_PATH.parent / "mi355_host_ops.so"
 
 F32, F16, BF16 = 0, 1, 2
 _DTYPE_CODE = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}
 
 _lock = threading.Lock()
 _lib = None
+_host = None
 
 _PROTOS = {
     "mi355_abi_version": (c_int, []),
@@ -93,6 +97,7 @@ _PROTOS = {
         c_int,
         [c_void_p] * 6 + [c_int64] * 6 + [ctypes.POINTER(c_int64)] * 4 + [c_float, c_int, c_int, c_int, c_void_p, c_int64, c_void_p],
     ),
+    "mi355_paged_tree_default_splits": (c_int64, [c_int64] * 6),
     "mi355_paged_tree_attn": (c_int, [c_void_p] * 9 + [c_int64] * 9 + [c_float, c_int, c_void_p]),
     "mi355_verify_draft_workspace_bytes": (c_int64, [c_int64] * 3),
     "mi355_verify_draft": (c_int, [c_void_p] * 8 + [c_int64] * 3 + [c_void_p, c_int64, c_void_p]),
@@ -153,6 +158,29 @@ def load():
             raise KernelLibraryError(f"ABI version mismatch: library reports {lib.mi355_abi_version()}, binding expects 1")
         _lib = lib
     return _lib
+
+
+# what csrc/host_ops.cpp calls, in its bind()'s order
+_HOST_ENTRIES = ("mi355_rope", "mi355_rope_kv_append", "mi355_paged_batch_layout", "mi355_flash_attn_varlen_fwd",
+                 "mi355_flash_attn_varlen_workspace_bytes", "mi355_paged_tree_attn", "mi355_paged_tree_default_splits", "mi355_verify_draft",
+                 "mi355_verify_draft_workspace_bytes", "mi355_last_error")
+
+
+def host_ops():
+    """The extension module with the host side of the serving operators, bound to the loaded kernel library's entries."""
+    global _host
+    if _host is not None:
+        return _host
+    lib = load()
+    with _lock:
+        if _host is None:
+            if not HOST_PATH.exists():
+                raise KernelLibraryError(f"{HOST_PATH} is missing: build it with `python -m iree_turbine_amd.build`")
+            loader = importlib.machinery.ExtensionFileLoader(HOST_PATH.stem, str(HOST_PATH))
+            host = importlib.util.module_from_spec(importlib.util.spec_from_loader(HOST_PATH.stem, loader))
+            host.bind(*(ctypes.cast(getattr(lib, name), c_void_p).value for name in _HOST_ENTRIES))
+            _host = host
+    return _host
 
 
 def build_flags() -> str:

@@ -16,6 +16,7 @@ from pathlib import Path
 CSRC = Path(__file__).resolve().parent / "csrc"
 LIB_NAME = "libturbine_mi355.so"
 LIB_PATH = CSRC / LIB_NAME
+HOST_PATH = CSRC / "mi355_host_ops.so"
 SOURCES = ["capi.hip", "gemm_f16_nt.hip", "flash_attn_fwd.hip", "paged_decode.hip", "gemm_mxfp4.hip", "gemm_mxfp8.hip", "gemm_mxfp6.hip", "quantize_mxfp4.hip", "quantize_mxfp6.hip", "paged_layout.hip", "rope.hip", "paged_tree.hip", "verify_draft.hip", "calibrate.hip"]
 
 # -packed-fp32-ops: keep the compiler from forming v_pk_{add,mul,fma}_f32.
@@ -131,6 +132,22 @@ def build_library(verbose: bool = True, save_temps: bool = False, defines: tuple
     return lib_path
 
 
+def build_host_ops(verbose: bool = True) -> Path:
+    """Compiles the extension module with the host side of the serving operators (host code only, against torch's headers)."""
+    import sysconfig
+
+    import torch
+
+    root = Path(torch.__file__).parent
+    _run([shutil.which("g++") or "g++", "-std=c++17", "-O2", "-Wall", "-fPIC", "-shared", "-fvisibility=hidden", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
+          "-isystem", str(root / "include"), "-isystem", str(root / "include/torch/csrc/api/include"), "-isystem", sysconfig.get_paths()["include"],
+          "-isystem", str(Path(_hipcc()).resolve().parent.parent / "include"), str(CSRC / "host_ops.cpp"), "-o", str(HOST_PATH), "-L" + str(root / "lib"),
+          "-ltorch", "-ltorch_cpu", "-ltorch_python", "-lc10", "-lc10_hip"])
+    if verbose:
+        print(f"built {HOST_PATH} ({HOST_PATH.stat().st_size} bytes)")
+    return HOST_PATH
+
+
 PROBES = ["lds_read_patterns.hip", "load_rate.hip", "mfma_load_bubble.hip", "hbm_read_patterns.hip"]
 
 
@@ -165,3 +182,5 @@ if __name__ == "__main__":
     if a.probes:
         build_probes()
     build_library(save_temps=a.save_temps, defines=tuple(a.defines), out=a.out)
+    if a.out is None:
+        build_host_ops()

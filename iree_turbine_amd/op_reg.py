@@ -25,6 +25,8 @@ from typing import Any, Callable, Optional, Sequence, Type, Union
 import torch
 from torch import Tensor
 
+from . import _lib
+
 _CONFIG_LOCK = threading.Lock()
 
 DEFINED_OP_NAMES: set[tuple[str, str]] = set()
@@ -218,6 +220,10 @@ class CustomOp(ABC):
     # a launch runs it in place of `select`, whose descriptors only the Meta kernel and a spec key need.
     check: Optional[Callable[..., None]] = None
 
+    # The op's function in csrc/host_ops.cpp, which does a plain call's checks, results and launch natively and returns None for any
+    # other: that one takes the way through `check` and `eager_execute`, which copy what has to be copied or raise.
+    host: Optional[str] = None
+
     def eager_execute(self, *args):
         return NotImplemented
 
@@ -258,4 +264,15 @@ def device_impl(op: CustomOp):
             raise NotImplementedError(f"{op.name}: no device implementation (eager_execute returned NotImplemented)")
         return result
 
-    return handler
+    if op.host is None:
+        return handler
+    call = None
+
+    def plain_first(*args):
+        nonlocal call
+        if call is None:
+            call = getattr(_lib.host_ops(), op.host)
+        result = call(*args)
+        return handler(*args) if result is None else result
+
+    return plain_first

@@ -15,7 +15,7 @@ from torch import Tensor
 
 from . import launch
 from .contract import PAGE_SIZES, check_mx_operand as _check_mx_operand, check_paged_args as _check_paged_args  # noqa: F401
-from . import contract, op_reg
+from . import _lib, contract, op_reg
 from .contract import require as _require
 from .op_reg import CustomOp, KernelSelection
 
@@ -465,6 +465,7 @@ class paged_batch_layout(CustomOp):
     `slots` is what rope_kv_append takes, `cu_new` what flash_attn_varlen_fwd takes, `seq_lens` what the paged attention
     ops take.  Tokens that find no row are not admitted.  The same call again gives the same results."""
 
+    host = "paged_batch_layout"
     signature = "paged_batch_layout(Tensor(a!) block_table, Tensor context_lens, Tensor new_lens, Tensor free_pages, int page_size, int num_tokens) -> (Tensor, Tensor, Tensor, Tensor, Tensor, Tensor)"
 
     def select(self, sel: KernelSelection):
@@ -523,6 +524,7 @@ class rope(CustomOp):
     `rope_inv_freq`): angles are formed in 64 bits either way.  `inverse` turns back (times `scale`, not divided by it): the
     gradient, which autograd takes for x; positions and inv_freq get none."""
 
+    host = "rope"
     signature = "rope(Tensor x, Tensor positions, Tensor inv_freq, bool interleaved, bool inverse, float scale) -> Tensor"
 
     def select(self, sel: KernelSelection):
@@ -557,7 +559,8 @@ def _rope_below_autograd(*args):
 
 class _RopeGrad(torch.autograd.Function):
     """The rotation is linear in x: its transpose is the rotation by the negated angles.  The formula stands here, not in
-    register_autograd, for its cost: a forward and backward pass of a small x take the host 100 us instead of 165."""
+    register_autograd, for its cost: a forward and backward pass of a small x take the host 100 us instead of 165.  Plain
+    device tensors take its counterpart in csrc/host_ops.cpp; this one serves tracing and operands that need a copy."""
 
     @staticmethod
     def forward(ctx, x, positions, inv_freq, interleaved, inverse, scale):
@@ -580,7 +583,8 @@ class _RopeGrad(torch.autograd.Function):
 
 def _rope_autograd(x, *args):
     if x.requires_grad and torch.is_grad_enabled():
-        return _RopeGrad.apply(x, *args)
+        y = _lib.host_ops().rope_grad(x, *args) if _on_device_eagerly(x) else None
+        return _RopeGrad.apply(x, *args) if y is None else y
     return _rope_below_autograd(x, *args)
 
 
@@ -595,6 +599,7 @@ class rope_kv_append(CustomOp):
     them; -1 or anything outside the cache: that token is not stored).  q, k_new, v_new may be slices of a packed
     projection.  Slots inside the cache must differ.  Angles, layouts and `scale` as in `rope`."""
 
+    host = "rope_kv_append"
     signature = "rope_kv_append(Tensor q, Tensor k_new, Tensor v_new, Tensor positions, Tensor inv_freq, Tensor(a!) k_cache, Tensor(b!) v_cache, Tensor slots, bool interleaved, float scale) -> Tensor"
 
     def select(self, sel: KernelSelection):
@@ -622,6 +627,7 @@ class flash_attn_varlen_fwd(CustomOp):
     flash_attn_fwd does, so the earlier part of a prompt may stand in front of its keys.  scale <= 0 selects 1/sqrt(D).
     Lengths stay on the device.  Queries without a visible key and rows outside every sequence give zeros."""
 
+    host = "flash_attn_varlen_fwd"
     signature = "flash_attn_varlen_fwd(Tensor q, Tensor k, Tensor v, Tensor cu_seqlens_q, Tensor cu_seqlens_k, bool is_causal, float scale) -> Tensor"
 
     def select(self, sel: KernelSelection):
@@ -642,15 +648,6 @@ class flash_attn_varlen_fwd(CustomOp):
         return launch._flash_attn_varlen_fwd(dev, q, k, v, cu_seqlens_q, cu_seqlens_k, out, is_causal, scale, True)
 
 
-def default_num_tree_splits(reach: int, num_seqs: int, rows: int, num_kv_heads: int) -> int:
-    """Chunks of a table's reach for paged_tree_attn: about 1024 workgroups (two rounds of what is resident; the kernels hand out
-    full chunks first) where the batch is small, of at least 512 tokens each and at most 32.  Measured: 64 sequences of
-    512-8192 tokens with 64 rows 231 / 170 / 175 / 206 us with 1 / 2 / 3 / 8 chunks; 16 of them with 128 rows 77 / 61 / 78 with
-    4 / 8 / 12; one of 32768 tokens 42 / 36 / 36 / 41 with 16 / 24 / 32 / 64."""
-    blocks = num_seqs * num_kv_heads * -(-rows // 128)
-    return max(1, min(1024 // blocks if blocks <= 1024 else 1, reach // 512, 32))
-
-
 @CustomOp.register
 class paged_tree_attn(CustomOp):
     """Attention of drafted token trees over the paged cache: q [S, N, Hq, 128], N <= 64 nodes per sequence, whose K/V are the last N
@@ -660,6 +657,7 @@ class paged_tree_attn(CustomOp):
     unwritten).  num_kv_splits <= 0 picks a default from the table width; scale <= 0 selects 1/sqrt(D).  Returns
     [S, N, Hq, 128]."""
 
+    host = "paged_tree_attn"
     signature = "paged_tree_attn(Tensor q, Tensor k_cache, Tensor v_cache, Tensor block_table, Tensor seq_lens, Tensor parents, float scale, int num_kv_splits) -> Tensor"
 
     def select(self, sel: KernelSelection):
@@ -677,7 +675,7 @@ class paged_tree_attn(CustomOp):
 
     def eager_execute(self, q, k_cache, v_cache, block_table, seq_lens, parents, scale, num_kv_splits):
         if num_kv_splits <= 0:
-            num_kv_splits = default_num_tree_splits(block_table.size(1) * k_cache.size(1), q.size(0), q.size(1) * q.size(2) // k_cache.size(2), k_cache.size(2))
+            num_kv_splits = _lib.load().mi355_paged_tree_default_splits(*q.shape[:3], k_cache.size(2), k_cache.size(1), block_table.size(1))
         dev = launch._dev(q, k_cache, v_cache, block_table, seq_lens, parents)
         out = q.new_empty(q.shape)
         return launch._paged_tree_attn(dev, q, k_cache, v_cache, block_table, seq_lens, parents, out, scale, num_kv_splits, None, None)
@@ -694,6 +692,7 @@ class verify_draft(CustomOp):
     Returns (path [S, N], num_accepted [S], next_token [S]) int32: the accepted nodes in order, then -1.  The rule stands at
     mi355_verify_draft; sums and comparisons are in 64 bits.  With parents as given to paged_tree_attn."""
 
+    host = "verify_draft"
     signature = "verify_draft(Tensor target_probs, Tensor? draft_probs, Tensor tokens, Tensor parents, Tensor uniforms) -> (Tensor, Tensor, Tensor)"
 
     def select(self, sel: KernelSelection):

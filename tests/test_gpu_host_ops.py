@@ -1,0 +1,146 @@
+"""GPU: the native host side of the serving operators gives what the way through Python gives, leaves every other call to it,
+and its gradient node behaves as one."""
+
+import pytest
+import torch
+
+import iree_turbine_amd as ita
+from conftest import announce
+from iree_turbine_amd import _lib, op_reg
+
+pytestmark = pytest.mark.gpu
+OPS = torch.ops.mi355
+
+
+# operands that may have an entry less: frequencies, free pages, the columns of a block table
+FEWER_IS_FINE = {("rope", 2), ("rope_kv_append", 4), ("paged_batch_layout", 0), ("paged_batch_layout", 3), ("paged_tree_attn", 3)}
+
+
+def _calls(dev):
+    g = torch.Generator().manual_seed(3)
+    r = lambda *s: torch.randn(*s, generator=g).half().to(dev)
+    i = lambda *v: torch.tensor(v, dtype=torch.int32, device=dev)
+    f = ita.rope_inv_freq(128, device=dev)[0]
+    kc, vc = r(9, 16, 2, 128), r(9, 16, 2, 128)
+    table = torch.tensor([[3, 1, 7], [0, 2, 8]], dtype=torch.int32, device=dev)
+    par = i(-1, 0, 0, -1, 0, 1).view(2, 3)
+    p = torch.softmax(torch.randn(2, 3, 50, generator=g), -1).to(dev)
+    return {
+        "rope": (r(5, 4, 128), i(0, 3, 9, 1, 1), f, False, True, 1.5),
+        "rope_kv_append": (r(3, 4, 128), r(3, 2, 128), r(3, 2, 128), i(5, 6, 7), f, kc, vc, torch.tensor([4, -1, 100], device=dev), True, 1.0),
+        "paged_batch_layout": (table.clone(), i(20, 3), i(9, 1), i(5, 4, 6), 16, 12),
+        "flash_attn_varlen_fwd": (r(12, 4, 128), r(12, 2, 128), r(12, 2, 128), i(0, 5, 12), i(0, 5, 12), True, 0.0),
+        "paged_tree_attn": (r(2, 3, 4, 128), kc, vc, table, i(40, 33), par, 0.0, 0),
+        "verify_draft": (p, p.flip(0).contiguous(), i(1, 2, 3, 4, 5, 6).view(2, 3), par, torch.rand(2, 3, generator=g).to(dev)),
+    }
+
+
+def _same(a, b):
+    a, b = ([t] if isinstance(t, torch.Tensor) else list(t) for t in (a, b))
+    assert len(a) == len(b) and all(x.dtype == y.dtype and x.stride() == y.stride() and torch.equal(x, y) for x, y in zip(a, b))
+
+
+@pytest.mark.parametrize("name", ["rope", "rope_kv_append", "paged_batch_layout", "flash_attn_varlen_fwd", "paged_tree_attn", "verify_draft"])
+def test_same_as_the_way_through_python(dev, name):
+    announce(f"host ops {name}")
+    args = _calls(dev)[name]
+    copies = lambda: tuple(a.clone() if isinstance(a, torch.Tensor) else a for a in args)
+    mine, theirs = copies(), copies()
+    native = getattr(_lib.host_ops(), name)(*mine)
+    assert native is not None
+    _same(native, op_reg.ALL_CUSTOM_OP_REGS[f"mi355.{name}"].eager_execute(*theirs))
+    for a, b in zip(mine, theirs):  # what is written in place
+        if isinstance(a, torch.Tensor):
+            assert torch.equal(a, b)
+    # operands that are not laid out as the kernels take them are left to Python, and the op gives the same
+    for k, a in enumerate(args):
+        if not isinstance(a, torch.Tensor) or (name, k) in (("rope_kv_append", 5), ("rope_kv_append", 6), ("paged_batch_layout", 0)):
+            continue
+        odd = list(copies())
+        odd[k] = torch.stack([a, torch.zeros_like(a)], -1)[..., 0]
+        assert not odd[k].is_contiguous() and getattr(_lib.host_ops(), name)(*odd) is None
+        _same(getattr(OPS, name)(*odd), native)
+
+
+@pytest.mark.parametrize("name", ["rope", "rope_kv_append", "paged_batch_layout", "flash_attn_varlen_fwd", "paged_tree_attn", "verify_draft"])
+def test_what_breaks_the_contract_is_refused(dev, name):
+    """One operand at a time: a row fewer, an axis more, another type, on the host.  Nothing is launched for any of them."""
+    announce(f"host ops refusals {name}")
+    args = _calls(dev)[name]
+    op, native = getattr(OPS, name), getattr(_lib.host_ops(), name)
+    for k, a in enumerate(args):
+        if not isinstance(a, torch.Tensor):
+            continue
+        bad = [a[None], a.to(torch.int16), a.cpu()]
+        if (name, k) not in FEWER_IS_FINE:
+            bad.append(a[..., :-1].contiguous())
+        for b in bad:
+            changed = (*args[:k], b, *args[k + 1 :])
+            assert native(*changed) is None, (k, b.shape, b.dtype, b.device)
+            with pytest.raises((ValueError, RuntimeError, NotImplementedError)):
+                op(*changed)
+    assert native(*args[:-1]) is None and native(*args, 1) is None and native(*([None] * len(args))) is None
+
+
+def test_gradient_node(dev):
+    """Twice differentiable, careful about its saved tensors, through hooks, and with gradients of any strides."""
+    announce("host ops gradient node")
+    pos, f = torch.arange(6, dtype=torch.int32, device=dev), ita.rope_inv_freq(64, device=dev)[0]
+    x = torch.randn(6, 3, 96, device=dev, requires_grad=True)
+    call = lambda t: OPS.rope(t, pos, f, True, False, 2.0)
+    y = call(x)
+    assert "RopeGrad" in y.grad_fn.name() and y.grad_fn.name() != "_RopeGradBackward"
+    g = torch.randn(6, 3, 96, device=dev)
+    back = OPS.rope(g, pos, f, True, True, 2.0)
+    assert torch.equal(torch.autograd.grad(y, x, g, retain_graph=True)[0], back)
+    for odd in (g.transpose(0, 2).contiguous().transpose(0, 2), torch.stack([g, g], -1)[..., 1], g[:1].expand(6, 3, 96)):
+        assert torch.equal(torch.autograd.grad(y, x, odd, retain_graph=True)[0], OPS.rope(odd.contiguous(), pos, f, True, True, 2.0))
+    gr = g.clone().requires_grad_()
+    dx = torch.autograd.grad(y, x, gr, create_graph=True)[0]
+    again = torch.autograd.grad(dx, gr, x.detach(), create_graph=True)[0]
+    assert again is not None and torch.equal(again, call(x.detach()))
+    packed = []
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: (packed.append(t.shape), t.cpu())[1], lambda t: t.to(dev)):
+        z = call(x)
+    assert len(packed) == 2 and torch.equal(torch.autograd.grad(z, x, g)[0], back)
+    with torch.no_grad():
+        assert not call(x).requires_grad
+    z = call(x)
+    pos.add_(1)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        torch.autograd.grad(z, x, g)
+    pos.sub_(1)
+    side = torch.cuda.Stream(dev)
+    side.wait_stream(torch.cuda.current_stream(dev))
+    with torch.cuda.stream(side):
+        z = call(x * 1.0)
+    torch.cuda.current_stream(dev).wait_stream(side)
+    dx = torch.autograd.grad(z, x, g)[0]
+    torch.cuda.synchronize()
+    assert torch.equal(dx, back)
+
+
+def test_threads_and_streams(dev):
+    """Calls from several threads, each on a stream of its own."""
+    import threading
+
+    announce("host ops threads")
+    args = _calls(dev)
+    want = OPS.flash_attn_varlen_fwd(*args["flash_attn_varlen_fwd"])
+    turned = OPS.rope(*args["rope"])
+    torch.cuda.synchronize()
+    bad = []
+
+    def work():
+        s = torch.cuda.Stream(dev)
+        with torch.cuda.stream(s):
+            outs = [(OPS.flash_attn_varlen_fwd(*args["flash_attn_varlen_fwd"]), OPS.rope(*args["rope"])) for _ in range(50)]
+        s.synchronize()
+        bad.extend(1 for a, b in outs if not (torch.equal(a, want) and torch.equal(b, turned)))
+
+    threads = [threading.Thread(target=work) for _ in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not bad

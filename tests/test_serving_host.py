@@ -8,7 +8,7 @@ import pytest
 import torch
 
 import iree_turbine_amd as ita
-from iree_turbine_amd import _lib
+from iree_turbine_amd import _lib, op_reg
 from oracle import serving
 
 OPS = torch.ops.mi355
@@ -275,3 +275,18 @@ def test_rope_gradient_formula_is_traced_and_differentiable_twice():
 
     calls = [n for n in make_fx(step)(m(5, 3, 96, dt=F32), pos, f, m(5, 3, 96, dt=F32)).graph.nodes if "rope" in str(n.target)]
     assert [n.args[4] for n in calls] == [False, True]
+
+
+def test_native_host_side_leaves_other_calls_alone():
+    host = _lib.host_ops()
+    names = [n for n in dir(host) if not n.startswith("_") and n != "bind"]
+    assert sorted(names) == sorted(["rope_grad"] + [op.host for op in op_reg.ALL_CUSTOM_OP_REGS.values() if op.host])
+    cpu = (torch.zeros(2, 2, 64), torch.zeros(2, dtype=I32), torch.zeros(32, dtype=F64), False, False, 1.0)
+    for name in names:
+        f = getattr(host, name)
+        assert f() is None and f(*cpu) is None and f(*([3] * 6)) is None and f(*([None] * 10)) is None
+    with pytest.raises(TypeError):
+        host.bind()
+    with pytest.raises(ValueError):
+        host.bind(*([0] * 10))
+    assert _lib.host_ops() is host
