@@ -399,17 +399,19 @@ static int run_tree(TreeArgs a, int num_seqs, hipStream_t stream) {
 
 using namespace mi355;
 
-// About 1024 workgroups (two rounds of what is resident; the kernels hand out full chunks first) where the batch is small, of
-// at least 512 tokens each and at most 32 chunks.  Measured: 64 sequences of 512-8192 tokens with 64 rows 231 / 170 / 175 / 206 us
-// with 1 / 2 / 3 / 8 chunks; 16 of them with 128 rows 77 / 61 / 78 with 4 / 8 / 12; one of 32768 tokens 42 / 36 / 36 / 41 with
-// 16 / 24 / 32 / 64.
+// Chunks of at least 128 tokens, at most 64, for about so many workgroups: 256 where few (sequence, K/V head, 128 rows) blocks read
+// long caches on the kernel above, which a workgroup per CU drives at memory's rate (one sequence of 32768 tokens 36 / 31 / 35 us
+// with 128 / 256 / 384 workgroups), 512 where the prefill form does, which needs two per CU (64 rows: 41 / 37 with 256 / 384), or
+// with 20 to 32 blocks; more blocks differ in length, and 1024 in order of their size even that out (64 sequences of
+// 512-8192 tokens with 64 rows 231 / 170 / 175 / 206 us with 512 / 1024 / 1536 / 4096, 8 of 1000-16384 63 / 51 / 62 with 512 / 1024 / 1536).
 extern "C" int64_t mi355_paged_tree_default_splits(int64_t num_seqs, int64_t num_nodes, int64_t num_q_heads, int64_t num_kv_heads,
                                                    int64_t page_size, int64_t max_pages_per_seq) {
   if (num_seqs <= 0 || num_nodes <= 0 || num_q_heads <= 0 || num_kv_heads <= 0) return 1;
   const int64_t rows = num_nodes * num_q_heads / num_kv_heads, blocks = num_seqs * num_kv_heads * ((rows + 127) / 128);
-  const int64_t fill = blocks <= 1024 && blocks > 0 ? 1024 / blocks : 1, tokens = max_pages_per_seq * page_size / 512;
-  const int64_t n = fill < tokens ? fill : tokens;
-  return n < 1 ? 1 : n > 32 ? 32 : n;
+  if (blocks <= 0 || blocks > 1024) return 1;
+  const int64_t wgs = blocks > 32 ? 1024 : blocks >= 20 || rows > 32 ? 512 : 256;
+  const int64_t fill = wgs / blocks, tokens = max_pages_per_seq * page_size / 128, n = fill < tokens ? fill : tokens;
+  return n < 1 ? 1 : n > 64 ? 64 : n;
 }
 
 extern "C" int mi355_paged_tree_attn(const void* q, const void* k_cache, const void* v_cache, const int32_t* block_table,
