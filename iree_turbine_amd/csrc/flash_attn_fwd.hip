@@ -639,9 +639,14 @@ __device__ __forceinline__ bool fa_find_unit(const FaVarlen& vl, int group, int 
       if (vl.pairs) n = (n + 1) >> 1;
     }
     if (vl.ranked) {
-      for (int j = 0; j < vl.num_seqs; j++) {
-        const int kj = __builtin_amdgcn_readlane(kl, j), nj = __builtin_amdgcn_readlane(n, j);
-        before += (kj > kl || (kj == kl && j < lane)) ? nj : 0;
+      // one number per sequence orders them: more keys first, then as they come; lanes behind the last have no units
+      const int key = kl < 0 ? -1 : (kl << 6) | (63 - lane);
+      for (int j0 = 0; j0 < vl.num_seqs; j0 += 8) {
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+          const int kj = __builtin_amdgcn_readlane(key, j0 + e), nj = __builtin_amdgcn_readlane(n, j0 + e);
+          before += kj > key ? nj : 0;
+        }
       }
     } else {
       int incl = n;
@@ -2116,8 +2121,9 @@ static FaVarlenPlan fa_varlen_plan(int64_t num_seqs, int64_t total_q, int64_t to
   // One prompt of 1024 tokens (32 query heads over 8) 23 against 29 us, 32 of 16 tokens 8.0 against 9.7; where the chip
   // is full the 64-row blocks are bound by LDS reads: 8 prompts of 256 tokens 22 against 20, one of 4096 164 against 134.
   p.qg = blocks < 512 ? 1 : 2;
-  // Ranking costs every workgroup some 20 ns per sequence: worth it where sequences are long or few.
-  p.ranked = num_seqs > 1 && num_seqs <= 64 && total_k / num_seqs >= 16 * num_seqs;
+  // Ranking costs every workgroup some 12 ns per sequence: worth it where sequences are long or few (32 of 2 to 600 tokens, 16
+  // heads over one, 22.9 against 25.7 us, 16 of them 15.7 against 16.6; 64 of 2 to 100 tokens, 32 heads over 8, 21.3 against 18.0).
+  p.ranked = num_seqs > 1 && num_seqs <= 64 && total_k / num_seqs >= 3 * num_seqs;
   // Few blocks that walk many keys: the number of chunks whose estimate is the smallest, in us: 3.5 for a workgroup and 0.85 for
   // each of its key tiles, twice and more where there are more workgroups than the 512 resident ones; and for the
   // joining 4 and the partial results written and read at 3.5 TB/s.  One to four sequences of 8192 keys and up to 128 new

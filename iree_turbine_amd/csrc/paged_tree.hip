@@ -17,9 +17,9 @@
 // its result directly, the others write fp32 partials that a second launch merges (two launches wherever the table's reach
 // is cut: the lengths are not known on the host).  Full chunks are handed out before shorter ones, see tree.hpp.
 //
-// Measured (8 K/V heads, 64 rows, bf16): one sequence of 32768 tokens 33 us, of which the second launch is 5 (the first
-// reads 5.1 TB/s), 64 of 512 to 8192
-// tokens 175 us (4.3 TB/s of the 5.0 that a copy reaches).  Looking masked steps over for non-finite values is 1 to 5 of these.
+// Measured, 8 K/V heads: one sequence of 32768 tokens (28 rows, fp16) 33 us, of which the second launch is 5 (the first reads
+// 5.1 TB/s); 64 of 512 to 8192 tokens (64 rows, bf16) 175 us, 4.3 TB/s.  Looking masked steps over for non-finite values is 1
+// of the one and 5 of the other.
 #include "tree.hpp"
 #include <math.h>
 
