@@ -217,3 +217,34 @@ def test_lazily_negated_operands_and_gradients(dev):
     w = z.clone().requires_grad_()
     v = w.conj().imag
     torch.testing.assert_close(torch.autograd.grad(call(v), w, want)[0], torch.autograd.grad(call(-w.imag), w, want)[0], rtol=0, atol=0)
+
+
+def test_rows_past_32_bit_offsets(dev):
+    """Rows a mebi-element apart, read and written in place; a cache whose last slots lie more than 2^32 elements in."""
+    from oracle import serving
+
+    announce("rope far rows")
+    T, pitch = 2300, 1 << 20
+    far = torch.empty(T * pitch, dtype=torch.float16, device=dev).view(T, pitch)[:, 64:64 + 256].view(T, 2, 128)
+    x = torch.randn(T, 2, 128).half()
+    far.copy_(x)
+    pos, f = torch.arange(T, dtype=torch.int32), _freq(128)[0]
+    want, bound = serving.rope_ref(x, pos, f, False)
+    _inside(torch.ops.mi355.rope(far, pos.to(dev), f.to(dev), False, False, 1.0), want, bound)
+    from iree_turbine_amd import launch
+
+    launch.rope_out(far, pos.to(dev), f.to(dev), far, False, False, 1.0)
+    _inside(far, want, bound)
+    del far
+    P = (1 << 32) // (256 * 8 * 128) + 2
+    kc, vc = (torch.empty(P, 256, 8, 128, dtype=torch.float16, device=dev) for _ in range(2))
+    last = P * 256
+    slots = torch.tensor([last - 1, 0, last, -(2**40), last - 300], device=dev)
+    q, k, v = (torch.randn(5, h, 128).half() for h in (8, 8, 8))
+    p5 = pos[:5] * 100
+    torch.ops.mi355.rope_kv_append(q.to(dev), k.to(dev), v.to(dev), p5.to(dev), f.to(dev), kc, vc, slots, False, 1.0)
+    want, bound = serving.rope_ref(k, p5, f, False)
+    flat_k, flat_v = kc.view(-1, 8, 128), vc.view(-1, 8, 128)
+    for row, slot in ((0, last - 1), (1, 0), (4, last - 300)):
+        _inside(flat_k[slot], want[row], bound[row])
+        assert torch.equal(flat_v[slot].cpu(), v[row])

@@ -261,3 +261,25 @@ def test_captured_for_any_lengths(dev):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(out, torch.ops.mi355.flash_attn_varlen_fwd(q, k, v, cu, cu, True, 0.0))
+
+
+@pytest.mark.parametrize("lens", [[2300, 1], [2, 4, 2400]], ids=["chunks", "last"])
+def test_rows_past_32_bit_offsets(dev, lens):
+    """Rows a mebi-element apart: the last ones lie more than 2^32 bytes behind the first."""
+    from oracle import serving
+
+    announce(f"varlen far rows {lens}")
+    T, pitch = sum(lens), 1 << 20
+    far = torch.empty(T * pitch, dtype=torch.bfloat16, device=dev).view(T, pitch)
+    assert far.numel() * 2 > 2**32
+    q, k, v, o = (far[:, 256 * i : 256 * i + 256].view(T, 2, 128) for i in range(4))
+    host = [torch.randn(T, 2, 128).bfloat16() for _ in range(3)]
+    for t, h in zip((q, k, v), host):
+        t.copy_(h)
+    cu = _cu(lens)
+    want, bound = serving.varlen_ref(*host, cu, cu, True)
+    _inside(torch.ops.mi355.flash_attn_varlen_fwd(q, k, v, cu.to(dev), cu.to(dev), True, 0.0), want, bound)
+    from iree_turbine_amd import launch
+
+    launch.flash_attn_varlen_fwd_out(q, k, v, cu.to(dev), cu.to(dev), o, True, 0.0)
+    _inside(o, want, bound)
