@@ -290,3 +290,10 @@ def test_native_host_side_leaves_other_calls_alone():
     with pytest.raises(ValueError):
         host.bind(*([0] * 10))
     assert _lib.host_ops() is host
+
+
+def test_missing_native_host_side_is_an_error(monkeypatch, tmp_path):
+    monkeypatch.setattr(_lib, "_host", None)
+    monkeypatch.setattr(_lib, "HOST_PATH", tmp_path / "mi355_host_ops.so")
+    with pytest.raises(_lib.KernelLibraryError, match="build it"):
+        _lib.host_ops()
