@@ -221,6 +221,22 @@ def test_offsets_outside_the_stream(dev):
     assert got.shape == q.shape
 
 
+def test_offsets_outside_the_stream_in_chunks(dev):
+    """The same where the keys are cut into chunks."""
+    announce("varlen wild offsets, chunks")
+    q, k, v = (torch.randn(t, 2, 128).half().to(dev) for t in (50, 4000, 4000))
+    i = lambda *x: torch.tensor(x, dtype=torch.int32, device=dev)
+    a = torch.ops.mi355.flash_attn_varlen_fwd(q, k, v, i(-9, 20, 2**31 - 1), i(-5, 1500, 2**31 - 1), True, 0.0)
+    b = torch.ops.mi355.flash_attn_varlen_fwd(q, k, v, i(0, 20, 50), i(0, 1500, 4000), True, 0.0)
+    assert torch.equal(a, b) and torch.isfinite(a).all()
+    got = torch.ops.mi355.flash_attn_varlen_fwd(q, k, v, i(0, 30, 10, 50), i(0, 3000, 10, 4000), True, 0.0)
+    torch.cuda.synchronize()
+    assert got.shape == q.shape
+    # a sequence whose keys begin behind its end, one without keys, one without queries
+    c = torch.ops.mi355.flash_attn_varlen_fwd(q, k, v, i(0, 20, 40, 40, 50), i(3000, 3000, 3000, 3500, 4000), False, 0.0)
+    assert torch.equal(c[:40], torch.zeros_like(c[:40])) and bool((c[40:] != 0).any(-1).all())
+
+
 def test_agrees_with_the_rectangular_op_and_reads_slices(dev):
     """Equal lengths: the rectangular op's result within the two kernels' rounding; slices of a packed projection are read
     in place and give the same bits as copies; so do rows off the 16-byte borders, which are copied."""
