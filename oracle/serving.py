@@ -69,7 +69,11 @@ def attention_ref(q, k, v, visible, scale: float | None = None):
     The bound, with h = half a step of the 16-bit type and f = 2^-24: a score of D products summed in 32 bits is off by
     at most D f (scale |q| . |k|), its product with the scale and the subtraction of the maximum by 4 f (|s| + |max|); with
     d the largest of these, weights move by a factor e^(2 d) at most; each weight is rounded to 16 bits once (h) and again where its sum is taken from the
-    rounded ones (h); the accumulation over m keys adds (m + 64) f; the result is rounded once (h)."""
+    rounded ones (h); the accumulation over m keys adds (m + 64) f; the result is rounded once (h).
+
+    fp16 weights below 2^-14 are off by up to t = 2^-25 instead, in the result and in the weights' sum: t (sum |v| + n |out|) over that
+    sum, n the visible keys.  A weight is exp(score - r) with r a maximum of scores seen so far, which the true maximum is never below, and is only ever scaled
+    down afterwards, so that the weights' sum is at least that of exp(score - true maximum), but for e^d."""
     n, hq, D = q.shape
     m, hkv = k.shape[0], k.shape[1]
     scale = 1 / math.sqrt(D) if scale is None else scale
@@ -88,10 +92,12 @@ def attention_ref(q, k, v, visible, scale: float | None = None):
         off = mag * D * f + 4 * f * torch.where(visible, s.abs() + top.abs(), 0.0)
         d = off.amax(-1, keepdim=True)
         w = torch.exp(s - torch.where(top == -math.inf, 0.0, top))
-        w = w / torch.where(w.sum(-1, keepdim=True) > 0, w.sum(-1, keepdim=True), 1.0)
+        total = w.sum(-1, keepdim=True)
+        total = torch.where(total > 0, total, 1.0)
+        w = w / total
         out[:, j] = w @ vv
-        # fp16 weights below 2^-14 lose relative precision: half their smallest step each, against a sum of at least 2^-8
-        small = tiny * 2**8 * (visible.double() @ vv.abs())
+        seen = visible.double()
+        small = tiny * torch.exp(2 * d) / total * (seen @ vv.abs() + seen.sum(-1, keepdim=True) * out[:, j].abs())
         bound[:, j] = (torch.expm1(2 * d) + 2 * h + (m + 64) * f) * (w @ vv.abs()) + h * out[:, j].abs() + small + tiny
     return out, bound
 

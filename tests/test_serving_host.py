@@ -297,3 +297,36 @@ def test_missing_native_host_side_is_an_error(monkeypatch, tmp_path):
     monkeypatch.setattr(_lib, "HOST_PATH", tmp_path / "mi355_host_ops.so")
     with pytest.raises(_lib.KernelLibraryError, match="build it"):
         _lib.host_ops()
+
+
+@pytest.mark.parametrize("m", [65, 130, 257, 515, 700, 900, 1033, 1500, 1900, 2300, 2600, 4000])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_oracle_attention_bound_sees_a_lost_tile(dtype, m):
+    """At the lengths that the attention tests use, a result without one tile of 64 keys, one 32-key step or one of 16 chunks
+    is outside the bound, wherever it lies."""
+    q, k, v = (torch.randn(n, h, 128).to(dtype) for n, h in ((4, 4), (m, 2), (m, 2)))
+    vis = torch.ones(4, m, dtype=torch.bool)
+    out, bound = serving.attention_ref(q, k, v, vis)
+    for width in {32, 64, -(-m // 1024) * 64}:
+        for at in {0, (m - width) // 2, m - width}:
+            lost = vis.clone()
+            lost[:, at : at + width] = False
+            assert float(((serving.attention_ref(q, k, v, lost)[0] - out).abs() / bound).max()) > 1, (width, at)
+    assert float((out.abs() / bound).median()) > 1  # nor would zeros pass
+
+
+def test_oracle_attention_bound_holds_for_16_bit_weights():
+    """The bound's own model, step by step: weights against a maximum that lags by up to 2^8, rounded to 16 bits, summed either way,
+    scaled down later.  Wide scores leave most fp16 weights below 2^-14."""
+    for dtype in (torch.float16, torch.bfloat16):
+        for spread in (1.0, 3.0, 12.0):
+            q, k, v = (torch.randn(n, 1, 128) for n in (16, 500, 500))
+            q, k, v = (q * spread).to(dtype), k.to(dtype), v.to(dtype)
+            out, bound = serving.attention_ref(q, k, v, torch.ones(16, 500, dtype=torch.bool))
+            s = (q[:, 0].float() @ k[:, 0].float().t()) * 128**-0.5
+            for lag in (0.0, 5.5):  # in nats
+                w = torch.exp(s - s.amax(-1, keepdim=True) + lag)
+                r = w.to(dtype).double()
+                for total in (w.double().sum(-1, keepdim=True), r.sum(-1, keepdim=True)):
+                    got = ((r @ v[:, 0].double()) / total).to(dtype).double()
+                    assert bool(((got - out[:, 0]).abs() <= bound[:, 0]).all())
