@@ -12,6 +12,7 @@
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <ATen/ATen.h>
+#include <ATen/core/dispatch/Dispatcher.h>
 #include <c10/hip/HIPFunctions.h>
 #include <c10/hip/HIPStream.h>
 
@@ -65,12 +66,18 @@ double number(PyObject* o) {
   return PyFloat_AS_DOUBLE(o);
 }
 
+// Memory that is what the tensor stands for.  (Below the dispatcher every tensor is; the rotation is also called above it,
+// with lazily negated ones, zeros without memory, and the wrappers of torch.func and of tensor subclasses.)
+bool is_plain(const Tensor& t) {
+  static const c10::DispatchKeySet odd({c10::DispatchKey::Negative, c10::DispatchKey::ZeroTensor, c10::DispatchKey::FuncTorchBatched,
+                                        c10::DispatchKey::FuncTorchGradWrapper, c10::DispatchKey::Functionalize, c10::DispatchKey::Python});
+  return t.layout() == at::kStrided && !t.key_set().has_any(odd);
+}
 // All on one device, the current one: the caller of the kernel needs no guard then.
 template <typename... Ts>
 void on_current(const Tensor& first, const Ts&... rest) {
   const c10::Device dev = first.device();
-  // (below the dispatcher no tensor is lazily negated or a zero without memory; the rotation is also called above it)
-  auto plain = [&](const Tensor& t) { return t.device() == dev && t.layout() == at::kStrided && !t.is_neg() && !t._is_zerotensor(); };
+  auto plain = [&](const Tensor& t) { return t.device() == dev && is_plain(t); };
   want(dev.is_cuda() && dev.index() == c10::hip::current_device() && plain(first) && (plain(rest) && ...));
 }
 void* current_stream(const Tensor& t) { return (void*)c10::hip::getCurrentHIPStream(t.get_device()).stream(); }
@@ -134,8 +141,15 @@ Tensor rope(const Tensor& x, const Tensor& pos, const Tensor& freq, bool inter, 
   return out;
 }
 
+// The op itself, for what the functions here do not take: the lock is taken on the way.
+Tensor rope_by_dispatcher(const Tensor& x, const Tensor& pos, const Tensor& freq, bool inter, bool inverse, double scale) {
+  static const auto op = c10::Dispatcher::singleton().findSchemaOrThrow("mi355::rope", "").typed<Tensor(const Tensor&, const Tensor&, const Tensor&, bool, bool, double)>();
+  return op.call(x, pos, freq, inter, inverse, scale);
+}
+
 // The gradient as a node of the engine's own kind: its backward pass takes no interpreter lock (a forward and backward pass of a
-// small x: 98 us with the node in Python).  Same formula and same saved tensors as ops._RopeGrad.
+// small x: 98 us with the node in Python).  Same formula and same saved tensors as ops._RopeGrad.  Gradients that are to be
+// differentiated, have a tangent, or are no plain tensors go through the op.
 struct RopeGrad : torch::autograd::Function<RopeGrad> {
   static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& x, const Tensor& pos, const Tensor& freq, bool inter, bool inverse,
                         double scale) {
@@ -149,17 +163,11 @@ struct RopeGrad : torch::autograd::Function<RopeGrad> {
     const auto saved = ctx->get_saved_variables();
     const bool inter = ctx->saved_data["inter"].toBool(), inverse = !ctx->saved_data["inverse"].toBool();
     const double scale = ctx->saved_data["scale"].toDouble();
-    Tensor g = grads[0];
-    if (g._is_zerotensor()) g = at::zeros(g.sizes(), g.options());
-    if (g.is_neg() || g.stride(2) != 1) g = g.resolve_neg().contiguous();
-    Tensor dx;
-    if (at::GradMode::is_enabled() && g.requires_grad()) {
-      try {
-        dx = RopeGrad::apply(g, saved[0], saved[1], inter, inverse, scale);
-      } catch (NotTaken&) {
-        TORCH_CHECK(false, "rope: the gradient's rotation was refused: ", entry.last_error());
-      }
+    Tensor g = grads[0], dx;
+    if ((at::GradMode::is_enabled() && g.requires_grad()) || g._fw_grad(0).defined() || !is_plain(g)) {
+      dx = rope_by_dispatcher(g, saved[0], saved[1], inter, inverse, scale);
     } else {
+      if (g.stride(2) != 1) g = g.contiguous();
       dx = fresh(g.sizes(), g, g.scalar_type());
       TORCH_CHECK(run_rope(g, saved[0], saved[1], dx, inter, inverse, scale) == 0, "rope: the gradient's rotation failed: ", entry.last_error());
     }

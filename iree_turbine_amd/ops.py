@@ -12,6 +12,8 @@ import math
 
 import torch
 from torch import Tensor
+from torch._functorch.autograd_function import enable_single_level_autograd_function
+from torch.autograd import forward_ad
 
 from . import launch
 from .contract import PAGE_SIZES, check_mx_operand as _check_mx_operand, check_paged_args as _check_paged_args  # noqa: F401
@@ -546,33 +548,47 @@ class rope(CustomOp):
 
 def _on_device_eagerly(x: Tensor) -> bool:
     """A plain device tensor outside every dispatch mode: the launch needs no further pass through the dispatcher.  Meta
-    and fake tensors and tracing do, and lazily negated or zero ones, whose memory is not yet what they stand for."""
-    return type(x) in (Tensor, torch.nn.Parameter) and x.is_cuda and torch._C._len_torch_dispatch_stack() == 0 and not x.is_neg() and not x._is_zerotensor()
+    and fake tensors and tracing do, torch.func's wrappers, and lazily negated or zero ones, whose memory is not yet what they
+    stand for."""
+    return type(x) in (Tensor, torch.nn.Parameter) and x.is_cuda and torch._C._len_torch_dispatch_stack() == 0 and not x.is_neg() and not x._is_zerotensor() \
+        and not torch._C._functorch.is_functorch_wrapped_tensor(x)
+
+
+def _has_tangent(x: Tensor) -> bool:
+    return forward_ad._current_level >= 0 and forward_ad.unpack_dual(x).tangent is not None
 
 
 def _rope_below_autograd(*args):
-    if _on_device_eagerly(args[0]) and not args[2].is_neg():
-        return _rope_on_device(*args)
+    if args[0].is_cuda and torch._C._len_torch_dispatch_stack() == 0:
+        y = _lib.host_ops().rope(*args)  # None for all but plain device tensors
+        if y is not None:
+            return y
     with torch._C._AutoDispatchBelowAutograd():
         return torch.ops.mi355.rope(*args)
 
 
 class _RopeGrad(torch.autograd.Function):
-    """The rotation is linear in x: its transpose is the rotation by the negated angles.  The formula stands here, not in
-    register_autograd, for its cost: a forward and backward pass of a small x take the host 100 us instead of 165.  Plain
-    device tensors take its counterpart in csrc/host_ops.cpp; this one serves tracing and operands that need a copy."""
+    """The rotation is linear in x: its transpose is the rotation by the negated angles, its tangent the rotation of x's.  The
+    formula stands here, not in register_autograd, for its cost: a forward and backward pass of a small x take the host 100 us
+    instead of 165.  Plain device tensors take its counterpart in csrc/host_ops.cpp; this one serves tracing, forward mode,
+    torch.func and operands that need a copy."""
 
     @staticmethod
     def forward(ctx, x, positions, inv_freq, interleaved, inverse, scale):
         ctx.interleaved, ctx.inverse, ctx.scale = interleaved, inverse, scale
         ctx.save_for_backward(positions, inv_freq)
-        return _rope_below_autograd(x, positions, inv_freq, interleaved, inverse, scale)
+        ctx.save_for_forward(positions, inv_freq)
+        args = (x, positions, inv_freq, interleaved, inverse, scale)
+        if not torch._C._are_functorch_transforms_active():
+            return _rope_below_autograd(*args)
+        with torch.enable_grad(), forward_ad._set_fwd_grad_enabled(True):  # this call has turned them off for the levels below as well
+            return _rope_below_autograd(*args)
 
     @staticmethod
     def backward(ctx, grad):
         positions, inv_freq = ctx.saved_tensors
         how = (ctx.interleaved, not ctx.inverse, ctx.scale)
-        if torch.is_grad_enabled():
+        if torch.is_grad_enabled() or _has_tangent(grad):
             dx = torch.ops.mi355.rope(grad, positions, inv_freq, *how)
         elif _on_device_eagerly(grad):  # its sizes and type are the result's, whose call has been checked
             dx = launch._rope(grad.device, grad, positions, inv_freq, grad.new_empty(grad.shape), *how)
@@ -580,15 +596,31 @@ class _RopeGrad(torch.autograd.Function):
             dx = _rope_below_autograd(grad, positions, inv_freq, *how)
         return dx, None, None, None, None, None
 
+    @staticmethod
+    def jvp(ctx, tangent, *_):
+        if tangent is None:
+            return None
+        positions, inv_freq = ctx.saved_tensors
+        return torch.ops.mi355.rope(tangent, positions, inv_freq, ctx.interleaved, ctx.inverse, ctx.scale)
+
+
+def _rope_grad(*args):
+    if not torch._C._are_functorch_transforms_active():
+        return _RopeGrad.apply(*args)
+    # The dispatcher has done the transform's part when it gets to the Autograd key: what is left is one node at its level.
+    # (autograd.Function.apply would start with the transforms again.)
+    with enable_single_level_autograd_function():
+        return super(torch.autograd.Function, _RopeGrad).apply(*args)
+
 
 def _rope_autograd(x, *args):
-    if x.requires_grad and torch.is_grad_enabled():
-        y = _lib.host_ops().rope_grad(x, *args) if _on_device_eagerly(x) else None
-        return _RopeGrad.apply(x, *args) if y is None else y
+    tangent = _has_tangent(x)
+    if tangent or (x.requires_grad and torch.is_grad_enabled()):
+        y = _lib.host_ops().rope_grad(x, *args) if x.is_cuda and not tangent and torch._C._len_torch_dispatch_stack() == 0 else None
+        return _rope_grad(x, *args) if y is None else y
     return _rope_below_autograd(x, *args)
 
 
-_rope_on_device = op_reg.device_impl(op_reg.ALL_CUSTOM_OP_REGS["mi355.rope"])
 op_reg.MI355_LIBRARY.impl("rope", _rope_autograd, "Autograd")
 
 

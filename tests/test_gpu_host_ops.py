@@ -144,3 +144,34 @@ def test_threads_and_streams(dev):
     for t in threads:
         t.join()
     assert not bad
+
+
+@pytest.mark.filterwarnings("ignore:There is a performance drop")
+def test_forward_mode_and_transforms_on_the_device(dev):
+    """Tangents, torch.func and batched gradients of the rotation give what calls on plain tensors give."""
+    import torch.autograd.forward_ad as fw
+
+    announce("rope forward mode and torch.func")
+    pos, f = torch.arange(5, dtype=torch.int32, device=dev) * 77, ita.rope_inv_freq(64, device=dev)[0]
+    call, back = (lambda v: OPS.rope(v, pos, f, False, False, 1.5)), (lambda v: OPS.rope(v, pos, f, False, True, 1.5))
+    x, t = (torch.randn(5, 2, 96, device=dev) for _ in range(2))
+    with fw.dual_level():
+        for leaf in (x, x.clone().requires_grad_()):
+            y = fw.unpack_dual(call(fw.make_dual(leaf, t)))
+            assert torch.equal(y.tangent, call(t)) and torch.equal(y.primal, call(x))
+        leaf = x.clone().requires_grad_()
+        for graph in (False, True):
+            dx, = torch.autograd.grad(call(leaf), leaf, fw.make_dual(x, t), create_graph=graph)
+            assert torch.equal(fw.unpack_dual(dx).tangent, back(t)) and torch.equal(fw.unpack_dual(dx).primal, back(x))
+    many = torch.stack([x, t, x - t])
+    want = torch.stack([call(v) for v in many])
+    assert torch.equal(torch.func.vmap(call)(many), want)
+    assert torch.equal(torch.func.jvp(call, (x,), (t,))[1], call(t)) and torch.equal(torch.func.vjp(call, x)[1](t)[0], back(t))
+    assert torch.equal(torch.func.grad(lambda v: (call(v) * t).sum())(x), back(t))
+    assert torch.equal(torch.func.vmap(torch.func.grad(lambda v: (call(v) * t).sum()))(many), back(t).expand(3, 5, 2, 96))
+    assert torch.equal(torch.func.vmap(torch.func.jvp, in_dims=(None, None, 0))(call, (x,), (many,))[1], want)
+    assert torch.equal(torch.func.jvp(lambda v: torch.func.grad(lambda w: (call(w) ** 2).sum() / 2)(v), (x,), (t,))[1], back(call(t)))
+    leaf = x.clone().requires_grad_()
+    y = call(leaf)
+    assert "RopeGrad" in y.grad_fn.name()
+    assert torch.equal(torch.autograd.grad(y, leaf, many, is_grads_batched=True)[0], torch.stack([back(v) for v in many]))

@@ -330,3 +330,62 @@ def test_oracle_attention_bound_holds_for_16_bit_weights():
                 for total in (w.double().sum(-1, keepdim=True), r.sum(-1, keepdim=True)):
                     got = ((r @ v[:, 0].double()) / total).to(dtype).double()
                     assert bool(((got - out[:, 0]).abs() <= bound[:, 0]).all())
+
+
+@pytest.fixture
+def rope_on_cpu():
+    """The oracle's rotation as the op's CPU kernel, below the op's own derivative formulas."""
+    with torch.library._scoped_library("mi355", "IMPL") as lib:
+        lib.impl("rope", lambda x, *a: serving.rope_ref(x, *a)[0].to(x.dtype), "CPU")
+        yield
+
+
+def _rotation():
+    pos, f = torch.tensor([0, 5, 1000], dtype=I32), ita.rope_inv_freq(12)[0]
+    x, t = (torch.randn(3, 2, 16, dtype=F64) for _ in range(2))
+    return (lambda v: OPS.rope(v, pos, f, True, False, 1.5)), (lambda v: OPS.rope(v, pos, f, True, True, 1.5)), x, t
+
+
+def test_rope_forward_mode(rope_on_cpu):
+    """The tangent is the rotation of the operand's: of tensors with and without requires_grad, without grad mode, and through
+    the gradient."""
+    import torch.autograd.forward_ad as fw
+
+    call, back, x, t = _rotation()
+    with fw.dual_level():
+        for leaf in (x, x.clone().requires_grad_()):
+            y = fw.unpack_dual(call(fw.make_dual(leaf, t)))
+            assert torch.equal(y.tangent, call(t)) and torch.equal(y.primal, call(x))
+        with torch.no_grad():
+            assert torch.equal(fw.unpack_dual(call(fw.make_dual(x, t))).tangent, call(t))
+        assert fw.unpack_dual(call(x)).tangent is None
+        # the gradient's tangent, by one node and by the node of the node
+        leaf = x.clone().requires_grad_()
+        for graph in (False, True):
+            dx, = torch.autograd.grad(call(leaf), leaf, fw.make_dual(x, t), create_graph=graph)
+            assert torch.equal(fw.unpack_dual(dx).tangent, back(t)) and torch.equal(fw.unpack_dual(dx).primal, back(x))
+    assert torch.autograd.gradcheck(call, (x.clone().requires_grad_(),), check_forward_ad=True, check_batched_grad=True)
+    assert torch.autograd.gradgradcheck(call, (x.clone().requires_grad_(),))
+
+
+@pytest.mark.filterwarnings("ignore:There is a performance drop")
+def test_rope_under_torch_func(rope_on_cpu):
+    call, back, x, t = _rotation()
+    torch.testing.assert_close(torch.func.grad(lambda v: (call(v) * t).sum())(x), back(t))
+    y, dy = torch.func.jvp(call, (x,), (t,))
+    assert torch.equal(y, call(x)) and torch.equal(dy, call(t))
+    y, pull = torch.func.vjp(call, x)
+    assert torch.equal(y, call(x)) and torch.equal(pull(t)[0], back(t))
+    many = torch.stack([x, t, x - t])
+    want = torch.stack([call(v) for v in many])
+    assert torch.equal(torch.func.vmap(call)(many), want)
+    torch.testing.assert_close(torch.func.vmap(torch.func.grad(lambda v: (call(v) * t).sum()))(many), back(t).expand(3, 3, 2, 16))
+    assert torch.equal(torch.func.vmap(torch.func.jvp, in_dims=(None, None, 0))(call, (x,), (many,))[1], want)
+    fwd, rev = torch.func.jacfwd(call)(x), torch.func.jacrev(call)(x)
+    torch.testing.assert_close(fwd, rev)
+    torch.testing.assert_close(torch.einsum("abcdef,def->abc", rev, t), call(t))
+    h = torch.func.hessian(lambda v: (call(v) ** 2).sum() / 2)(x)  # R^T R = 1.5^2 on the turned elements
+    torch.testing.assert_close(torch.einsum("abcdef,def->abc", h, t), torch.cat([t[..., :12] * 2.25, t[..., 12:]], -1))
+    leaf = x.clone().requires_grad_()
+    got, = torch.autograd.grad(call(leaf), leaf, many, is_grads_batched=True)
+    assert torch.equal(got, torch.stack([back(v) for v in many]))
