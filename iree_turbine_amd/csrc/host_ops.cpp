@@ -69,9 +69,9 @@ double number(PyObject* o) {
 // Memory that is what the tensor stands for.  (Below the dispatcher every tensor is; the rotation is also called above it,
 // with lazily negated ones, zeros without memory, and the wrappers of torch.func and of tensor subclasses.)
 bool is_plain(const Tensor& t) {
-  static const c10::DispatchKeySet odd({c10::DispatchKey::Negative, c10::DispatchKey::ZeroTensor, c10::DispatchKey::FuncTorchBatched,
+  static const c10::DispatchKeySet odd({c10::DispatchKey::Negative, c10::DispatchKey::ZeroTensor, c10::DispatchKey::FuncTorchBatched, c10::DispatchKey::Batched,
                                         c10::DispatchKey::FuncTorchGradWrapper, c10::DispatchKey::Functionalize, c10::DispatchKey::Python});
-  return t.layout() == at::kStrided && !t.key_set().has_any(odd);
+  return t.layout() == at::kStrided && t.has_storage() && !t.key_set().has_any(odd);
 }
 // All on one device, the current one: the caller of the kernel needs no guard then.
 template <typename... Ts>
