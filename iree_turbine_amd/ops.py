@@ -546,14 +546,6 @@ class rope(CustomOp):
         return launch._rope(dev, x, positions, inv_freq, x.new_empty(x.shape), interleaved, inverse, scale)
 
 
-def _on_device_eagerly(x: Tensor) -> bool:
-    """A plain device tensor outside every dispatch mode: the launch needs no further pass through the dispatcher.  Meta
-    and fake tensors and tracing do, torch.func's wrappers, and lazily negated or zero ones, whose memory is not yet what they
-    stand for."""
-    return type(x) in (Tensor, torch.nn.Parameter) and x.is_cuda and torch._C._len_torch_dispatch_stack() == 0 and not x.is_neg() and not x._is_zerotensor() \
-        and not torch._C._functorch.is_functorch_wrapped_tensor(x)
-
-
 def _has_tangent(x: Tensor) -> bool:
     return forward_ad._current_level >= 0 and forward_ad.unpack_dual(x).tangent is not None
 
@@ -587,13 +579,7 @@ class _RopeGrad(torch.autograd.Function):
     @staticmethod
     def backward(ctx, grad):
         positions, inv_freq = ctx.saved_tensors
-        how = (ctx.interleaved, not ctx.inverse, ctx.scale)
-        if torch.is_grad_enabled() or _has_tangent(grad):
-            dx = torch.ops.mi355.rope(grad, positions, inv_freq, *how)
-        elif _on_device_eagerly(grad):  # its sizes and type are the result's, whose call has been checked
-            dx = launch._rope(grad.device, grad, positions, inv_freq, grad.new_empty(grad.shape), *how)
-        else:
-            dx = _rope_below_autograd(grad, positions, inv_freq, *how)
+        dx = torch.ops.mi355.rope(grad, positions, inv_freq, ctx.interleaved, not ctx.inverse, ctx.scale)
         return dx, None, None, None, None, None
 
     @staticmethod

@@ -248,3 +248,18 @@ def test_rows_past_32_bit_offsets(dev):
     for row, slot in ((0, last - 1), (1, 0), (4, last - 300)):
         _inside(flat_k[slot], want[row], bound[row])
         assert torch.equal(flat_v[slot].cpu(), v[row])
+
+
+def test_gradient_with_lazily_negated_frequencies(dev):
+    """Frequencies that carry torch's negation as a flag turn the gradient the way that their values say."""
+    announce("rope gradient, lazily negated frequencies")
+    pos, f = torch.arange(5, dtype=torch.int32, device=dev) * 3, _freq(64, device=dev)[0]
+    lazy = torch._neg_view(f)
+    assert lazy.is_neg() and lazy.is_contiguous()
+    x, g = (torch.randn(5, 2, 64, device=dev) for _ in range(2))
+    leaf = x.clone().requires_grad_()
+    y, plain = (torch.ops.mi355.rope(leaf, pos, freq, False, False, 1.0) for freq in (lazy, -f))
+    assert torch.equal(y, plain)
+    want, = torch.autograd.grad(plain, leaf, g)
+    assert torch.equal(torch.autograd.grad(y, leaf, g)[0], want)
+    assert not torch.equal(want, torch.ops.mi355.rope(g, pos, f, False, True, 1.0))
