@@ -127,17 +127,13 @@ void check_rope(const Tensor& x, const Tensor& pos, const Tensor& freq) {
   check_angles(pos, freq, T, D);
 }
 
-// the entry's code; `out` as x, contiguous
-int run_rope(const Tensor& x, const Tensor& pos, const Tensor& freq, Tensor& out, bool inter, bool inverse, double scale) {
-  const int64_t xs[2] = {x.stride(0), x.stride(1)}, os[2] = {out.stride(0), out.stride(1)};
-  return entry.rope(x.data_ptr(), out.data_ptr(), (const int32_t*)pos.data_ptr(), freq.data_ptr(), freq.scalar_type() == at::kDouble, x.size(0),
-                    x.size(1), x.size(2), 2 * freq.size(0), xs, os, inter, inverse, (float)scale,
-                    x.scalar_type() == at::kFloat ? MI355_F32 : half_code(x), current_stream(x));
-}
 Tensor rope(const Tensor& x, const Tensor& pos, const Tensor& freq, bool inter, bool inverse, double scale) {
   check_rope(x, pos, freq);
   Tensor out = fresh(x.sizes(), x, x.scalar_type());
-  want(run_rope(x, pos, freq, out, inter, inverse, scale) == 0);
+  const int64_t xs[2] = {x.stride(0), x.stride(1)}, os[2] = {out.stride(0), out.stride(1)};
+  want(entry.rope(x.data_ptr(), out.data_ptr(), (const int32_t*)pos.data_ptr(), freq.data_ptr(), freq.scalar_type() == at::kDouble, x.size(0),
+                  x.size(1), x.size(2), 2 * freq.size(0), xs, os, inter, inverse, (float)scale,
+                  x.scalar_type() == at::kFloat ? MI355_F32 : half_code(x), current_stream(x)) == 0);
   return out;
 }
 
@@ -149,7 +145,7 @@ Tensor rope_by_dispatcher(const Tensor& x, const Tensor& pos, const Tensor& freq
 
 // The gradient as a node of the engine's own kind: its backward pass takes no interpreter lock (a forward and backward pass of a
 // small x: 98 us with the node in Python).  Same formula and same saved tensors as ops._RopeGrad.  Gradients that are to be
-// differentiated, have a tangent, or are no plain tensors go through the op.
+// differentiated, have a tangent, or are no plain tensors go through the op, and so does what a function here does not take.
 struct RopeGrad : torch::autograd::Function<RopeGrad> {
   static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& x, const Tensor& pos, const Tensor& freq, bool inter, bool inverse,
                         double scale) {
@@ -164,13 +160,14 @@ struct RopeGrad : torch::autograd::Function<RopeGrad> {
     const bool inter = ctx->saved_data["inter"].toBool(), inverse = !ctx->saved_data["inverse"].toBool();
     const double scale = ctx->saved_data["scale"].toDouble();
     Tensor g = grads[0], dx;
-    if ((at::GradMode::is_enabled() && g.requires_grad()) || g._fw_grad(0).defined() || !is_plain(g)) {
-      dx = rope_by_dispatcher(g, saved[0], saved[1], inter, inverse, scale);
-    } else {
+    if (!(at::GradMode::is_enabled() && g.requires_grad()) && !g._fw_grad(0).defined() && is_plain(g)) {
       if (g.stride(2) != 1) g = g.contiguous();
-      dx = fresh(g.sizes(), g, g.scalar_type());
-      TORCH_CHECK(run_rope(g, saved[0], saved[1], dx, inter, inverse, scale) == 0, "rope: the gradient's rotation failed: ", entry.last_error());
+      try {
+        dx = rope(g, saved[0], saved[1], inter, inverse, scale);  // (saved-tensor hooks may have put anything in their place)
+      } catch (NotTaken&) {
+      }
     }
+    if (!dx.defined()) dx = rope_by_dispatcher(g, saved[0], saved[1], inter, inverse, scale);
     return {dx, Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
   }
 };

@@ -175,3 +175,26 @@ def test_forward_mode_and_transforms_on_the_device(dev):
     y = call(leaf)
     assert "RopeGrad" in y.grad_fn.name()
     assert torch.equal(torch.autograd.grad(y, leaf, many, is_grads_batched=True)[0], torch.stack([back(v) for v in many]))
+
+
+def test_gradient_of_what_saved_tensor_hooks_give_back(dev):
+    """Positions and frequencies that come back laid out otherwise are read as they are; on the host, of another type or
+    length they are refused, nothing is launched for them."""
+    announce("rope gradient, unpacked tensors")
+    pos, f = torch.arange(6, dtype=torch.int32, device=dev) * 9, ita.rope_inv_freq(64, device=dev)[0]
+    x, g = (torch.randn(6, 3, 96, device=dev) for _ in range(2))
+    leaf = x.clone().requires_grad_()
+
+    def grad(unpack):
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t, unpack):
+            y = OPS.rope(leaf, pos, f, True, False, 2.0)
+        assert y.grad_fn.name() != "_RopeGradBackward"
+        return torch.autograd.grad(y, leaf, g)[0]
+
+    want = OPS.rope(g, pos, f, True, True, 2.0)
+    assert torch.equal(grad(lambda t: t), want)
+    assert torch.equal(grad(lambda t: torch.stack([t, t], -1)[..., 0]), want)
+    assert torch.equal(grad(lambda t: torch._neg_view(-t)), want)
+    for bad in (lambda t: t.cpu(), lambda t: t.to(torch.int64), lambda t: t.repeat(2), lambda t: t[:0]):
+        with pytest.raises((ValueError, RuntimeError, NotImplementedError)):
+            grad(bad)
