@@ -45,6 +45,7 @@ extern "C" {
 #define MI355_E_ALIGN 3     /* a pointer is not aligned as the kernel requires (16 bytes) */
 #define MI355_E_DTYPE 4     /* unknown out_dtype / variant selector */
 #define MI355_E_SCRATCH 5   /* split-K scratch missing or too small */
+#define MI355_E_OVERLAP 6   /* an operand that is written shares memory with another one */
 
 /* output element types */
 #define MI355_F32 0
@@ -425,6 +426,8 @@ int mi355_verify_draft(const float* target_probs, const float* draft_probs, cons
  *   position lies behind the table); padding rows: 0, -1, -1;
  *   pages_needed[0]: pages the step needs (more than num_free: the rest is missing).
  * The pages taken are free_pages[0 .. min(pages_needed, num_free)).  The same call again gives the same results.
+ * Workgroups read the lengths while others write results: what is written (block_table and the outputs) shares no memory with any
+ * other operand (-MI355_E_OVERLAP; seq_lens is not context_lens).
  * page_size 16, 32, 64, 128 or 256; num_seqs <= 65535, num_tokens, num_free <= 2^30.  No counterpart in the reference.
  */
 int mi355_paged_batch_layout(int32_t* block_table, const int32_t* context_lens, const int32_t* new_lens,

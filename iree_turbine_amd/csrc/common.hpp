@@ -179,6 +179,16 @@ int check_launch(const char* kernel, dim3 grid, dim3 block, size_t lds);
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
+// A dense operand's memory.
+struct Extent {
+  const void* at;
+  int64_t bytes;
+};
+inline bool overlap(const Extent& a, const Extent& b) {
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a.at), y = reinterpret_cast<uintptr_t>(b.at);
+  return a.bytes > 0 && b.bytes > 0 && x < y + (uintptr_t)b.bytes && y < x + (uintptr_t)a.bytes;
+}
+
 // Raises a kernel's dynamic-LDS limit, once per device.  The attribute belongs to the (kernel, device) pair
 // and a process may drive several devices, so `done` -- the call site's own record -- holds one bit per device
 // ordinal; ordinals past 63 set the attribute on every launch.

@@ -164,6 +164,13 @@ extern "C" int mi355_paged_batch_layout(int32_t* block_table, const int32_t* con
       num_tokens > (1 << 30) || num_free < 0 || num_free > (1 << 30))
     return fail(-MI355_E_SHAPE, "%s: bad sizes seqs=%lld max_pages=%lld tokens=%lld free=%lld", fn, (long long)num_seqs,
                 (long long)max_pages_per_seq, (long long)num_tokens, (long long)num_free);
+  // the first seven are written
+  const Extent all[10] = {{block_table, num_seqs * max_pages_per_seq * 4}, {seq_lens, num_seqs * 4}, {cu_new, (num_seqs + 1) * 4}, {positions, num_tokens * 4},
+                          {seq_ids, num_tokens * 4}, {slots, num_tokens * 8}, {pages_needed, 4}, {context_lens, num_seqs * 4}, {new_lens, num_seqs * 4},
+                          {free_pages, num_free * 4}};
+  for (int i = 0; i < 7; i++)
+    for (int j = i + 1; j < 10; j++)
+      if (overlap(all[i], all[j])) return fail(-MI355_E_OVERLAP, "%s: block_table and the outputs must not share memory with each other or with an input", fn);
   dim3 grid((unsigned)((num_tokens + PL_ROWS - 1) / PL_ROWS)), block(PL_THREADS);
   hipLaunchKernelGGL(paged_layout_kernel, grid, block, 0, reinterpret_cast<hipStream_t>(stream), block_table, context_lens,
                      new_lens, free_pages, (int)num_free, (int)num_seqs, (int)max_pages_per_seq, page_bits, (int)num_tokens,

@@ -389,3 +389,24 @@ def test_rope_under_torch_func(rope_on_cpu):
     leaf = x.clone().requires_grad_()
     got, = torch.autograd.grad(call(leaf), leaf, many, is_grads_batched=True)
     assert torch.equal(got, torch.stack([back(v) for v in many]))
+
+
+def test_batch_layout_refuses_shared_memory():
+    """Lengths are read by all workgroups while the first writes its results: none of those lies in an operand's memory.  Addresses
+    only; every one of these calls is refused before a launch."""
+    lib = _lib.load()
+    S, W, T, F = 3, 4, 9, 5
+    size = dict(bt=S * W * 4, sl=S * 4, cu=(S + 1) * 4, pos=T * 4, ids=T * 4, slots=T * 8, need=4, ctx=S * 4, new=S * 4, free=F * 4)
+    base = {name: 4096 * (i + 1) for i, name in enumerate(size)}
+
+    def call(**at):
+        a = {**base, **at}
+        return lib.mi355_paged_batch_layout(a["bt"], a["ctx"], a["new"], a["free"], F, S, W, 16, T, a["sl"], a["cu"], a["pos"], a["ids"], a["slots"], a["need"], None)
+
+    written = ["bt", "sl", "cu", "pos", "ids", "slots", "need"]
+    for one in written:
+        for other in size:
+            if one != other:
+                for at in (base[other], base[other] + size[other] - 4, base[other] - size[one] + 4):
+                    assert call(**{one: at}) == -6, (one, other)
+    assert b"share memory" in lib.mi355_last_error()
