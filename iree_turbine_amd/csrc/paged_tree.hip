@@ -190,14 +190,16 @@ __global__ __launch_bounds__(PT_WAVES * 64) __attribute__((amdgpu_waves_per_eu(2
           const float alpha = none_yet ? 1.f : __builtin_amdgcn_exp2f((m_run[c] - m_new) * a.scale_log2e);
           const float mc = none_yet ? 0.f : m_new * a.scale_log2e;
           m_run[c] = m_new;
+          // weights go into the second product in 16 bits, and the sum is that of the rounded ones: their error then is one of
+          // weights that add up to 1, and the same as in the form with more rows
           float psum = 0.f;
 #pragma unroll
-          for (int r = 0; r < 4; r++) {
-            const float p0 = __builtin_amdgcn_exp2f(s0[r] * a.scale_log2e - mc);
-            const float p1 = __builtin_amdgcn_exp2f(s1[r] * a.scale_log2e - mc);
-            psum += p0 + p1;
-            pf[c][r] = cvt16<BF>(p0);
-            pf[c][4 + r] = cvt16<BF>(p1);
+          for (int r = 0; r < 4; r += 2) {
+            const half2v p0 = cvt16x2<BF>(__builtin_amdgcn_exp2f(s0[r] * a.scale_log2e - mc), __builtin_amdgcn_exp2f(s0[r + 1] * a.scale_log2e - mc));
+            const half2v p1 = cvt16x2<BF>(__builtin_amdgcn_exp2f(s1[r] * a.scale_log2e - mc), __builtin_amdgcn_exp2f(s1[r + 1] * a.scale_log2e - mc));
+            psum = dot2_ones<BF>(p1, dot2_ones<BF>(p0, psum));
+            pf[c][r] = p0[0], pf[c][r + 1] = p0[1];
+            pf[c][4 + r] = p1[0], pf[c][5 + r] = p1[1];
           }
           l_run[c] = l_run[c] * alpha + psum;
 #pragma unroll

@@ -213,3 +213,25 @@ def test_two_streams_and_a_capture(dev):
         torch.cuda.synchronize()
         eager = torch.ops.mi355.paged_tree_attn(*ins, par, 0.0, 4)
         assert all(torch.equal(out, eager) for _, out in graphs)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("N,hq,hkv", [(4, 4, 1), (7, 8, 2), (12, 8, 2), (40, 8, 2)], ids=["16 rows", "32 rows", "64 rows", "160 rows"])
+@pytest.mark.parametrize("splits", [1, 2])
+def test_weights_add_up_to_one(dev, splits, N, hq, hkv, dtype):
+    """Equal values come out as they went in, whatever the weights' rounding to 16 bits loses: one key of weight 1 and the
+    others just below the middle between 1/2 and the next 16-bit number, all of which round down."""
+    announce(f"tree equal values N={N} hq={hq} {dtype} splits={splits}")
+    eps = torch.finfo(dtype).eps
+    L = max(32, N + 20)
+    k = torch.zeros(64, hkv, 128, dtype=dtype)
+    k[1:, :, 0], k[1:, :, 1] = -1.0, 0.95 * eps / 2 / 0.6931  # 2^(-1 + d), about 1/2 (1 + 0.95 eps / 2)
+    v = torch.full((64, hkv, 128), 2 - eps, dtype=dtype)
+    q = torch.zeros(1, N, hq, 128, dtype=dtype)
+    q[..., :2] = 1.0
+    table, lens, par = torch.tensor([[0]], dtype=torch.int32), torch.tensor([L], dtype=torch.int32), _parents(1, 1, N, 3)
+    weights = torch.exp2((k[:L, 0, 0] + k[:L, 0, 1]).double())
+    lost = 1 - weights.to(dtype).double().sum() / weights.sum()
+    assert float(lost) > eps / 4  # more than half a step of a value next to 2
+    got = torch.ops.mi355.paged_tree_attn(*(t.to(dev) for t in (q, k[None], v[None], table, lens, par)), 0.6931471805599453, splits)
+    assert torch.equal(got.cpu(), torch.full((1, N, hq, 128), 2 - eps, dtype=dtype))
