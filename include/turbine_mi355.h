@@ -377,12 +377,13 @@ int mi355_paged_prefill_attn_bf16(const void* q, const void* k_cache, const void
  * written, other branches, the rest of the last page).
  * 1 <= num_nodes <= 64, num_q_heads / num_kv_heads <= 128, D == 128, page_size 16, 32, 64,
  * 128 or 256, 1 <= num_splits <= 1024.  A chain (parents[n] = n - 1) is the causal mask among the drafts.
- * num_splits cuts the table's reach into that many chunks, each by its own workgroups; num_splits > 1 needs
+ * num_splits cuts the longest sequence (up to 512 sequences; the table's reach with more) into up to that many chunks of at least
+ * 128 tokens and the others into chunks as long, each by its own workgroups; spare columns of the table change nothing.  num_splits > 1 needs
  * part_acc [num_seqs, num_nodes, num_q_heads, num_splits, D] and part_ml [.., num_splits, 2], fp32, written before they are
  * read in the same call, and at most 2^23 query rows (num_seqs * num_nodes * num_q_heads).  No counterpart in the
  * reference; the mask generalises tests/dynamo/llama_test.py:285-290.
  */
-/* A default for num_splits, from sizes alone. */
+/* A default for num_splits, from sizes alone; scratch and grid grow with it, a table wider than the sequences costs nothing more. */
 int64_t mi355_paged_tree_default_splits(int64_t num_seqs, int64_t num_nodes, int64_t num_q_heads, int64_t num_kv_heads,
                                         int64_t page_size, int64_t max_pages_per_seq);
 int mi355_paged_tree_attn(const void* q, const void* k_cache, const void* v_cache,

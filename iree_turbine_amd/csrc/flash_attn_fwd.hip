@@ -676,7 +676,8 @@ __device__ __forceinline__ bool fa_find_unit(const FaVarlen& vl, int group, int 
 struct FaTree : FaPaged {
   const int* parents;           // [batch][nodes]
   float *part_acc, *part_ml;    // [batch][nodes][query heads][splits][128], [..][2]
-  int nodes, num_kv_heads, num_seqs, row_blocks, num_splits, chunk_tiles;
+  int nodes, num_kv_heads, num_seqs, row_blocks, num_splits;
+  unsigned per_half;
 };
 
 // Measured, causal, the packed forms: 32 prompts of 1 to 300 tokens (32 query heads over 8) 26 us, bound by the
@@ -736,6 +737,7 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
   size_t q_first = 0, k_first = 0;  // (VARLEN) the sequence's first rows
   int seq_q = 0;                    // (VARLEN) its query tokens; Sq counts rows
   int split = 0, first_tile = 0;    // (CHUNKS) the chunk of the keys, and where it begins
+  int chunk_tiles = 0;              // (TREE) tiles of a chunk
   if constexpr (VARLEN) {
     const int pid = blockIdx.x;
     if (pg.zero_rest) {
@@ -777,8 +779,9 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
     const int kvh = pid % pg.num_kv_heads;
     pid /= pg.num_kv_heads;
     unit = pid % pg.row_blocks;
-    if (!tree_item(pg.seq_lens, pg.num_seqs, pg.num_splits, pg.chunk_tiles * 2, (pg.max_pages * 16) << pg.page_shift, pid / pg.row_blocks, b_idx, split))
-      return;
+    const int reach = (pg.max_pages * 16) << pg.page_shift, chunk_steps = tree_chunk_steps(pg.seq_lens, pg.num_seqs, pg.num_splits, pg.per_half, reach);
+    if (!tree_item(pg.seq_lens, pg.num_seqs, pg.num_splits, chunk_steps, reach, pid / pg.row_blocks, b_idx, split)) return;
+    chunk_tiles = chunk_steps / 2;
     h_idx = kvh * lay.group;
     bh = 0;
     Sq = pg.nodes * lay.group;
@@ -827,9 +830,9 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
   if constexpr (TREE) {
     draft0 = Sk - pg.nodes;
     const int tiles = (Sk + FA_BLOCK_N - 1) / FA_BLOCK_N;
-    first_tile = split * pg.chunk_tiles;
+    first_tile = split * chunk_tiles;
     if (first_tile >= tiles && split > 0) return;  // chunk 0 of an empty sequence writes its zeros
-    single = tiles <= pg.chunk_tiles;
+    single = tiles <= chunk_tiles;
     // the ancestors of this block's rows, behind the rings
     unsigned long long* seen = reinterpret_cast<unsigned long long*>(lds + 2 * FA_STAGE);
     if (wave == 0) seen[lane] = tree_ancestors(pg.parents + (size_t)b_idx * pg.nodes, pg.nodes);
@@ -903,7 +906,7 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
   int n_tiles = k_end > 0 ? (k_end + FA_BLOCK_N - 1) / FA_BLOCK_N : 0;
   if constexpr (TREE) {
     n_tiles -= first_tile;
-    n_tiles = n_tiles < pg.chunk_tiles ? n_tiles : pg.chunk_tiles;
+    n_tiles = n_tiles < chunk_tiles ? n_tiles : chunk_tiles;
   } else if constexpr (CHUNKS) {
     const FaChunks ch = fa_chunks(n_tiles, pg.chunks);
     if (split >= ch.count) return;
@@ -2077,7 +2080,7 @@ extern "C" int mi355_paged_prefill_attn_bf16(const void* q, const void* k_cache,
 
 namespace mi355 {
 
-// The tree form's launch: arguments checked by the caller (paged_tree.hip); chunk_steps counts 32-token steps and is even.
+// The tree form's launch: arguments checked by the caller (paged_tree.hip).
 template <bool BF, int QG>
 static int fa_tree_launch(const TreeArgs& a, int num_seqs, hipStream_t stream) {
   auto kern = fa_fwd_d128_m16<false, BF, 4, false, FaForm::TREE, QG>;
@@ -2093,7 +2096,7 @@ static int fa_tree_launch(const TreeArgs& a, int num_seqs, hipStream_t stream) {
   FaTree tr;
   tr.block_table = a.table, tr.seq_lens = a.seq_lens, tr.max_pages = a.max_pages, tr.num_pages = a.num_pages, tr.page_shift = a.page_shift;
   tr.parents = a.parents, tr.part_acc = a.part_acc, tr.part_ml = a.part_ml, tr.nodes = a.nodes, tr.num_kv_heads = a.num_kv_heads;
-  tr.num_seqs = num_seqs, tr.num_splits = a.num_splits, tr.chunk_tiles = a.chunk_steps / 2;
+  tr.num_seqs = num_seqs, tr.num_splits = a.num_splits, tr.per_half = a.per_half;
   tr.row_blocks = (a.nodes * a.group + block_m - 1) / block_m;
   const int64_t wgs = (int64_t)num_seqs * a.num_splits * a.num_kv_heads * tr.row_blocks;
   if (wgs >= (1ll << 24)) return fail(-MI355_E_SHAPE, "paged_tree_attn: too many workgroups");  // 2^32 threads

@@ -13,9 +13,10 @@
 // split the rows and share a tile: with four column groups here every wave read every V fragment for itself, and 64
 // sequences of 512 to 8192 tokens with 64 rows took 317 us, on the TREE form 208 (and 175 with today's order of work).
 //
-// The table's reach is cut into num_splits chunks of equally many 32-token steps; a sequence that fits one chunk writes
-// its result directly, the others write fp32 partials that a second launch merges (two launches wherever the table's reach
-// is cut: the lengths are not known on the host).  Full chunks are handed out before shorter ones, see tree.hpp.
+// The longest sequence is cut into up to num_splits chunks of equally many 32-token steps, the others into chunks as long (see
+// tree_chunk_steps); a sequence that fits one chunk writes its result directly, the others write fp32 partials that a second
+// launch merges (two launches wherever num_splits > 1: the lengths are not known on the host).  Full chunks are handed out before
+// shorter ones, see tree.hpp.
 //
 // Measured, 8 K/V heads: one sequence of 32768 tokens (28 rows, fp16) 33 us, of which the second launch is 5 (the first reads
 // 5.1 TB/s); 64 of 512 to 8192 tokens (64 rows, bf16) 175 us, 4.3 TB/s.  Looking masked steps over for non-finite values is 1
@@ -56,7 +57,8 @@ __global__ __launch_bounds__(PT_WAVES * 64) __attribute__((amdgpu_waves_per_eu(2
   const int reach = (a.max_pages << a.page_shift) * 16;
   const int kvh = blockIdx.x % a.num_kv_heads;
   int seq, split;
-  if (!tree_item(a.seq_lens, a.num_seqs, a.num_splits, a.chunk_steps, reach, blockIdx.x / a.num_kv_heads, seq, split)) return;
+  const int chunk_steps = tree_chunk_steps(a.seq_lens, a.num_seqs, a.num_splits, a.per_half, reach);
+  if (!tree_item(a.seq_lens, a.num_seqs, a.num_splits, chunk_steps, reach, blockIdx.x / a.num_kv_heads, seq, split)) return;
   const int R = a.nodes * a.group;
   const int num_q_heads = a.num_kv_heads * a.group;
 
@@ -64,11 +66,11 @@ __global__ __launch_bounds__(PT_WAVES * 64) __attribute__((amdgpu_waves_per_eu(2
   const int L = L_in < 0 ? 0 : (L_in > reach ? reach : L_in);
   const int draft0 = L - a.nodes;  // position of node 0 (negative: the first nodes are not in the cache)
   const int steps = (L + 31) >> 5;
-  const int s_begin = split * a.chunk_steps;
-  const int s_end = s_begin + a.chunk_steps < steps ? s_begin + a.chunk_steps : steps;
+  const int s_begin = split * chunk_steps;
+  const int s_end = s_begin + chunk_steps < steps ? s_begin + chunk_steps : steps;
   // a chunk behind the sequence's end has nothing to do; chunk 0 of an empty sequence writes its zeros
   if (s_begin >= steps && split > 0) return;
-  const bool single = steps <= a.chunk_steps;
+  const bool single = steps <= chunk_steps;
   const int p_end = (L + 15) >> 4;  // 16-token blocks
   const int n_steps = s_end - s_begin;
 
@@ -329,7 +331,8 @@ __global__ __launch_bounds__(256) void paged_tree_merge_kernel(TreeArgs a, int n
   const int L_in = a.seq_lens[seq];
   const int L = L_in < 0 ? 0 : (L_in > reach ? reach : L_in);
   const int steps = (L + 31) >> 5;
-  const int n = !on || steps <= a.chunk_steps ? 0 : (steps + a.chunk_steps - 1) / a.chunk_steps;
+  const int chunk_steps = tree_chunk_steps(a.seq_lens, a.num_seqs, a.num_splits, a.per_half, reach);
+  const int n = !on || steps <= chunk_steps ? 0 : (steps + chunk_steps - 1) / chunk_steps;
   const float* ml = a.part_ml + (size_t)row * a.num_splits * 2;
   const float* acc = a.part_acc + (size_t)row * a.num_splits * 128 + l32 * 4;
   float m_tot = -INFINITY;
@@ -402,7 +405,7 @@ static int run_tree(TreeArgs a, int num_seqs, hipStream_t stream) {
 
 using namespace mi355;
 
-// Chunks of at least 128 tokens, at most 64, for about so many workgroups: 256 where few (sequence, K/V head, 128 rows) blocks read
+// At most 64 chunks, and no more than a full table has 128-token ones, for about so many workgroups: 256 where few (sequence, K/V head, 128 rows) blocks read
 // long caches on the kernel above, which a workgroup per CU drives at memory's rate (one sequence of 32768 tokens 36 / 31 / 35 us
 // with 128 / 256 / 384 workgroups), 512 where the prefill form does, which needs two per CU (64 rows: 41 / 37 with 256 / 384), or
 // with 20 to 32 blocks; more blocks differ in length, and 1024 in order of their size even that out (64 sequences of
@@ -448,11 +451,9 @@ extern "C" int mi355_paged_tree_attn(const void* q, const void* k_cache, const v
     return fail(-MI355_E_ALIGN, "%s: q, k_cache, v_cache, out must be 16-byte aligned", fn);
   if (num_splits > 1 && (!part_acc || !part_ml)) return fail(-MI355_E_SCRATCH, "%s: num_splits > 1 needs part_acc / part_ml scratch", fn);
   if (num_splits > 1 && !aligned16(part_acc)) return fail(-MI355_E_ALIGN, "%s: part_acc must be 16-byte aligned", fn);
-  const int64_t reach_steps = (max_pages_per_seq * page_size + 31) / 32;
   TreeArgs a{(const half_t*)q, (const half_t*)k_cache, (const half_t*)v_cache, block_table, seq_lens, parents, (half_t*)out,
            part_acc, part_ml, (int)num_kv_heads, (int)(num_q_heads / num_kv_heads), (int)num_nodes, (int)max_pages_per_seq,
-           (int)num_pages, page_shift, (int)num_splits, (int)((reach_steps + 2 * num_splits - 1) / (2 * num_splits)) * 2,
-           (int)num_seqs, scale * 1.4426950408889634f};
+           (int)num_pages, page_shift, (int)num_splits, (int)num_seqs, tree_per_half(num_splits), scale * 1.4426950408889634f};
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   return dtype == MI355_BF16 ? run_tree<true>(a, (int)num_seqs, s) : run_tree<false>(a, (int)num_seqs, s);
 }

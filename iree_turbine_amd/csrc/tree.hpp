@@ -11,8 +11,9 @@ struct TreeArgs {
   const int *table, *seq_lens, *parents;
   half_t* out;
   float *part_acc, *part_ml;  // [S, N, Hq, splits, 128] and [.., 2]
-  int num_kv_heads, group, nodes, max_pages, num_pages, page_shift, num_splits, chunk_steps;
+  int num_kv_heads, group, nodes, max_pages, num_pages, page_shift, num_splits;
   int num_seqs;
+  unsigned per_half;  // see tree_chunk_steps
   float scale_log2e;
 };
 
@@ -63,6 +64,42 @@ __device__ __forceinline__ float tree_value(unsigned bits) {
   return BF ? __builtin_bit_cast(float, bits << 16) : (float)__builtin_bit_cast(half_t, (unsigned short)bits);
 }
 
+// Chunks: 32-token steps in each, the same number in every workgroup and in the merge; even, and at least 128 tokens.  The longest
+// sequence's steps over num_splits, not the block table's: a server's table is as wide as its longest context may get, and where
+// its columns were cut (32 chunks of 131072) a sequence of 4096 tokens was one chunk on eight workgroups (56 us; 17 by its length).
+// Above 512 sequences, where looking at every length would take longer than a chunk, the table's width.
+constexpr int TREE_LENGTHS = 512;
+__device__ __forceinline__ int tree_chunk_steps(const int* seq_lens, int num_seqs, int num_splits, unsigned per_half, int reach) {
+  int longest = reach;
+  if (num_splits > 1 && num_seqs <= TREE_LENGTHS) {
+    int len = 0;
+    if (num_seqs == 1) {
+      len = seq_lens[0];
+    } else {
+      const int lane = threadIdx.x & 63;
+      len = lane < num_seqs ? seq_lens[lane] : 0;  // (the load that tree_item needs too)
+      for (int s = lane + 64; s < num_seqs; s += 64) {
+        const int l = seq_lens[s];
+        len = l > len ? l : len;
+      }
+      auto with = [&](int l) { len = l > len ? l : len; };  // (lanes without a partner keep their own)
+      with(__builtin_amdgcn_update_dpp(len, len, 0x111, 0xF, 0xF, false));  // row_shr:1, 2, 4, 8: lane 15 of each row has the row's
+      with(__builtin_amdgcn_update_dpp(len, len, 0x112, 0xF, 0xF, false));
+      with(__builtin_amdgcn_update_dpp(len, len, 0x114, 0xF, 0xF, false));
+      with(__builtin_amdgcn_update_dpp(len, len, 0x118, 0xF, 0xF, false));
+      with(__builtin_amdgcn_update_dpp(len, len, 0x142, 0xF, 0xF, false));  // row_bcast:15, 31: lane 63 has all
+      with(__builtin_amdgcn_update_dpp(len, len, 0x143, 0xF, 0xF, false));
+      len = __builtin_amdgcn_readlane(len, 63);
+    }
+    len = len > 0 ? len : 0;
+    longest = len < reach ? len : reach;
+  }
+  // per_half = ceil(2^32 / (2 num_splits)): the quotient's whole part, or one more, which only makes chunks longer
+  const int each = 2 * (int)__umulhi((unsigned)(((longest + 31) >> 5) + 2 * num_splits - 1), per_half);
+  return each < 4 ? 4 : each;
+}
+inline unsigned tree_per_half(int64_t num_splits) { return (unsigned)(((1ll << 32) + 2 * num_splits - 1) / (2 * num_splits)); }
+
 // Piece of work number `item` of a call whose sequences are cut into chunks of `chunk_steps` 32-token steps: its sequence and chunk;
 // false behind the last.  Up to 64 sequences (one per lane, every wave by itself): all full chunks first, then the
 // sequences' last chunks, the longest first, so that the short ones make up the tail.  Nothing empty lies between: workgroups
@@ -94,7 +131,7 @@ __device__ __forceinline__ bool tree_item(const int* seq_lens, int num_seqs, int
   return true;
 }
 
-// The prefill kernel's tree form (flash_attn_fwd.hip): 64 or 128 query rows per workgroup.  chunk_steps even.
+// The prefill kernel's tree form (flash_attn_fwd.hip): 64 or 128 query rows per workgroup.
 int fa_tree(const TreeArgs& a, int num_seqs, bool bf16, hipStream_t stream);
 
 }  // namespace mi355

@@ -672,8 +672,8 @@ class paged_tree_attn(CustomOp):
     tokens of the cache (seq_lens int32 [S] counts them); parents int32 [S, N] (a value outside [0, n) for node n: a root).
     Node n sees every token in front of the drafts, its ancestors and itself; with parents[n] = n - 1 this is
     paged_prefill_attn of N new tokens.  What a node does not see does not reach it, whatever it holds (padding may stay
-    unwritten).  num_kv_splits <= 0 picks a default from the table width; scale <= 0 selects 1/sqrt(D).  Returns
-    [S, N, Hq, 128]."""
+    unwritten).  Keys are cut into up to num_kv_splits chunks of the longest sequence (<= 0 picks a default; a table wider than the
+    sequences need costs nothing, up to 512 of them); scale <= 0 selects 1/sqrt(D).  Returns [S, N, Hq, 128]."""
 
     host = "paged_tree_attn"
     signature = "paged_tree_attn(Tensor q, Tensor k_cache, Tensor v_cache, Tensor block_table, Tensor seq_lens, Tensor parents, float scale, int num_kv_splits) -> Tensor"

@@ -235,3 +235,36 @@ def test_weights_add_up_to_one(dev, splits, N, hq, hkv, dtype):
     assert float(lost) > eps / 4  # more than half a step of a value next to 2
     got = torch.ops.mi355.paged_tree_attn(*(t.to(dev) for t in (q, k[None], v[None], table, lens, par)), 0.6931471805599453, splits)
     assert torch.equal(got.cpu(), torch.full((1, N, hq, 128), 2 - eps, dtype=dtype))
+
+
+@pytest.mark.parametrize("N,hq,hkv", [(4, 4, 2), (7, 8, 2), (12, 8, 2), (40, 8, 2)], ids=["16 rows", "32 rows", "64 rows", "160 rows"])
+@pytest.mark.parametrize("lens", [[1300], [700, 0, 64, 1200, 33], [100, 900] + [70] * 68], ids=["one", "five", "seventy"])
+def test_spare_columns_change_nothing(dev, lens, N, hq, hkv):
+    """Keys are cut by the longest sequence: a block table with room for far longer ones gives the same bits, for any number of
+    chunks, and cuts as finely."""
+    announce(f"tree wide table N={N} hq={hq} sequences={len(lens)}")
+    ins = _inputs(N, lens, N, hq, hkv, 16, torch.bfloat16)
+    par = _parents(N, len(lens), N, 3)
+    wide = torch.full((len(lens), 3000), -1, dtype=torch.int32)
+    wide[:, : ins[3].shape[1]] = ins[3]
+    whole = _check(dev, ins, par, 1)
+    for splits in (2, 3, 16):
+        a = _check(dev, ins, par, splits)
+        assert torch.equal(a, _check(dev, (*ins[:3], wide, ins[4]), par, splits))
+        assert not torch.equal(a, whole)
+    # lengths wilder than either table's reach are cut to it
+    wild = torch.where(ins[4] == max(lens), torch.tensor(2**31 - 1, dtype=torch.int32), ins[4])
+    tame = torch.where(ins[4] == max(lens), torch.tensor(ins[3].shape[1] * 16, dtype=torch.int32), ins[4])
+    clean = [torch.nan_to_num(c, 0.0).to(dev) for c in ins[1:3]]
+    a, b = (torch.ops.mi355.paged_tree_attn(ins[0].to(dev), *clean, ins[3].to(dev), s.to(dev), par.to(dev), 0.0, 4) for s in (wild, tame))
+    assert torch.equal(a, b)
+
+
+def test_more_sequences_than_lengths_are_looked_at(dev):
+    """From 513 sequences on the table's width is cut."""
+    announce("tree 513 and 512 sequences")
+    rng = random.Random(1)
+    for S in (512, 513):
+        lens = [rng.choice([0, 1, 5, 40, rng.randrange(200)]) for _ in range(S)]
+        lens[7] = 300
+        _check(dev, _inputs(S, lens, 3, 2, 1, 16, torch.float16), _parents(S, S, 3, 2), 3)
