@@ -9,11 +9,13 @@
 // its message.  So the contract stays where it is (contract.py), and the tests here only have to be as strict.
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/accumulate_grad.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <ATen/ATen.h>
 #include <ATen/core/dispatch/Dispatcher.h>
 #include <c10/hip/HIPFunctions.h>
+#include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
 
 #include <cmath>
@@ -143,6 +145,19 @@ Tensor rope_by_dispatcher(const Tensor& x, const Tensor& pos, const Tensor& freq
   return op.call(x, pos, freq, inter, inverse, scale);
 }
 
+// A leaf's gradient goes on to its accumulator, on the stream that was current when the accumulator was made.  It lives as long
+// as a graph of the leaf does: with an eager one alive that is the default stream, which cannot wait for a stream under capture, and
+// the engine's attempt may end the process.  Refused here, before it.
+void refuse_capture_beside_eager_graph() {
+  const auto node = torch::autograd::get_current_node();
+  if (!node || node->num_outputs() == 0) return;
+  auto* leaf = dynamic_cast<torch::autograd::AccumulateGrad*>(node->next_edge(0).function.get());
+  if (!leaf || c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) return;
+  const auto stream = leaf->stream();
+  TORCH_CHECK(!stream || stream->id() != 0, "rope: a backward pass under capture while a graph of the same leaf, made on the default stream, is alive; "
+              "delete that graph (its outputs) before the capture, or make it on another stream");
+}
+
 // The gradient as a node of the engine's own kind: its backward pass takes no interpreter lock (a forward and backward pass of a
 // small x: 98 us with the node in Python).  Same formula and same saved tensors as ops._RopeGrad.  Gradients that are to be
 // differentiated, have a tangent, or are no plain tensors go through the op, and so does what a function here does not take.
@@ -156,6 +171,7 @@ struct RopeGrad : torch::autograd::Function<RopeGrad> {
     return rope(x, pos, freq, inter, inverse, scale);
   }
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
+    refuse_capture_beside_eager_graph();
     const auto saved = ctx->get_saved_variables();
     const bool inter = ctx->saved_data["inter"].toBool(), inverse = !ctx->saved_data["inverse"].toBool();
     const double scale = ctx->saved_data["scale"].toDouble();

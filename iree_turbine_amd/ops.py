@@ -524,7 +524,8 @@ class rope(CustomOp):
     and head strides) turned by positions[token] * inv_freq[i], times `scale`; elements from R on pass through.  Pair i is
     (2i, 2i + 1) when `interleaved`, else (i, i + R/2).  positions int32 [tokens]; inv_freq float64 or float32 (see
     `rope_inv_freq`): angles are formed in 64 bits either way.  `inverse` turns back (times `scale`, not divided by it): the
-    gradient, which autograd takes for x; positions and inv_freq get none."""
+    gradient, which autograd takes for x (in reverse and forward mode, any number of times, and under torch.func); positions and
+    inv_freq get none.  A backward pass under capture is refused while a graph of the same leaf x, made on the default stream, lives."""
 
     host = "rope"
     signature = "rope(Tensor x, Tensor positions, Tensor inv_freq, bool interleaved, bool inverse, float scale) -> Tensor"

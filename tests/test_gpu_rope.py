@@ -263,3 +263,30 @@ def test_gradient_with_lazily_negated_frequencies(dev):
     want, = torch.autograd.grad(plain, leaf, g)
     assert torch.equal(torch.autograd.grad(y, leaf, g)[0], want)
     assert not torch.equal(want, torch.ops.mi355.rope(g, pos, f, False, True, 1.0))
+
+
+def test_backward_captured_beside_an_eager_graph_of_the_same_leaf(dev):
+    """Refused while an eager graph of the leaf is alive: its accumulator works on the default stream, which cannot wait for a
+    captured one.  Without it the captured pass replays what the eager one gives."""
+    announce("rope backward captured, eager graph alive")
+    pos, f = torch.arange(9, dtype=torch.int32, device=dev) * 31, _freq(64, device=dev)[0]
+    leaf, g = torch.randn(9, 2, 64, device=dev, requires_grad=True), torch.randn(9, 2, 64, device=dev)
+    call = lambda: torch.ops.mi355.rope(leaf, pos, f, False, False, 1.0)
+    alive = call()
+    torch.cuda.synchronize()
+    with pytest.raises(RuntimeError, match="under capture while a graph of the same leaf"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            torch.autograd.grad(call(), leaf, g)
+    torch.cuda.synchronize()
+    want, = torch.autograd.grad(alive, leaf, g)
+    del alive
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got, = torch.autograd.grad(call(), leaf, g)
+    for k in range(3):
+        g.copy_(torch.randn(9, 2, 64))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got, torch.ops.mi355.rope(g, pos, f, False, True, 1.0))
+        assert torch.equal(got, torch.autograd.grad(call(), leaf, g)[0])
+    assert want.shape == got.shape
