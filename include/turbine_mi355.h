@@ -176,6 +176,7 @@ int mi355_flash_attn_fwd_strided_bf16(const void* q, const void* k, const void* 
  * Rows of o outside every sequence are left as they are; with zero_rest != 0 those in front of the first and behind
  * the last sequence are set to zero.  total_q, total_k <= 2^24, total_q * H / Hkv <= 2^30, num_seqs <= 65535.
  * With the mask, keys and values that a query does not see do not reach it, whatever they hold (NaN and infinities too).
+ * Scores, maxima, sums and accumulators are in 32 bits; weights are rounded to dtype before the second product.
  * Calls with few query rows and many keys cut the keys into chunks and join their results in a second launch: that takes the
  * workspace that mi355_flash_attn_varlen_workspace_bytes names (0: none wanted), scratch that is written before it is read
  * in the same call; without one, or with a smaller one, the call runs uncut.  16-byte aligned.
@@ -373,6 +374,7 @@ int mi355_paged_prefill_attn_bf16(const void* q, const void* k_cache, const void
  * seq_lens:    [num_seqs] int32, cut to [0, max_pages_per_seq * page_size]; shorter than num_nodes: the first nodes are not
  *              in the cache and nobody sees them
  * parents:     [num_seqs, num_nodes] int32; a value outside [0, n) for node n: it has no ancestors (a root)
+ * Scores, maxima, sums and accumulators are in 32 bits; weights are rounded to dtype before the second product.
  * A query that sees nothing gives zeros; what it does not see does not reach it, whatever is there (drafts that were never
  * written, other branches, the rest of the last page).
  * 1 <= num_nodes <= 64, num_q_heads / num_kv_heads <= 128, D == 128, page_size 16, 32, 64,

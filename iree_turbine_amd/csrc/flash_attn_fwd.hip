@@ -680,10 +680,11 @@ struct FaTree : FaPaged {
   unsigned per_half;
 };
 
-// Measured, causal, the packed forms: 32 prompts of 1 to 300 tokens (32 query heads over 8) 26 us, bound by the
-// workgroups' fixed cost (offsets, query rows and first tiles, one after the other: a single prompt of 16 tokens takes 6.6 us,
-// an empty launch 3.6); 12 of 100 to 700 tokens behind up
-// to 1500 (16 heads over one) 41 us; 4 of 1500 to 8192 1.07 to 1.11 ms, 1.02 to 1.06 PFLOP/s, the rate of the rectangular form.
+// Measured, causal, the packed forms: 32 prompts of 1 to 300 tokens (32 query heads over 8) 26 us (744 workgroups of 1 to 5 tiles
+// on 512 places; a single prompt of 16 tokens takes 6.6, an empty launch 3.6); 12 of 100 to 700 tokens behind up to 1500 (16 heads
+// over one) 40 us, bound by LDS reads: the waves of a 64-row block split its rows and read every tile whole, 0.85 us a tile, the
+// longest blocks 31 of them; 4 of 1500 to 8192 1.08 to 1.13 ms, 1.0 to 1.05 PFLOP/s, the rate of the rectangular form.
+// Weights enter the second product in 16 bits; the sum that normalises them is that of the rounded ones.
 enum class FaForm { PLAIN, PAGED, VARLEN, CHUNKED, TREE };  // CHUNKED: VARLEN with keys cut into chunks
 template <FaForm F>
 using FaFormArgs = std::conditional_t<F == FaForm::VARLEN || F == FaForm::CHUNKED, FaVarlen, std::conditional_t<F == FaForm::TREE, FaTree, FaPaged>>;
