@@ -177,7 +177,10 @@ def host_ops():
             if not HOST_PATH.exists():
                 raise KernelLibraryError(f"{HOST_PATH} is missing: build it with `python -m iree_turbine_amd.build`")
             loader = importlib.machinery.ExtensionFileLoader(HOST_PATH.stem, str(HOST_PATH))
-            host = importlib.util.module_from_spec(importlib.util.spec_from_loader(HOST_PATH.stem, loader))
+            try:
+                host = importlib.util.module_from_spec(importlib.util.spec_from_loader(HOST_PATH.stem, loader))
+            except ImportError as e:  # its symbols are those of the torch that it was built against
+                raise KernelLibraryError(f"{HOST_PATH} does not load beside torch {torch.__version__}: build it again with `python -m iree_turbine_amd.build` ({e})") from e
             host.bind(*(ctypes.cast(getattr(lib, name), c_void_p).value for name in _HOST_ENTRIES))
             _host = host
     return _host

@@ -198,3 +198,13 @@ def test_gradient_of_what_saved_tensor_hooks_give_back(dev):
     for bad in (lambda t: t.cpu(), lambda t: t.to(torch.int64), lambda t: t.repeat(2), lambda t: t[:0]):
         with pytest.raises((ValueError, RuntimeError, NotImplementedError)):
             grad(bad)
+
+
+@pytest.mark.parametrize("name", ["rope", "rope_kv_append", "paged_batch_layout", "flash_attn_varlen_fwd", "paged_tree_attn", "verify_draft"])
+def test_registered_as_torch_expects(dev, name):
+    """Schemas say what is written, fake tensors describe the results, and compiled calls with their gradients give the eager ones'."""
+    announce(f"opcheck {name}")
+    args = _calls(dev)[name]
+    torch.library.opcheck(getattr(OPS, name).default, args)
+    if name == "rope":
+        torch.library.opcheck(OPS.rope.default, (args[0].clone().requires_grad_(), *args[1:]))

@@ -410,3 +410,12 @@ def test_batch_layout_refuses_shared_memory():
                 for at in (base[other], base[other] + size[other] - 4, base[other] - size[one] + 4):
                     assert call(**{one: at}) == -6, (one, other)
     assert b"share memory" in lib.mi355_last_error()
+
+
+def test_host_side_of_another_torch_is_an_error(monkeypatch, tmp_path):
+    """A library that does not load (other symbols than this torch's, or no library at all) says what to do."""
+    (tmp_path / "mi355_host_ops.so").write_bytes(b"not a library")
+    monkeypatch.setattr(_lib, "_host", None)
+    monkeypatch.setattr(_lib, "HOST_PATH", tmp_path / "mi355_host_ops.so")
+    with pytest.raises(_lib.KernelLibraryError, match="build it again"):
+        _lib.host_ops()
