@@ -208,3 +208,41 @@ def test_registered_as_torch_expects(dev, name):
     torch.library.opcheck(getattr(OPS, name).default, args)
     if name == "rope":
         torch.library.opcheck(OPS.rope.default, (args[0].clone().requires_grad_(), *args[1:]))
+
+
+def test_limits_are_those_of_the_contract(dev):
+    """One past each limit of sizes: the native side leaves the call, and the op's own contract refuses it.  Broadcast operands stand
+    for large ones; nothing is launched."""
+    announce("host ops limits")
+    h = lambda *s, dt=torch.float16: torch.zeros(1, dtype=dt, device=dev).expand(*s) if len(s) else None
+    flat = lambda *s, dt=torch.int32: torch.zeros(*s, dtype=dt, device=dev)
+    f64, i64 = torch.float64, torch.int64
+    f = lambda n: flat(n, dt=f64)
+    rows = lambda t, heads: torch.zeros(1, heads, 128, dtype=torch.float16, device=dev).expand(t, heads, 128)
+    kc = flat(4, 16, 2, 128, dt=torch.float16)
+    table, lens = flat(2, 4), flat(2)
+    rope = lambda **k: ("rope", *{**dict(x=flat(4, 2, 64, dt=torch.float16), pos=flat(4), f=f(32), i=False, v=False, s=1.0), **k}.values())
+    append = lambda **k: ("rope_kv_append", *{**dict(q=rows(4, 4), k=rows(4, 2), v=rows(4, 2), pos=flat(4), f=f(64), kc=kc, vc=kc.clone(), slots=flat(4, dt=i64), i=False, s=1.0), **k}.values())
+    layout = lambda **k: ("paged_batch_layout", *{**dict(t=table, c=lens, n=lens, fr=flat(3), p=16, T=5), **k}.values())
+    varlen = lambda **k: ("flash_attn_varlen_fwd", *{**dict(q=rows(4, 4), k=rows(4, 2), v=rows(4, 2), cq=flat(3), ck=flat(3), causal=True, s=0.0), **k}.values())
+    tree = lambda **k: ("paged_tree_attn", *{**dict(q=flat(2, 3, 4, 128, dt=torch.float16), kc=kc, vc=kc, t=table, l=lens, p=flat(2, 3), s=0.0, n=0), **k}.values())
+    verify = lambda **k: ("verify_draft", *{**dict(p=flat(2, 3, 9, dt=torch.float32), d=None, t=flat(2, 3), a=flat(2, 3), u=flat(2, 3, dt=torch.float32)), **k}.values())
+    many = 1 << 24
+    calls = [
+        rope(x=h(many, 1, 2), pos=flat(many), f=f(1)), rope(x=h(1, 65536, 2), pos=flat(1), f=f(1)), rope(x=h(1, 1, 65537), pos=flat(1), f=f(1)),
+        rope(x=h(1, 1, 1100), pos=flat(1), f=f(513)), rope(f=f(33)), rope(x=h(1, 20000, 60000), pos=flat(1), f=f(1)),
+        append(q=rows(many, 1), k=rows(many, 2), v=rows(many, 2), pos=flat(many), slots=flat(many, dt=i64)), append(q=rows(4, 65536)), append(f=f(65)),
+        append(kc=flat(4, 8, 2, 128, dt=torch.float16), vc=flat(4, 8, 2, 128, dt=torch.float16)),
+        layout(t=flat(65536, 1), c=flat(65536), n=flat(65536)), layout(t=flat(1, (1 << 22) + 1), c=flat(1), n=flat(1)), layout(T=(1 << 30) + 1), layout(T=0), layout(p=512),
+        varlen(q=rows(many + 1, 2)), varlen(k=rows(many + 1, 2), v=rows(many + 1, 2)), varlen(q=rows(4, 65536)), varlen(q=rows(many, 130)), varlen(cq=flat(65537), ck=flat(65537)),
+        varlen(cq=flat(1), ck=flat(1)),
+        tree(q=flat(2, 65, 4, 128, dt=torch.float16), p=flat(2, 65)), tree(q=flat(2, 3, 258, 128, dt=torch.float16)), tree(n=1025), tree(t=flat(2, 0)),
+        verify(p=flat(65536, 1, 1, dt=torch.float32), t=flat(65536, 1), a=flat(65536, 1), u=flat(65536, 1, dt=torch.float32)),
+        verify(p=flat(1, 65, 1, dt=torch.float32), t=flat(1, 65), a=flat(1, 65), u=flat(1, 65, dt=torch.float32)),
+        verify(p=flat(1, 1, many + 1, dt=torch.float32), t=flat(1, 1), a=flat(1, 1), u=flat(1, 1, dt=torch.float32)),
+    ]
+    for name, *args in calls:
+        sizes = [tuple(a.shape) if isinstance(a, torch.Tensor) else a for a in args]
+        assert getattr(_lib.host_ops(), name)(*args) is None, (name, sizes)
+        with pytest.raises(ValueError):
+            getattr(OPS, name)(*args)
