@@ -14,6 +14,7 @@
 
 #include <ATen/ATen.h>
 #include <ATen/core/dispatch/Dispatcher.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPFunctions.h>
 #include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
@@ -160,7 +161,8 @@ void refuse_capture_beside_eager_graph() {
 
 // The gradient as a node of the engine's own kind: its backward pass takes no interpreter lock (a forward and backward pass of a
 // small x: 98 us with the node in Python).  Same formula and same saved tensors as ops._RopeGrad.  Gradients that are to be
-// differentiated, have a tangent, or are no plain tensors go through the op, and so does what a function here does not take.
+// differentiated, have a tangent, are no plain tensors or meet a dispatch mode go through the op, and so does what a function
+// here does not take.
 struct RopeGrad : torch::autograd::Function<RopeGrad> {
   static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& x, const Tensor& pos, const Tensor& freq, bool inter, bool inverse,
                         double scale) {
@@ -176,7 +178,7 @@ struct RopeGrad : torch::autograd::Function<RopeGrad> {
     const bool inter = ctx->saved_data["inter"].toBool(), inverse = !ctx->saved_data["inverse"].toBool();
     const double scale = ctx->saved_data["scale"].toDouble();
     Tensor g = grads[0], dx;
-    if (!(at::GradMode::is_enabled() && g.requires_grad()) && !g._fw_grad(0).defined() && is_plain(g)) {
+    if (!(at::GradMode::is_enabled() && g.requires_grad()) && !g._fw_grad(0).defined() && is_plain(g) && !c10::impl::TorchDispatchModeTLS::any_modes_set()) {
       if (g.stride(2) != 1) g = g.contiguous();
       try {
         dx = rope(g, saved[0], saved[1], inter, inverse, scale);  // (saved-tensor hooks may have put anything in their place)

@@ -246,3 +246,31 @@ def test_limits_are_those_of_the_contract(dev):
         assert getattr(_lib.host_ops(), name)(*args) is None, (name, sizes)
         with pytest.raises(ValueError):
             getattr(OPS, name)(*args)
+
+
+def test_dispatch_modes_see_the_gradient(dev):
+    """A dispatch mode that is entered for the backward pass alone sees the gradient's call as it sees the forward's."""
+    from torch.utils._python_dispatch import TorchDispatchMode
+
+    announce("rope gradient under a dispatch mode")
+
+    class Names(TorchDispatchMode):
+        def __init__(self):
+            super().__init__()
+            self.seen = []
+
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            self.seen.append(str(func))
+            return func(*args, **(kwargs or {}))
+
+    pos, f = torch.arange(4, dtype=torch.int32, device=dev), ita.rope_inv_freq(64, device=dev)[0]
+    leaf, g = torch.randn(4, 2, 64, device=dev, requires_grad=True), torch.randn(4, 2, 64, device=dev)
+    with Names() as forward:
+        y = OPS.rope(leaf, pos, f, False, False, 1.0)
+    assert "mi355.rope.default" in forward.seen
+    y = OPS.rope(leaf, pos, f, False, False, 1.0)
+    assert y.grad_fn.name() != "_RopeGradBackward"
+    with Names() as backward:
+        got, = torch.autograd.grad(y, leaf, g)
+    assert "mi355.rope.default" in backward.seen
+    assert torch.equal(got, OPS.rope(g, pos, f, False, True, 1.0))
