@@ -67,7 +67,8 @@ __device__ __forceinline__ float tree_value(unsigned bits) {
 // Chunks: 32-token steps in each, the same number in every workgroup and in the merge; even, and at least 128 tokens.  The longest
 // sequence's steps over num_splits, not the block table's: a server's table is as wide as its longest context may get, and where
 // its columns were cut (32 chunks of 131072) a sequence of 4096 tokens was one chunk on eight workgroups (56 us; 17 by its length).
-// Above 512 sequences, where looking at every length would take longer than a chunk, the table's width.
+// Above 512 sequences the table's width: a workgroup would look at lengths longer than that saves (1024 sequences of 100 tokens in
+// two chunks 30.5 us by length, 22.4 by the table; 4096 of 600 499 and 234; the default is one chunk there).
 constexpr int TREE_LENGTHS = 512;
 __device__ __forceinline__ int tree_chunk_steps(const int* seq_lens, int num_seqs, int num_splits, unsigned per_half, int reach) {
   int longest = reach;
@@ -78,9 +79,12 @@ __device__ __forceinline__ int tree_chunk_steps(const int* seq_lens, int num_seq
     } else {
       const int lane = threadIdx.x & 63;
       len = lane < num_seqs ? seq_lens[lane] : 0;  // (the load that tree_item needs too)
-      for (int s = lane + 64; s < num_seqs; s += 64) {
-        const int l = seq_lens[s];
-        len = l > len ? l : len;
+      if (num_seqs > 64) {  // all loads at once; lanes behind the last sequence take its length again
+#pragma unroll
+        for (int s = 64; s < TREE_LENGTHS; s += 64) {
+          const int l = seq_lens[s + lane < num_seqs ? s + lane : num_seqs - 1];
+          len = l > len ? l : len;
+        }
       }
       auto with = [&](int l) { len = l > len ? l : len; };  // (lanes without a partner keep their own)
       with(__builtin_amdgcn_update_dpp(len, len, 0x111, 0xF, 0xF, false));  // row_shr:1, 2, 4, 8: lane 15 of each row has the row's
